@@ -85,6 +85,12 @@ extern "C" {
                                reference's Pade approximant on its 8-wide vector part and exact
                                tanh on the flat tail of (M*N) % 8 elements, src/core/ops.zig:1947-1998 */
 
+/* Element types of the serving operators (below). */
+#define TML_TYPE_F32 0
+#define TML_TYPE_F16 1
+#define TML_TYPE_BF16 2
+#define TML_TYPE_I8 3 /* two's complement, with fp32 scales */
+
 /* ---------------------------------------------------------------- setup */
 
 /* Selects the current HIP device and creates the library's stream.  Called
@@ -364,6 +370,131 @@ int tml_hip_prepared_free(tml_prepared_t w);
  * (residual and activation after the bias). */
 int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const float *bias, const float *residual,
                              int act, float *C, float alpha, float beta, void *stream);
+
+/* ---------------------------------------------------- serving operators
+ * What a decoder step needs around its products, without the host in
+ * between: block tables and slot maps from request lengths, new keys and
+ * values to their slots, attention over the paged cache, the norm that
+ * feeds a product, and the product with 4-bit weights and group scales.  No
+ * counterpart in the reference (its cache is one contiguous run a request,
+ * src/core/cache.zig:1-30, on the host).
+ *
+ * All pointers are device pointers, all calls asynchronous on `stream` (a
+ * hipStream_t, NULL = the null stream), strides count elements unless said
+ * otherwise.  Sums, maxima, softmax statistics and norms are fp32; an output
+ * of fewer bits is rounded once, to nearest even.  The results do not depend
+ * on the order in which workgroups run.  A tensor is read and written inside
+ * the call's stream order only: on another stream than its maker's, order
+ * the streams first.  tml_hip_paged_attention_dev takes the device's
+ * workspace, with the rules of tml_hip_gemm_dev (grown on first use, refused
+ * while captured, one stream at a time); the others need none and can be
+ * captured at once. */
+
+/* Block tables and slot maps.  Request r has ctx_len[r] tokens in the cache
+ * and new_len[r] coming (a negative length counts as 0).  With B =
+ * block_size, its table row (at block_table + r * table_stride, table_width
+ * entries) holds the blocks of its first ceil(ctx_len / B) * B positions; the
+ * call appends the blocks it needs up to ceil((ctx_len + new_len) / B), in
+ * request order from free_blocks[0 .. n_free), and gives every new token,
+ * request after request, its slot block * B + position % B.
+ *   slots          [max_tokens] slot of each new token; -1 where it has none:
+ *                  the free list or the table row ended, the row's entry was
+ *                  negative, or there is no such token (padding)
+ *   token_request  [max_tokens] its request, positions [max_tokens] its
+ *                  position there; -1 for padding
+ *   seq_len        [requests] ctx_len + new_len
+ *   query_start    [requests + 1] first token of each request, then the sum
+ *   totals         [3] new tokens, blocks taken from the free list (more
+ *                  than n_free: the rest got -1), requests whose length does
+ *                  not fit table_width (their row takes what fits)
+ * The outputs after `slots` may be NULL.  If totals[0] exceeds max_tokens the
+ * plan is incomplete: tokens past it were neither mapped nor given blocks. */
+int tml_hip_kv_plan_dev(int64_t requests, int64_t block_size, const int *ctx_len, const int *new_len,
+                        const int *free_blocks, int64_t n_free, int *block_table, int64_t table_width,
+                        int64_t table_stride, int64_t max_tokens, int64_t *slots, int *token_request, int *positions,
+                        int *seq_len, int *query_start, int64_t *totals, void *stream);
+
+/* New keys and values to their slots: element d of head h of token t, at
+ * k + t * k_stride + h * head_dim + d (type `type`: F32, F16 or BF16), goes,
+ * converted to cache_type, to
+ *   k_cache + (slot / block_size) * block_stride + (slot % block_size) * token_stride + h * head_stride + d
+ * with slot = slots[t]; v alike, the caches having the same strides.  The
+ * strides say whether tokens or heads come first in a block.  A slot that is
+ * negative or not below n_blocks * block_size is skipped.  Two tokens with the
+ * same slot: one of them is stored, either. */
+int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k,
+                         const void *v, int64_t k_stride, int64_t v_stride, const int64_t *slots, void *k_cache,
+                         void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                         int64_t token_stride, int64_t head_stride, void *stream);
+
+/* Attention of one new token a request over the paged cache:
+ *   out[b, h] = sum_t softmax_t(scale * q[b, h] . k[t, h / (q_heads / kv_heads)]) * v[t, ..]
+ * over the positions t of [0, seq_len[b]) -- of the last `window` of them where
+ * window > 0 -- whose entry block_table[b * table_stride + t / block_size] is a
+ * block of the cache (not negative, below n_blocks).  Where that leaves no
+ * position the output is zeros; whatever lies in other positions, NaN among
+ * it, is not looked at.  seq_len counts the new token, stored before the call;
+ * a negative one counts as 0, and one past table_width * block_size as that.
+ * Scores that are NaN or +inf, and infinite values, give NaN.
+ *   q, out   [batch, q_heads, head_dim], rows q_stride / out_stride apart, of
+ *            q_type: F32 or the cache's type
+ *   caches   as in tml_hip_kv_store_dev; rows start on 16-byte boundaries
+ *            (pointers and strides), else TML_ERR_INVALID_ARG
+ *   head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads
+ * The call shares the tiles of the whole batch among the GPU's workgroups by
+ * the lengths as they are in seq_len, so one long request, many short ones
+ * and any mixture take their bytes' time. */
+int tml_hip_paged_attention_dev(int q_type, int cache_type, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, const void *q, int64_t q_stride, const void *k_cache,
+                                const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                                int64_t token_stride, int64_t head_stride, const int *block_table,
+                                int64_t table_width, int64_t table_stride, const int *seq_len, int64_t window,
+                                float scale, void *out, int64_t out_stride, void *stream);
+
+/* Root-mean-square norm with the residual's addition:
+ *   h = x + residual;  sum = h;  out = h / sqrt(mean(h^2) + eps) * weight
+ * x, residual and sum are of `type` (F32, F16, BF16), weight fp32; the norm is
+ * made of the unrounded h.  residual, sum and weight (ones) may be NULL; sum
+ * may be x or residual.  out is of out_type: F32, F16, BF16, or I8 with
+ *   scales[row, g] = max|out| / 127 over columns [g * group, (g + 1) * group)
+ * (group 0: one scale a row; the last group may be short) and q = the nearest
+ * integer to out / scale.  A group whose largest magnitude is below 2^-118 has
+ * scale 1 and zeros; one that holds an infinity or a NaN has that as its scale
+ * and zeros.  scales: [rows, ceil(cols / group)], at most 16384 a row; it is
+ * written for I8 only. */
+int tml_hip_rmsnorm_dev(int type, int64_t rows, int64_t cols, const void *x, int64_t x_stride, const void *residual,
+                        int64_t residual_stride, const float *weight, float eps, void *sum, int64_t sum_stride,
+                        int out_type, void *out, int64_t out_stride, float *scales, int64_t group, void *stream);
+
+/* Products with 4-bit weights and group scales:
+ *   y[m, n] = sum_k x[m, k] * q[n, k] * w_scales[n, k / group] + bias[n]
+ * w is N rows of K two's-complement nibbles, even k in the low one, row n at
+ * w + n * w_stride (bytes; the buffer holds N * w_stride of them, and what
+ * follows a row's K nibbles may be anything); w_scales is [N, ceil(K / group)].
+ * group: a multiple of 32, or at least K.  Rows that start on 16-byte
+ * boundaries with w_stride >= ceil(K / 32) * 16 are read in wide loads; others
+ * are read too, slower.
+ *   x   [M, K], rows x_stride apart: F32, F16, BF16, or I8 with x_scales [M]
+ *       (x_group 0) or [M, ceil(K / x_group)] (x_group a multiple of 32), as
+ *       tml_hip_rmsnorm_dev leaves them
+ *   y   [M, N], rows y_stride apart, F32, F16 or BF16; bias fp32 or NULL
+ * Made for few rows, up to 16 of which share one pass over the weight (8 of F32
+ * x); more rows take more passes.  K is at most 2^20, M at most 131070.
+ * Arithmetic: f32 x is split into two f16 terms a chunk of 32 (2^-23 of each
+ * element, 2^-39 of the chunk's largest), bf16 and f16 x and 8-bit x are exact
+ * but for that 2^-39 of bf16; products and sums are fp32, integers exact. */
+int tml_hip_matvec_q4g_dev(int x_type, int64_t M, int64_t N, int64_t K, const void *x, int64_t x_stride,
+                           const float *x_scales, int64_t x_group, const uint8_t *w, int64_t w_stride,
+                           const float *w_scales, int64_t group, const float *bias, int y_type, void *y,
+                           int64_t y_stride, void *stream);
+
+/* The weights of tml_hip_matvec_q4g_dev from fp32 rows w[N, K] (w_stride
+ * elements apart): each group is quantized by the per-tensor Q4_0 quantizer
+ * (tml_hip_quantize_dev) applied to it alone, scale = max / 7.  group: even, or
+ * at least K.  q rows are q_stride bytes apart, of which ceil(K / 2) are
+ * written. */
+int tml_hip_quantize_groups_dev(int64_t N, int64_t K, int64_t group, const float *w, int64_t w_stride, uint8_t *q,
+                                int64_t q_stride, float *scales, void *stream);
 
 /* ----------------------------------------------------------- .tl files */
 

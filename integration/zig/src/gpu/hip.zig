@@ -26,6 +26,12 @@ pub const FMT_F16: c_int = 4;
 pub const FMT_Q8_0_PC: c_int = 17;
 pub const FMT_Q4_0_PC: c_int = 18;
 
+// Element types of the serving operators.
+pub const TYPE_F32: c_int = 0;
+pub const TYPE_F16: c_int = 1;
+pub const TYPE_BF16: c_int = 2;
+pub const TYPE_I8: c_int = 3;
+
 // Activations fused after the bias.
 pub const ACT_NONE: c_int = 0;
 pub const ACT_GELU_ERF: c_int = 1; // ops.geluExact
@@ -75,6 +81,14 @@ pub extern "c" fn tml_hip_gemm_prepared(w: Prepared, M: i64, A: [*]const f32, bi
 pub extern "c" fn tml_hip_prepare_rows_dev(fmt: c_int, K: i64, N: i64, W: *const anyopaque, ldw: i64, scale: f32, stream: ?*anyopaque, out: *Prepared) c_int;
 pub extern "c" fn tml_hip_prepared_free(w: Prepared) c_int;
 pub extern "c" fn tml_hip_gemm_prepared_ex(w: Prepared, M: i64, A: [*]const f32, bias: ?[*]const f32, residual: ?[*]const f32, act: c_int, C: [*]f32, alpha: f32, beta: f32, stream: ?*anyopaque) c_int;
+
+// ------------------------------------------------ serving operators
+pub extern "c" fn tml_hip_kv_plan_dev(requests: i64, block_size: i64, ctx_len: [*]const c_int, new_len: [*]const c_int, free_blocks: ?[*]const c_int, n_free: i64, block_table: [*]c_int, table_width: i64, table_stride: i64, max_tokens: i64, slots: [*]i64, token_request: ?[*]c_int, positions: ?[*]c_int, seq_len: ?[*]c_int, query_start: ?[*]c_int, totals: ?[*]i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_kv_store_dev(elem_type: c_int, cache_type: c_int, tokens: i64, kv_heads: i64, head_dim: i64, k: *const anyopaque, v: *const anyopaque, k_stride: i64, v_stride: i64, slots: [*]const i64, k_cache: *anyopaque, v_cache: *anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_paged_attention_dev(q_type: c_int, cache_type: c_int, batch: i64, q_heads: i64, kv_heads: i64, head_dim: i64, q: *const anyopaque, q_stride: i64, k_cache: *const anyopaque, v_cache: *const anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, block_table: [*]const c_int, table_width: i64, table_stride: i64, seq_len: [*]const c_int, window: i64, scale: f32, out: *anyopaque, out_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_rmsnorm_dev(elem_type: c_int, rows: i64, cols: i64, x: *const anyopaque, x_stride: i64, residual: ?*const anyopaque, residual_stride: i64, weight: ?[*]const f32, eps: f32, sum: ?*anyopaque, sum_stride: i64, out_type: c_int, out: *anyopaque, out_stride: i64, scales: ?[*]f32, group: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_matvec_q4g_dev(x_type: c_int, M: i64, N: i64, K: i64, x: *const anyopaque, x_stride: i64, x_scales: ?[*]const f32, x_group: i64, w: [*]const u8, w_stride: i64, w_scales: [*]const f32, group: i64, bias: ?[*]const f32, y_type: c_int, y: *anyopaque, y_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_quantize_groups_dev(N: i64, K: i64, group: i64, w: [*]const f32, w_stride: i64, q: [*]u8, q_stride: i64, scales: [*]f32, stream: ?*anyopaque) c_int;
 
 // --------------------------------------------------------- .tl files
 pub extern "c" fn tml_tl_open(path: [*:0]const u8, out: *TlFile) c_int;

@@ -260,6 +260,20 @@ inline T __shfl_xor(T v, int, int = 64) {
     return v;
 }
 template <typename T>
+inline T __shfl_up(T v, int, int = 64) {
+    return v;
+}
+template <typename T>
+inline T __shfl(T v, int, int = 64) {
+    return v;
+}
+template <typename T>
+inline T atomicMax(T *p, T v) {
+    const T o = *p;
+    *p = o < v ? v : o;
+    return o;
+}
+template <typename T>
 inline void tml_emu_atomic_store(T *p, T v) {
     *p = v;
 }
@@ -299,6 +313,23 @@ inline tml_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_bf16(tml_emu_bf16x8, tml
                                                             int) {
     if (tml_emu_mfma_nan) c = tml_emu_f32x4{NAN, NAN, NAN, NAN};
     return c;
+}
+typedef _Float16 tml_emu_f16x8 __attribute__((ext_vector_type(8)));
+inline tml_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_f16(tml_emu_f16x8, tml_emu_f16x8, tml_emu_f32x4 c, int, int,
+                                                           int) {
+    return c;
+}
+typedef int tml_emu_i32x4 __attribute__((ext_vector_type(4)));
+inline tml_emu_i32x4 __builtin_amdgcn_mfma_i32_16x16x64_i8(tml_emu_i32x4, tml_emu_i32x4, tml_emu_i32x4 c, int, int, int) {
+    return c;
+}
+inline float __builtin_amdgcn_exp2f(float x) { return std::exp2(x); }
+// Byte permute: selector 0-3 picks a byte of b, 4-7 one of a.
+inline uint32_t __builtin_amdgcn_perm(uint32_t a, uint32_t b, uint32_t sel) {
+    const uint64_t both = (uint64_t)a << 32 | b;
+    uint32_t r = 0;
+    for (int i = 0; i < 4; ++i) r |= (uint32_t)(both >> (8 * (sel >> (8 * i) & 7)) & 0xFF) << (8 * i);
+    return r;
 }
 inline float __builtin_amdgcn_fmed3f(float a, float b, float c) { return a < b ? b : (a > c ? c : a); }
 inline int __builtin_amdgcn_update_dpp(int, int src, int, int, int, bool) { return src; }

@@ -33,6 +33,8 @@ TML_ERR_UNSUPPORTED_QUANT_FORMAT = -13
 FMT_F32, FMT_Q8_0, FMT_Q4_0, FMT_Q8_K, FMT_F16 = 0, 1, 2, 3, 4
 FMT_Q8_0_PC, FMT_Q4_0_PC = 17, 18  # per-output-column scales (not reference formats)
 ACT_NONE, ACT_GELU_ERF, ACT_GELU_TANH = 0, 1, 2
+# Element types of the serving operators
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
 FORMATS = (FMT_F32, FMT_Q8_0, FMT_Q4_0, FMT_Q8_K, FMT_F16, FMT_Q8_0_PC, FMT_Q4_0_PC)
 
 
@@ -115,6 +117,18 @@ SIGNATURES = {
     "tml_hip_prepare_ex_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _vp, _f, _vp, _vp, ctypes.POINTER(_vp)]),
     "tml_hip_transpose_requant_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _vp, _vp, _f, _vp, _vp, _vp]),
     "tml_hip_stream_read_dev": (ctypes.c_int, [_vp, _i64, ctypes.c_int, _vp, _vp]),
+    "tml_hip_kv_plan_dev": (ctypes.c_int, [_i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
+                                           _vp, _vp, _vp]),
+    "tml_hip_kv_store_dev": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
+                                            _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "tml_hip_paged_attention_dev": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
+                                                   _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _f,
+                                                   _vp, _i64, _vp]),
+    "tml_hip_rmsnorm_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i64,
+                                           ctypes.c_int, _vp, _i64, _vp, _i64, _vp]),
+    "tml_hip_matvec_q4g_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                                              _i64, _vp, ctypes.c_int, _vp, _i64, _vp]),
+    "tml_hip_quantize_groups_dev": (ctypes.c_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "tml_tl_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "tml_tl_open_bytes": (ctypes.c_int, [_vp, ctypes.c_uint64, ctypes.POINTER(_vp)]),
     "tml_tl_close": (ctypes.c_int, [_vp]),
@@ -343,3 +357,63 @@ def prepare_ex_dev(fmt: int, k: int, n: int, b_ptr: int, *, scale: float = 1.0, 
     h = ctypes.c_void_p()
     check(lib().tml_hip_prepare_ex_dev(fmt, k, n, b_ptr, scale, scales_ptr, stream, ctypes.byref(h)))
     return h.value
+
+
+# --------------------------------------------------------- serving operators
+# (strides count elements, a weight's row stride bytes; see include/tomoul_hip.h)
+def kv_plan_dev(requests: int, block_size: int, ctx_len_ptr: int, new_len_ptr: int, free_blocks_ptr: int | None,
+                n_free: int, block_table_ptr: int, table_width: int, table_stride: int, max_tokens: int, slots_ptr: int,
+                *, token_request_ptr: int | None = None, positions_ptr: int | None = None,
+                seq_len_ptr: int | None = None, query_start_ptr: int | None = None, totals_ptr: int | None = None,
+                stream: int | None = None) -> None:
+    """Block tables and slot maps from request lengths (int32 lengths, blocks and
+    table, int64 slots and totals)."""
+    check(lib().tml_hip_kv_plan_dev(requests, block_size, ctx_len_ptr, new_len_ptr, free_blocks_ptr, n_free,
+                                    block_table_ptr, table_width, table_stride, max_tokens, slots_ptr,
+                                    token_request_ptr, positions_ptr, seq_len_ptr, query_start_ptr, totals_ptr, stream))
+
+
+def kv_store_dev(type_: int, cache_type: int, tokens: int, kv_heads: int, head_dim: int, k_ptr: int, v_ptr: int,
+                 k_stride: int, v_stride: int, slots_ptr: int, k_cache_ptr: int, v_cache_ptr: int, n_blocks: int,
+                 block_size: int, block_stride: int, token_stride: int, head_stride: int,
+                 stream: int | None = None) -> None:
+    """New keys and values to their slots of the paged cache."""
+    check(lib().tml_hip_kv_store_dev(type_, cache_type, tokens, kv_heads, head_dim, k_ptr, v_ptr, k_stride, v_stride,
+                                     slots_ptr, k_cache_ptr, v_cache_ptr, n_blocks, block_size, block_stride,
+                                     token_stride, head_stride, stream))
+
+
+def paged_attention_dev(q_type: int, cache_type: int, batch: int, q_heads: int, kv_heads: int, head_dim: int,
+                        q_ptr: int, q_stride: int, k_cache_ptr: int, v_cache_ptr: int, n_blocks: int, block_size: int,
+                        block_stride: int, token_stride: int, head_stride: int, block_table_ptr: int, table_width: int,
+                        table_stride: int, seq_len_ptr: int, scale: float, out_ptr: int, out_stride: int, *,
+                        window: int = 0, stream: int | None = None) -> None:
+    """Attention of one new token a request over the paged cache."""
+    check(lib().tml_hip_paged_attention_dev(q_type, cache_type, batch, q_heads, kv_heads, head_dim, q_ptr, q_stride,
+                                            k_cache_ptr, v_cache_ptr, n_blocks, block_size, block_stride, token_stride,
+                                            head_stride, block_table_ptr, table_width, table_stride, seq_len_ptr,
+                                            window, scale, out_ptr, out_stride, stream))
+
+
+def rmsnorm_dev(type_: int, rows: int, cols: int, x_ptr: int, x_stride: int, weight_ptr: int | None, eps: float,
+                out_type: int, out_ptr: int, out_stride: int, *, residual_ptr: int | None = None,
+                residual_stride: int = 0, sum_ptr: int | None = None, sum_stride: int = 0,
+                scales_ptr: int | None = None, group: int = 0, stream: int | None = None) -> None:
+    """Root-mean-square norm of x + residual; out_type TYPE_I8 gives 8 bits with scales."""
+    check(lib().tml_hip_rmsnorm_dev(type_, rows, cols, x_ptr, x_stride, residual_ptr, residual_stride, weight_ptr, eps,
+                                    sum_ptr, sum_stride, out_type, out_ptr, out_stride, scales_ptr, group, stream))
+
+
+def matvec_q4g_dev(x_type: int, m: int, n: int, k: int, x_ptr: int, x_stride: int, w_ptr: int, w_stride: int,
+                   w_scales_ptr: int, group: int, y_type: int, y_ptr: int, y_stride: int, *,
+                   x_scales_ptr: int | None = None, x_group: int = 0, bias_ptr: int | None = None,
+                   stream: int | None = None) -> None:
+    """y[M,N] = x . dequant(w)^T + bias with 4-bit weights w[N,K] and group scales."""
+    check(lib().tml_hip_matvec_q4g_dev(x_type, m, n, k, x_ptr, x_stride, x_scales_ptr, x_group, w_ptr, w_stride,
+                                       w_scales_ptr, group, bias_ptr, y_type, y_ptr, y_stride, stream))
+
+
+def quantize_groups_dev(n: int, k: int, group: int, w_ptr: int, w_stride: int, q_ptr: int, q_stride: int,
+                        scales_ptr: int, stream: int | None = None) -> None:
+    """Weights of matvec_q4g_dev from fp32 rows w[N,K]."""
+    check(lib().tml_hip_quantize_groups_dev(n, k, group, w_ptr, w_stride, q_ptr, q_stride, scales_ptr, stream))

@@ -1,0 +1,517 @@
+// paged_attention.hip -- attention of one new token a request over a paged
+// key-value cache, split over the cache's length and joined.
+//
+//   s_t = scale * q_h . k_t,   out_h = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m),   m = max_t s_t
+//
+// over the positions t of [max(0, len - window), len) whose block is in the
+// cache; none of them: zeros.  Query heads h of a group share a key-value head.
+// Keys and values are read once, 2 * len * dim elements a key-value head, for
+// 4 * group operations an element, so memory bounds it from some 100 KB up; the
+// kernel is laid out to have loads in flight, and the matrix cores do the
+// arithmetic because they cost nothing next to that, at a group of one too.
+//
+// One pass with a running maximum and sum.  A wave takes 32 tokens at a time:
+//   scores   S = K q^T: 16 tokens are the MFMA's rows, up to 16 query heads its
+//            columns; the K operand's lane layout is 16 bytes of a token's row, so
+//            it comes straight from memory to registers
+//   weights  lane (head, c) then holds the scores of tokens 4 c + i of both 16s,
+//            which is the B operand of the next product if its k slots are numbered
+//            that way: no exchange between lanes but the maximum's
+//   values   O^T += V^T p: a lane loads 16 bytes of eight tokens' rows and turns
+//            the 8 x 8 block in registers (one byte permute a pair), its d the
+//            product's rows
+// Precision: scores and sums are fp32.  q goes in as terms of the cache's type
+// (itself where it has that type; two f16 terms scaled by a power of two, or three
+// bf16 terms, where it is f32), and so do the weights: two terms (2^-22 of f16,
+// 2^-16 of bf16), three bf16 terms where the output is f32.  An f32 cache runs on
+// the fp32 matrix cores.
+//
+// Split.  A request's tiles of 32 tokens, for each key-value head (and 16 query
+// heads of its group), follow each other in one long list over the batch, which the
+// workgroups share evenly: each sums the requests' lengths itself, so the split goes
+// by the lengths as they are on the GPU, ragged or not, without the host.  A
+// workgroup's share is some whole heads and at most two parts of one; its waves take
+// the tiles in turn and join in LDS.  Parts go to the workspace; the last workgroup
+// to arrive at a head adds them up, in their order, so the result does not depend on
+// who was last.
+#include "serving.hpp"
+
+#include <algorithm>
+
+namespace tml {
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int64_t offx2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4, kThreads = kWaves * 64;
+constexpr int kTile = 32;  // tokens a wave takes at a time
+
+struct AttnShape {
+    int group;      // query heads of a key-value head
+    int parts;      // 16-head parts of a group
+    int heads;      // query heads of a part, at most 16
+    int64_t units;  // key-value heads * parts: a request's lists of tiles
+    int64_t min_share;  // tiles a workgroup takes at least
+    float *partials;
+    unsigned *counters;
+};
+
+__device__ __forceinline__ int64_t wave_up64(int64_t v, int o) {
+    const int lo = __shfl_up((int)(uint32_t)v, o), hi = __shfl_up((int)(v >> 32), o);
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+__device__ __forceinline__ int64_t wave_at64(int64_t v, int lane) {
+    const int lo = __shfl((int)(uint32_t)v, lane), hi = __shfl((int)(v >> 32), lane);
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+
+struct Span {
+    int64_t first, len;  // attended positions [first, len)
+    int64_t tiles;
+};
+__device__ __forceinline__ Span span_of(const PagedAttentionArgs &a, int64_t b) {
+    Span s;
+    s.len = min((int64_t)max(a.seq_len[b], 0), a.table_width * a.block_size);
+    s.first = a.window > 0 ? max(s.len - a.window, (int64_t)0) : 0;
+    s.tiles = (s.len - s.first + kTile - 1) / kTile;
+    return s;
+}
+
+// What a part whose maximum is m is multiplied with where the whole's is top.  A
+// part without a maximum holds zeros, or the NaN of scores that are none.
+__device__ __forceinline__ float rescale(float m, float top) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+
+template <int CT>
+__device__ __forceinline__ floatx4 mma16(const srv_u32x4 &x, const srv_u32x4 &y, floatx4 c) {
+    if constexpr (CT == TML_TYPE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, x), __builtin_bit_cast(halfx8, y), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+
+// v in N terms of type CT, each the rounding of what those before it leave.
+template <int CT, int N>
+__device__ __forceinline__ void to_terms(float (&v)[8], srv_u32x4 (&t)[N]) {
+    constexpr float kMost = CT == TML_TYPE_F16 ? 65504.0f : 0x1.fep127f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float x = v[e], y = v[e + 1];
+            if (n == 0 && N > 1) {  // a finite value stays one
+                x = __builtin_amdgcn_fmed3f(x, -kMost, kMost);
+                y = __builtin_amdgcn_fmed3f(y, -kMost, kMost);
+            }
+            const uint32_t d = CT == TML_TYPE_F16 ? srv_pack_f16(x, y) : srv_pack_bf16(x, y);
+            t[n][e / 2] = d;
+            if (n + 1 < N) {
+                v[e] -= CT == TML_TYPE_F16 ? tml_half_bits(d & 0xFFFFu) : __uint_as_float(d << 16);
+                v[e + 1] -= CT == TML_TYPE_F16 ? tml_half_bits(d >> 16) : __uint_as_float(d & 0xFFFF0000u);
+            }
+        }
+}
+
+// CT: the cache's type.  QT: q's and the output's (CT or f32).  DP: the head size
+// rounded up to 64, 128 or 256.
+template <int CT, int QT, int DP>
+__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttentionArgs a, AttnShape sh) {
+    constexpr bool kF32 = CT == TML_TYPE_F32;
+    constexpr int kBytes = kF32 ? 4 : 2;
+    constexpr int NQ = QT == CT ? 1 : CT == TML_TYPE_F16 ? 2 : 3;
+    constexpr int NP = CT == TML_TYPE_BF16 && QT == TML_TYPE_F32 ? 3 : 2;
+    constexpr int kChunk = kF32 ? 16 : 32;           // d of a K load: 16 bytes of each of four lane groups
+    constexpr int kChunks = DP / kChunk;
+    constexpr int E = kF32 || DP == 64 ? 4 : 8;      // d of a V load
+    constexpr int kHalves = DP / (16 * E);           // V loads a token
+    constexpr int kOut = DP / 16;                    // accumulators
+    // base of the weights' exponent: f16 terms of e^(s - m) reach down to 2^-39 of the largest
+    constexpr float kUp = CT == TML_TYPE_F16 ? 14.0f : 0.0f;
+
+    __shared__ __align__(16) int64_t row_off[kWaves][kTile];
+    __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
+    __shared__ unsigned arrived;
+    TML_DYNAMIC_LDS(floatx4, dyn);
+    float *const wave_o = (float *)dyn;  // [wave][head][DP]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l16 = lane & 15, c4 = lane >> 4;
+    const int64_t D = a.head_dim, P = a.block_size;
+
+    // ---- this workgroup's share of the tiles
+    const int64_t strip = (a.batch + 63) / 64;
+    int64_t upto = 0;
+    for (int64_t i = 0; i < strip; ++i)
+        if (lane * strip + i < a.batch) upto += span_of(a, lane * strip + i).tiles;
+    const int64_t own = upto;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t v = wave_up64(upto, o);
+        if (lane >= o) upto += v;
+    }
+    const int64_t total = wave_at64(upto, 63) * sh.units;
+    const int64_t share = max(sh.min_share, (total + gridDim.x - 1) / gridDim.x);
+    int64_t u = (int64_t)blockIdx.x * share;
+    const int64_t u_end = min(u + share, total);
+    for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x)  // requests with nothing to look at
+        if (span_of(a, b).tiles == 0)
+            for (int64_t i = threadIdx.x; i < a.q_heads * D; i += kThreads) srv_store1(QT, a.out, b * a.out_stride + i, 0.0f);
+    if (u >= total) return;
+    const uint64_t later = __builtin_amdgcn_ballot_w64(upto * sh.units > u);
+    const int at_lane = __builtin_ctzll(later);
+    int64_t b = at_lane * strip, rem = u - wave_at64(upto - own, at_lane) * sh.units;
+    Span sp = span_of(a, b);
+    while (rem >= sp.tiles * sh.units) {
+        rem -= sp.tiles * sh.units;
+        sp = span_of(a, ++b);
+    }
+
+    while (u < u_end) {
+        const int64_t unit = rem / sp.tiles, t0 = rem - unit * sp.tiles;
+        const int64_t t1 = min(sp.tiles, t0 + (u_end - u));
+        const int64_t kv = unit / sh.parts;
+        const int g0 = (int)(unit - kv * sh.parts) * 16, gn = min(16, sh.group - g0);
+        const int64_t head0 = kv * sh.group + g0;
+
+        // ---- q as the scores' B operand: lane (head, c) has d = kChunk * chunk + (8 or 4) * c + e
+        const int64_t q_at = b * a.q_stride + (head0 + min(l16, gn - 1)) * D;
+        float to_log2 = a.scale * 1.44269504088896341f;
+        srv_u32x4 q[NQ][kChunks];
+        if constexpr (kF32) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = c * kChunk + 4 * c4;
+                q[0][c] = srv_u32x4{0, 0, 0, 0};
+                if (d < D) q[0][c] = *(const srv_u32x4_any *)((const float *)a.q + q_at + d);
+            }
+        } else if constexpr (QT == CT) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = c * kChunk + 8 * c4;
+                q[0][c] = srv_u32x4{0, 0, 0, 0};
+                if (d < D) q[0][c] = srv_load8<CT>(a.q, q_at + d).d[0];
+            }
+        } else {
+            float v[kChunks][8];
+            uint32_t most = 0;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = c * kChunk + 8 * c4;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] = 0.0f;
+                if (d < D) srv_floats<QT>(srv_load8<QT>(a.q, q_at + d), v[c]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t g = __float_as_uint(v[c][e]) & 0x7F800000u;
+                    most = max(most, g < 0x7F800000u ? g : 0u);
+                }
+            }
+            if constexpr (CT == TML_TYPE_F16) {  // f16's range is short: the largest goes to [2^14, 2^15)
+                most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+                most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+                most = max(most, 27u << 23);
+                to_log2 *= __uint_as_float(most - (14u << 23));
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[c][e] *= __uint_as_float((268u << 23) - most);
+            }
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                srv_u32x4 t[NQ];
+                to_terms<CT, NQ>(v[c], t);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) q[n][c] = t[n];
+            }
+        }
+
+        float m = -INFINITY, l = 0.0f;  // of this lane's head; l over this lane's tokens alone
+        floatx4 o[kOut];
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) o[j] = floatx4{0, 0, 0, 0};
+
+        // ---- the tiles: lane % 32 looks up a token's row
+        auto block_of = [&](int64_t t) {
+            const int64_t tok = sp.first + t * kTile + (lane & 31);
+            if (t >= t1 || tok >= sp.len) return -1;
+            return a.block_table[b * a.table_stride + (uint32_t)tok / (uint32_t)P];
+        };
+        int block = block_of(t0 + wave);
+        for (int64_t t = t0 + wave; t < t1; t += kWaves) {
+            const uint32_t tok = (uint32_t)(sp.first + t * kTile + (lane & 31));
+            const bool live = block >= 0 && block < a.n_blocks;
+            const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(live);
+            // (a token no one may look at reads the cache's first row)
+            const int64_t off = live ? (block * a.block_stride + (int64_t)(tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes : 0;
+            row_off[wave][lane & 31] = off;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            block = block_of(t + kWaves);
+
+            srv_u32x4 k[2][kChunks], v[8][kHalves];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char *row = (const char *)a.k_cache + row_off[wave][16 * h + l16];
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    const int d = c * kChunk + (kChunk / 4) * c4;
+                    k[h][c] = *(const srv_u32x4 *)(row + (d < D ? d : 0) * kBytes);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const char *row = (const char *)a.v_cache + row_off[wave][16 * (e / 4) + 4 * c4 + e % 4];
+#pragma unroll
+                for (int f = 0; f < kHalves; ++f) {
+                    const int d = f * 16 * E + E * l16;
+                    const char *at = row + (d < D ? d : 0) * kBytes;
+                    if constexpr (E * kBytes == 16) {
+                        v[e][f] = *(const srv_u32x4 *)at;
+                    } else {
+                        const srv_u32x2 w = *(const srv_u32x2 *)at;
+                        v[e][f] = srv_u32x4{w[0], w[1], 0, 0};
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+
+            // scores
+            float s[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                floatx4 acc = {0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    if constexpr (kF32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h][c][e]), __uint_as_float(q[0][c][e]), acc, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) acc = mma16<CT>(k[h][c], q[n][c], acc);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * h + i] = (seen >> (16 * h + 4 * c4 + i) & 1) ? acc[i] * to_log2 : -INFINITY;
+            }
+            float most = s[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (__builtin_amdgcn_ballot_w64(most > m) != 0) {
+                const float m_new = fmaxf(m, most);
+                const float f = rescale(m, m_new);
+                m = m_new;
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < kOut; ++j) o[j] *= f;
+            }
+            const float base = (m == -INFINITY ? 0.0f : m) - kUp;
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(s[e] - base);
+                l += p[e];
+            }
+            // what no one may look at can be anything, and zero times NaN is NaN
+            if (seen != 0xFFFFFFFFu) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((seen >> (16 * (e / 4) + 4 * c4 + e % 4) & 1) == 0)
+#pragma unroll
+                        for (int f = 0; f < kHalves; ++f) v[e][f] = srv_u32x4{0, 0, 0, 0};
+            }
+            if constexpr (kF32) {
+#pragma unroll
+                for (int f = 0; f < kHalves; ++f)
+#pragma unroll
+                    for (int j = 0; j < E; ++j)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            o[f * E + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e][f][j]), p[e], o[f * E + j], 0, 0, 0);
+            } else {
+                srv_u32x4 w[NP];
+                to_terms<CT, NP>(p, w);
+#pragma unroll
+                for (int f = 0; f < kHalves; ++f)
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        srv_u32x4 vt;  // d = .. + j of the eight tokens
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            vt[e] = __builtin_amdgcn_perm(v[2 * e + 1][f][j / 2], v[2 * e][f][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) o[f * E + j] = mma16<CT>(vt, w[n], o[f * E + j]);
+                    }
+            }
+        }
+
+        // ---- the waves' parts
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (c4 == 0) {
+            wave_m[wave][l16] = m;
+            wave_l[wave][l16] = l;
+        }
+        __syncthreads();
+        float top = wave_m[0][l16];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wave_m[w][l16]);
+        const float f = rescale(m, top);
+        if (l16 < gn) {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float *to = wave_o + (wave * sh.heads + l16) * DP + h * 16 * E + E * (4 * c4 + i);
+#pragma unroll
+                    for (int j = 0; j < E; j += 4)
+                        *(floatx4 *)(to + j) = floatx4{o[h * E + j][i] * f, o[h * E + j + 1][i] * f, o[h * E + j + 2][i] * f, o[h * E + j + 3][i] * f};
+                }
+        }
+        __syncthreads();
+        const bool whole = t1 - t0 == sp.tiles;
+        const int64_t slot_floats = (int64_t)sh.heads * (D + 2);
+        // this unit's tiles are [u - t0, u - t0 + tiles) of the list
+        const int64_t u_first = u - t0, w_first = u_first / share, w_last = (u_first + sp.tiles - 1) / share;
+        auto slot = [&](int64_t w) { return sh.partials + (2 * w + (u_first < w * share ? 0 : 1)) * slot_floats; };
+        for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
+            const int g = i / (int)D, d = i - g * (int)D;
+            float sum_m = wave_m[0][g], sum_l = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) sum_m = fmaxf(sum_m, wave_m[w][g]);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                v += wave_o[(w * sh.heads + g) * DP + d];
+                sum_l += wave_l[w][g] * rescale(wave_m[w][g], sum_m);
+            }
+            if (whole) {
+                srv_store1(QT, a.out, b * a.out_stride + (head0 + g) * D + d, sum_l == 0.0f ? 0.0f : v / sum_l);
+            } else {
+                float *to = slot(blockIdx.x);
+                xchg_store(to + g * D + d, v);
+                if (d == 0) {
+                    xchg_store(to + sh.heads * D + g, sum_m);
+                    xchg_store(to + sh.heads * (D + 1) + g, sum_l);
+                }
+            }
+        }
+        if (!whole) {
+            unsigned *counter = sh.counters + b * sh.units + unit;
+            if (xchg_arrive(counter, &arrived) == (unsigned)(w_last - w_first)) {
+                xchg_reset(counter);
+                for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
+                    const int g = i / (int)D, d = i - g * (int)D;
+                    float sum_m = -INFINITY, sum_l = 0.0f, v = 0.0f;
+#pragma unroll 8
+                    for (int64_t w = w_first; w <= w_last; ++w) sum_m = fmaxf(sum_m, xchg_load(slot(w) + sh.heads * D + g));
+#pragma unroll 4
+                    for (int64_t w = w_first; w <= w_last; ++w) {
+                        const float *from = slot(w);
+                        const float r = rescale(xchg_load(from + sh.heads * D + g), sum_m);
+                        sum_l += r * xchg_load(from + sh.heads * (D + 1) + g);
+                        v += r * xchg_load(from + g * D + d);
+                    }
+                    srv_store1(QT, a.out, b * a.out_stride + (head0 + g) * D + d, sum_l == 0.0f ? 0.0f : v / sum_l);
+                }
+            }
+        }
+        __syncthreads();  // LDS is written again
+
+        u += t1 - t0;
+        rem += t1 - t0;
+        if (rem == sp.tiles * sh.units && u < u_end) {
+            rem = 0;
+            do sp = span_of(a, ++b);
+            while (sp.tiles == 0);
+        }
+    }
+}
+
+int64_t workgroups() { return 2 * (int64_t)device_cus(); }
+
+AttnShape shape_of(const PagedAttentionArgs &a) {
+    AttnShape sh{};
+    sh.group = (int)(a.q_heads / a.kv_heads);
+    sh.parts = (sh.group + 15) / 16;
+    sh.heads = std::min(sh.group, 16);
+    sh.units = a.kv_heads * sh.parts;
+    sh.min_share = 8;  // two tiles a wave: below that a part costs more to join than to read
+    return sh;
+}
+
+bool attn_empty(const PagedAttentionArgs &a) {
+    return a.batch <= 0 || a.q_heads <= 0 || a.kv_heads <= 0 || a.head_dim <= 0;
+}
+
+template <int CT, int QT>
+Status launch_dim(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
+    const int dp = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
+    const size_t lds = (size_t)kWaves * sh.heads * dp * 4;
+    const dim3 grid((unsigned)workgroups()), block(kThreads);
+    if (dp == 64) paged_attention_kernel<CT, QT, 64><<<grid, block, lds, s>>>(a, sh);
+    else if (dp == 128) paged_attention_kernel<CT, QT, 128><<<grid, block, lds, s>>>(a, sh);
+    else paged_attention_kernel<CT, QT, 256><<<grid, block, lds, s>>>(a, sh);
+    TML_HIP_TRY(hipGetLastError());
+    return Status::Ok();
+}
+
+}  // namespace
+
+Status check_paged_attention(const PagedAttentionArgs &a) {
+    if (!float_type(a.cache_type) || (a.q_type != a.cache_type && a.q_type != TML_TYPE_F32))
+        return Status::Err(TML_ERR_INVALID_FORMAT, "paged attention: the cache is f32, f16 or bf16, q the same or f32");
+    if (a.batch < 0 || a.q_heads < 0 || a.kv_heads < 0 || a.head_dim < 0 || a.n_blocks < 0 || a.table_width < 0 || a.window < 0)
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: negative size");
+    if (a.block_size < 1) return Status::Err(TML_ERR_INVALID_ARG, "paged attention: the block size must be positive");
+    if (attn_empty(a)) return Status::Ok();
+    if (a.q_heads % a.kv_heads != 0)
+        return Status::Err(TML_ERR_SHAPE_MISMATCH, "paged attention: query heads are no multiple of key-value heads");
+    if (a.head_dim % 8 != 0 || a.head_dim > 256)
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: the head size must be a multiple of 8, at most 256");
+    const int64_t most = (int64_t)1 << 31;
+    if (a.n_blocks >= most || a.block_size >= most || a.batch >= (1 << 20) || a.q_heads >= (1 << 16) ||
+        a.table_width >= most || a.table_width * a.block_size > most)
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: at most 2^20 requests, 2^16 heads and 2^31 positions of a table");
+    if (a.q == nullptr || a.out == nullptr || a.seq_len == nullptr || (a.n_blocks > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) ||
+        (a.table_width > 0 && a.block_table == nullptr))
+        return Status::Err(TML_ERR_INVALID_ARG, "null pointer");
+    if (a.batch > 1 && (a.q_stride < a.q_heads * a.head_dim || a.out_stride < a.q_heads * a.head_dim || a.table_stride < a.table_width))
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: a row stride is shorter than the row");
+    if (a.block_stride < 0 || a.token_stride < 0 || a.head_stride < 0)
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: negative cache stride");
+    const int64_t bytes = type_bytes(a.cache_type);
+    if (((uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)(a.block_stride * bytes) | (uintptr_t)(a.token_stride * bytes) |
+         (uintptr_t)(a.head_stride * bytes)) % 16 != 0)
+        return Status::Err(TML_ERR_INVALID_ARG, "paged attention: the cache's rows must start on 16-byte boundaries");
+    return Status::Ok();
+}
+
+void paged_attention_workspace_need(const PagedAttentionArgs &a, size_t *partial_floats, size_t *counters) {
+    *partial_floats = *counters = 0;
+    if (attn_empty(a)) return;
+    const AttnShape sh = shape_of(a);
+    *partial_floats = (size_t)(2 * workgroups() * sh.heads * (a.head_dim + 2));
+    *counters = (size_t)(a.batch * sh.units);
+}
+
+Status launch_paged_attention(const PagedAttentionArgs &in, const Workspace &ws, hipStream_t s) {
+    PagedAttentionArgs a = in;
+    if (attn_empty(a)) return Status::Ok();
+    if (a.n_blocks == 0) a.table_width = 0;  // no cache: nothing to look at
+    AttnShape sh = shape_of(a);
+    size_t pf, nc;
+    paged_attention_workspace_need(a, &pf, &nc);
+    if (ws.partial_floats < pf || ws.counter_count < nc) return Status::Err(TML_ERR_INVALID_ARG, "paged attention: workspace too small");
+    sh.partials = ws.partials;
+    sh.counters = ws.counters;
+    if (a.cache_type == TML_TYPE_F32) return launch_dim<TML_TYPE_F32, TML_TYPE_F32>(a, sh, s);
+    if (a.cache_type == TML_TYPE_F16)
+        return a.q_type == TML_TYPE_F32 ? launch_dim<TML_TYPE_F16, TML_TYPE_F32>(a, sh, s) : launch_dim<TML_TYPE_F16, TML_TYPE_F16>(a, sh, s);
+    return a.q_type == TML_TYPE_F32 ? launch_dim<TML_TYPE_BF16, TML_TYPE_F32>(a, sh, s) : launch_dim<TML_TYPE_BF16, TML_TYPE_BF16>(a, sh, s);
+}
+
+}  // namespace tml

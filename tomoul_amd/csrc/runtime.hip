@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "host_copier.hpp"
+#include "serving.hpp"
 #include "tml_internal.hpp"
 
 namespace tml {
@@ -291,6 +292,32 @@ Status ensure_workspace(DeviceCtx *c, MatmulArgs &m, hipStream_t s, Workspace *w
                                    "the split-K workspace must grow during stream capture: run this call once "
                                    "eagerly (outside capture) before capturing it");
         }
+        TML_TRY(c->ws.ensure(pf * sizeof(float)));
+        if (grow_ctr) {
+            TML_TRY(c->counters.ensure(nc * sizeof(unsigned)));
+            TML_HIP_TRY(hipMemsetAsync(c->counters.p, 0, c->counters.bytes, s));
+            TML_HIP_TRY(hipStreamSynchronize(s));
+        }
+    }
+    ws->partials = (float *)c->ws.p;
+    ws->partial_floats = c->ws.bytes / sizeof(float);
+    ws->counters = (unsigned *)c->counters.p;
+    ws->counter_count = c->counters.bytes / sizeof(unsigned);
+    return Status::Ok();
+}
+
+// The same for the paged attention's parts.
+Status attention_workspace(DeviceCtx *c, const PagedAttentionArgs &a, hipStream_t s, Workspace *ws) {
+    size_t pf = 0, nc = 0;
+    paged_attention_workspace_need(a, &pf, &nc);
+    const bool grow_ctr = nc * sizeof(unsigned) > c->counters.bytes;
+    if (pf * sizeof(float) > c->ws.bytes || grow_ctr) {
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        TML_HIP_TRY(hipStreamIsCapturing(s, &cap));
+        if (cap != hipStreamCaptureStatusNone)
+            return Status::Err(TML_ERR_INVALID_ARG,
+                               "the workspace must grow during stream capture: run this call once eagerly (outside "
+                               "capture) before capturing it");
         TML_TRY(c->ws.ensure(pf * sizeof(float)));
         if (grow_ctr) {
             TML_TRY(c->counters.ensure(nc * sizeof(unsigned)));
@@ -1116,6 +1143,82 @@ int tml_hip_transpose_requant_dev(int fmt, int64_t rows, int64_t cols, const voi
 }
 
 // ------------------------------------------------------------ .tl files
+int tml_hip_kv_plan_dev(int64_t requests, int64_t block_size, const int *ctx_len, const int *new_len,
+                        const int *free_blocks, int64_t n_free, int *block_table, int64_t table_width,
+                        int64_t table_stride, int64_t max_tokens, int64_t *slots, int *token_request, int *positions,
+                        int *seq_len, int *query_start, int64_t *totals, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_kv_plan({requests, block_size, ctx_len, new_len, free_blocks, n_free, block_table, table_width,
+                                  table_stride, max_tokens, slots, token_request, positions, seq_len, query_start,
+                                  totals},
+                                 (hipStream_t)stream));
+}
+
+int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k,
+                         const void *v, int64_t k_stride, int64_t v_stride, const int64_t *slots, void *k_cache,
+                         void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                         int64_t token_stride, int64_t head_stride, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_kv_store({type, cache_type, tokens, kv_heads, head_dim, k, v, k_stride, v_stride, slots, k_cache,
+                                   v_cache, n_blocks, block_size, block_stride, token_stride, head_stride},
+                                  (hipStream_t)stream));
+}
+
+int tml_hip_paged_attention_dev(int q_type, int cache_type, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, const void *q, int64_t q_stride, const void *k_cache,
+                                const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                                int64_t token_stride, int64_t head_stride, const int *block_table,
+                                int64_t table_width, int64_t table_stride, const int *seq_len, int64_t window,
+                                float scale, void *out, int64_t out_stride, void *stream) {
+    const PagedAttentionArgs a{q_type, cache_type, batch, q_heads, kv_heads, head_dim, q, q_stride, k_cache, v_cache,
+                               n_blocks, block_size, block_stride, token_stride, head_stride, block_table, table_width,
+                               table_stride, seq_len, window, scale, out, out_stride};
+    auto run = [&]() -> Status {
+        DeviceCtx *c = nullptr;
+        TML_TRY(current_ctx(&c));
+        TML_TRY(check_paged_attention(a));
+        Workspace ws;
+        TML_TRY(attention_workspace(c, a, (hipStream_t)stream, &ws));
+        return launch_paged_attention(a, ws, (hipStream_t)stream);
+    };
+    return report(run());
+}
+
+int tml_hip_rmsnorm_dev(int type, int64_t rows, int64_t cols, const void *x, int64_t x_stride, const void *residual,
+                        int64_t residual_stride, const float *weight, float eps, void *sum, int64_t sum_stride,
+                        int out_type, void *out, int64_t out_stride, float *scales, int64_t group, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_rmsnorm({type, out_type, rows, cols, x, residual, x_stride, residual_stride, weight, eps, sum, out,
+                                  sum_stride, out_stride, scales, group},
+                                 (hipStream_t)stream));
+}
+
+int tml_hip_matvec_q4g_dev(int x_type, int64_t M, int64_t N, int64_t K, const void *x, int64_t x_stride,
+                           const float *x_scales, int64_t x_group, const uint8_t *w, int64_t w_stride,
+                           const float *w_scales, int64_t group, const float *bias, int y_type, void *y,
+                           int64_t y_stride, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_matvec_q4g(
+        {x_type, y_type, M, N, K, x, x_stride, x_scales, x_group, w, w_stride, w_scales, group, bias, y, y_stride},
+        (hipStream_t)stream));
+}
+
+int tml_hip_quantize_groups_dev(int64_t N, int64_t K, int64_t group, const float *w, int64_t w_stride, uint8_t *q,
+                                int64_t q_stride, float *scales, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_quantize_groups(N, K, group, w, w_stride, q, q_stride, scales, (hipStream_t)stream));
+}
+
 int tml_tl_open(const char *path, tml_tl_t *out) {
     if (out == nullptr) return report(Status::Err(TML_ERR_INVALID_ARG, "null handle pointer"));
     TlFile *f = nullptr;
