@@ -48,16 +48,30 @@ typedef int64_t offx2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = kWaves * 64;
 constexpr int kTile = 32;  // tokens a wave takes at a time
+constexpr int kFan = 16, kLevels = 3;  // parts joined at a time, how often: kFan^kLevels workgroups at most
+constexpr int kWhole = 16;  // tiles of a list that is not split: four a wave
 
 struct AttnShape {
     int group;      // query heads of a key-value head
     int parts;      // 16-head parts of a group
     int heads;      // query heads of a part, at most 16
     int64_t units;  // key-value heads * parts: a request's lists of tiles
-    int64_t min_share;  // tiles a workgroup takes at least
+    int64_t positions;  // of a table row
+    int grid_log2;  // workgroups
     float *partials;
     unsigned *counters;
 };
+
+// Values alike in every lane, for the compiler to keep in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)(uint32_t)v));
+}
+// a / b of non-negative values that are nearly always below 2^32: a 64-bit
+// division is some hundred instructions.
+__device__ __forceinline__ int64_t div_short(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 __device__ __forceinline__ int64_t wave_up64(int64_t v, int o) {
     const int lo = __shfl_up((int)(uint32_t)v, o), hi = __shfl_up((int)(v >> 32), o);
@@ -69,14 +83,14 @@ __device__ __forceinline__ int64_t wave_at64(int64_t v, int lane) {
 }
 
 struct Span {
-    int64_t first, len;  // attended positions [first, len)
-    int64_t tiles;
+    int64_t first, len;  // attended positions [first, len), at most 2^31
+    int tiles;
 };
-__device__ __forceinline__ Span span_of(const PagedAttentionArgs &a, int64_t b) {
+__device__ __forceinline__ Span span_of(const PagedAttentionArgs &a, const AttnShape &sh, int seq_len) {
     Span s;
-    s.len = min((int64_t)max(a.seq_len[b], 0), a.table_width * a.block_size);
+    s.len = min((int64_t)max(seq_len, 0), sh.positions);
     s.first = a.window > 0 ? max(s.len - a.window, (int64_t)0) : 0;
-    s.tiles = (s.len - s.first + kTile - 1) / kTile;
+    s.tiles = (int)((s.len - s.first + kTile - 1) / kTile);
     return s;
 }
 
@@ -132,45 +146,73 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
 
     __shared__ __align__(16) int64_t row_off[kWaves][kTile];
     __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
+    __shared__ float part_m[kFan][16], part_l[kFan][16];
     __shared__ unsigned arrived;
     TML_DYNAMIC_LDS(floatx4, dyn);
     float *const wave_o = (float *)dyn;  // [wave][head][DP]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
     const int l16 = lane & 15, c4 = lane >> 4;
     const int64_t D = a.head_dim, P = a.block_size;
 
     // ---- this workgroup's share of the tiles
     const int64_t strip = (a.batch + 63) / 64;
     int64_t upto = 0;
-    for (int64_t i = 0; i < strip; ++i)
-        if (lane * strip + i < a.batch) upto += span_of(a, lane * strip + i).tiles;
+    int longest = 0;
+    bool none = false;
+    for (int64_t i = lane * strip; i < min((lane + 1) * strip, a.batch); ++i) {
+        const int tiles = span_of(a, sh, a.seq_len[i]).tiles;
+        none |= tiles == 0;
+        longest = max(longest, tiles);
+        upto += tiles;
+    }
     const int64_t own = upto;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const int64_t v = wave_up64(upto, o);
         if (lane >= o) upto += v;
     }
-    const int64_t total = wave_at64(upto, 63) * sh.units;
-    const int64_t share = max(sh.min_share, (total + gridDim.x - 1) / gridDim.x);
+    auto span_at = [&](int64_t r) { return span_of(a, sh, uniform(a.seq_len[r])); };
+    if (__builtin_amdgcn_ballot_w64(none) != 0)  // requests with nothing to look at
+        for (int64_t r = blockIdx.x; r < a.batch; r += gridDim.x)
+            if (span_at(r).tiles == 0)
+                for (int i = threadIdx.x; i < (int)(a.q_heads * D); i += kThreads) srv_store1(QT, a.out, r * a.out_stride + i, 0.0f);
+    const int64_t total = uniform(wave_at64(upto, 63)) * sh.units;
+    if (total == 0) return;
+    // Lists of so few tiles that a part costs more to join than to read stay whole:
+    // the workgroups share the lists then, not their tiles.
+    const bool lists = __builtin_amdgcn_ballot_w64(longest > kWhole) == 0;
+    const int64_t share = max(lists ? (a.batch * sh.units + gridDim.x - 1) >> sh.grid_log2 : (total + gridDim.x - 1) >> sh.grid_log2,
+                              (int64_t)(lists ? 1 : kWhole / 2));
     int64_t u = (int64_t)blockIdx.x * share;
-    const int64_t u_end = min(u + share, total);
-    for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x)  // requests with nothing to look at
-        if (span_of(a, b).tiles == 0)
-            for (int64_t i = threadIdx.x; i < a.q_heads * D; i += kThreads) srv_store1(QT, a.out, b * a.out_stride + i, 0.0f);
-    if (u >= total) return;
-    const uint64_t later = __builtin_amdgcn_ballot_w64(upto * sh.units > u);
-    const int at_lane = __builtin_ctzll(later);
-    int64_t b = at_lane * strip, rem = u - wave_at64(upto - own, at_lane) * sh.units;
-    Span sp = span_of(a, b);
-    while (rem >= sp.tiles * sh.units) {
-        rem -= sp.tiles * sh.units;
-        sp = span_of(a, ++b);
+    const int64_t u_end = min(u + share, lists ? a.batch * sh.units : total);
+    if (u >= u_end) return;
+    int64_t b, unit;
+    int t0 = 0;
+    Span sp;
+    if (lists) {
+        b = div_short(u, sh.units);
+        unit = u - b * sh.units;
+        for (sp = span_at(b); sp.tiles == 0; sp = span_at(++b)) {
+            u += sh.units - unit;
+            unit = 0;
+            if (u >= u_end) return;
+        }
+    } else {
+        const int at_lane = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto * sh.units > u));
+        int64_t rem = u - uniform(wave_at64(upto - own, at_lane)) * sh.units;
+        b = at_lane * strip;
+        sp = span_at(b);
+        while (rem >= sp.tiles * sh.units) {
+            rem -= sp.tiles * sh.units;
+            sp = span_at(++b);
+        }
+        unit = div_short(rem, sp.tiles);
+        t0 = (int)(rem - unit * sp.tiles);
     }
 
-    while (u < u_end) {
-        const int64_t unit = rem / sp.tiles, t0 = rem - unit * sp.tiles;
-        const int64_t t1 = min(sp.tiles, t0 + (u_end - u));
-        const int64_t kv = unit / sh.parts;
+    for (;;) {
+        const int t1 = lists ? sp.tiles : (int)min((int64_t)sp.tiles, t0 + (u_end - u));
+        const int64_t kv = sh.parts == 1 ? unit : div_short(unit, sh.parts);
         const int g0 = (int)(unit - kv * sh.parts) * 16, gn = min(16, sh.group - g0);
         const int64_t head0 = kv * sh.group + g0;
 
@@ -232,14 +274,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
         for (int j = 0; j < kOut; ++j) o[j] = floatx4{0, 0, 0, 0};
 
         // ---- the tiles: lane % 32 looks up a token's row
-        auto block_of = [&](int64_t t) {
-            const int64_t tok = sp.first + t * kTile + (lane & 31);
+        auto block_of = [&](int t) {
+            const int64_t tok = sp.first + (int64_t)t * kTile + (lane & 31);
             if (t >= t1 || tok >= sp.len) return -1;
             return a.block_table[b * a.table_stride + (uint32_t)tok / (uint32_t)P];
         };
         int block = block_of(t0 + wave);
-        for (int64_t t = t0 + wave; t < t1; t += kWaves) {
-            const uint32_t tok = (uint32_t)(sp.first + t * kTile + (lane & 31));
+        for (int t = t0 + wave; t < t1; t += kWaves) {
+            const uint32_t tok = (uint32_t)(sp.first + (int64_t)t * kTile + (lane & 31));
             const bool live = block >= 0 && block < a.n_blocks;
             const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(live);
             // (a token no one may look at reads the cache's first row)
@@ -374,12 +416,26 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
         }
         __syncthreads();
         const bool whole = t1 - t0 == sp.tiles;
-        const int64_t slot_floats = (int64_t)sh.heads * (D + 2);
-        // this unit's tiles are [u - t0, u - t0 + tiles) of the list
-        const int64_t u_first = u - t0, w_first = u_first / share, w_last = (u_first + sp.tiles - 1) / share;
-        auto slot = [&](int64_t w) { return sh.partials + (2 * w + (u_first < w * share ? 0 : 1)) * slot_floats; };
+        const int slot_floats = sh.heads * (int)(D + 2);
+        // this unit's tiles are [u - t0, u - t0 + tiles) of the list; a workgroup's first part
+        // that began before its share has its first slot, one that goes on past it the second
+        const int64_t u_first = u - t0;
+        auto slot_of = [&](int64_t w) { return 2 * w + (u_first < w * share ? 0 : 1); };
+        // a value of the unit's result: to the output, or as a part to the workspace
+        auto put = [&](bool last, float *part, int g, int d, float v, float sum_m, float sum_l) {
+            if (last) {
+                srv_store1(QT, a.out, b * a.out_stride + (head0 + g) * D + d, sum_l == 0.0f ? 0.0f : v / sum_l);
+            } else {
+                xchg_store(part + g * (int)D + d, v);
+                if (d == 0) {
+                    xchg_store(part + sh.heads * (int)D + 2 * g, sum_m);
+                    xchg_store(part + sh.heads * (int)D + 2 * g + 1, sum_l);
+                }
+            }
+        };
+        float *part = sh.partials + slot_of(blockIdx.x) * slot_floats;
         for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
-            const int g = i / (int)D, d = i - g * (int)D;
+            const int g = (int)((uint32_t)i / (uint32_t)D), d = i - g * (int)D;
             float sum_m = wave_m[0][g], sum_l = 0.0f, v = 0.0f;
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) sum_m = fmaxf(sum_m, wave_m[w][g]);
@@ -388,50 +444,66 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                 v += wave_o[(w * sh.heads + g) * DP + d];
                 sum_l += wave_l[w][g] * rescale(wave_m[w][g], sum_m);
             }
-            if (whole) {
-                srv_store1(QT, a.out, b * a.out_stride + (head0 + g) * D + d, sum_l == 0.0f ? 0.0f : v / sum_l);
-            } else {
-                float *to = slot(blockIdx.x);
-                xchg_store(to + g * D + d, v);
-                if (d == 0) {
-                    xchg_store(to + sh.heads * D + g, sum_m);
-                    xchg_store(to + sh.heads * (D + 1) + g, sum_l);
-                }
-            }
+            put(whole, part, g, d, v, sum_m, sum_l);
         }
         if (!whole) {
-            unsigned *counter = sh.counters + b * sh.units + unit;
-            if (xchg_arrive(counter, &arrived) == (unsigned)(w_last - w_first)) {
+            // Parts are joined in groups of kFan, the groups' sums in groups again: what
+            // one workgroup reads, parts and heads alike, is a few round trips.
+            const int64_t w_first = div_short(u_first, share);
+            int n = (int)(div_short(u_first + sp.tiles - 1, share) - w_first + 1), at = (int)(blockIdx.x - w_first), stride = 1;
+            for (int level = 0; n > 1; ++level) {
+                const int first = at / kFan * kFan, size = min(kFan, n - first);
+                auto part_at = [&](int k) { return sh.partials + slot_of(w_first + (int64_t)(first + k) * stride) * slot_floats; };
+                unsigned *counter = sh.counters + ((int64_t)level << (sh.grid_log2 + 1)) + slot_of(w_first + (int64_t)first * stride);
+                if (xchg_arrive(counter, &arrived) != (unsigned)(size - 1)) break;
                 xchg_reset(counter);
-                for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
-                    const int g = i / (int)D, d = i - g * (int)D;
-                    float sum_m = -INFINITY, sum_l = 0.0f, v = 0.0f;
-#pragma unroll 8
-                    for (int64_t w = w_first; w <= w_last; ++w) sum_m = fmaxf(sum_m, xchg_load(slot(w) + sh.heads * D + g));
-#pragma unroll 4
-                    for (int64_t w = w_first; w <= w_last; ++w) {
-                        const float *from = slot(w);
-                        const float r = rescale(xchg_load(from + sh.heads * D + g), sum_m);
-                        sum_l += r * xchg_load(from + sh.heads * (D + 1) + g);
-                        v += r * xchg_load(from + g * D + d);
-                    }
-                    srv_store1(QT, a.out, b * a.out_stride + (head0 + g) * D + d, sum_l == 0.0f ? 0.0f : v / sum_l);
+                for (int i = threadIdx.x; i < size * gn; i += kThreads) {
+                    const int k = (int)((uint32_t)i / (uint32_t)gn), g = i - k * gn;
+                    const float *from = part_at(k) + sh.heads * (int)D + 2 * g;
+                    part_m[k][g] = xchg_load(from);
+                    part_l[k][g] = xchg_load(from + 1);
                 }
+                __syncthreads();
+                n = (n + kFan - 1) / kFan;
+                at /= kFan;
+                part = part_at(0);
+                for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
+                    const int g = (int)((uint32_t)i / (uint32_t)D), d = i - g * (int)D;
+                    float o_part[kFan], sum_m = -INFINITY, sum_l = 0.0f, v = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kFan; ++k) o_part[k] = xchg_load(part_at(min(k, size - 1)) + g * (int)D + d);
+                    for (int k = 0; k < size; ++k) sum_m = fmaxf(sum_m, part_m[k][g]);
+#pragma unroll
+                    for (int k = 0; k < kFan; ++k)
+                        if (k < size) {
+                            const float r = rescale(part_m[k][g], sum_m);
+                            sum_l += r * part_l[k][g];
+                            v += r * o_part[k];
+                        }
+                    put(n == 1, part, g, d, v, sum_m, sum_l);
+                }
+                stride *= kFan;
             }
         }
+        // ---- the next list
+        u += lists ? 1 : t1 - t0;
+        if (u >= u_end) return;
         __syncthreads();  // LDS is written again
-
-        u += t1 - t0;
-        rem += t1 - t0;
-        if (rem == sp.tiles * sh.units && u < u_end) {
-            rem = 0;
-            do sp = span_of(a, ++b);
-            while (sp.tiles == 0);
+        t0 = 0;
+        if (++unit == sh.units) {
+            unit = 0;
+            for (sp = span_at(++b); sp.tiles == 0; sp = span_at(++b))
+                if (lists && (u += sh.units) >= u_end) return;
         }
     }
 }
 
-int64_t workgroups() { return 2 * (int64_t)device_cus(); }
+// Workgroups: a power of two, the largest of which two fit each CU.
+int workgroups_log2() {
+    const unsigned n = 2 * (unsigned)std::max(1, device_cus());
+    return std::min(31 - __builtin_clz(n), 4 * kLevels);
+}
+int64_t workgroups() { return (int64_t)1 << workgroups_log2(); }
 
 AttnShape shape_of(const PagedAttentionArgs &a) {
     AttnShape sh{};
@@ -439,7 +511,8 @@ AttnShape shape_of(const PagedAttentionArgs &a) {
     sh.parts = (sh.group + 15) / 16;
     sh.heads = std::min(sh.group, 16);
     sh.units = a.kv_heads * sh.parts;
-    sh.min_share = 8;  // two tiles a wave: below that a part costs more to join than to read
+    sh.positions = a.table_width * a.block_size;
+    sh.grid_log2 = workgroups_log2();
     return sh;
 }
 
@@ -495,7 +568,7 @@ void paged_attention_workspace_need(const PagedAttentionArgs &a, size_t *partial
     if (attn_empty(a)) return;
     const AttnShape sh = shape_of(a);
     *partial_floats = (size_t)(2 * workgroups() * sh.heads * (a.head_dim + 2));
-    *counters = (size_t)(a.batch * sh.units);
+    *counters = (size_t)(kLevels * 2 * workgroups());
 }
 
 Status launch_paged_attention(const PagedAttentionArgs &in, const Workspace &ws, hipStream_t s) {
