@@ -306,6 +306,10 @@ template <typename T>
 inline T __builtin_amdgcn_readfirstlane(T v) {
     return v;
 }
+template <typename T>
+inline T __builtin_amdgcn_readlane(T v, int) {
+    return v;
+}
 inline bool tml_emu_mfma_nan = false;  // the bf16 matrix cores' sums are NaN
 inline tml_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x4f32(float, float, tml_emu_f32x4 c, int, int, int) { return c; }
 typedef __bf16 tml_emu_bf16x8 __attribute__((ext_vector_type(8)));

@@ -31,9 +31,8 @@
 // workgroups share evenly: each sums the requests' lengths itself, so the split goes
 // by the lengths as they are on the GPU, ragged or not, without the host.  A
 // workgroup's share is some whole heads and at most two parts of one; its waves take
-// the tiles in turn and join in LDS.  Parts go to the workspace; the last workgroup
-// to arrive at a head adds them up, in their order, so the result does not depend on
-// who was last.
+// the tiles in turn and join in LDS.  Parts go to the workspace, and a second, small
+// kernel adds them up in their order.
 #include "serving.hpp"
 
 #include <algorithm>
@@ -48,8 +47,12 @@ typedef int64_t offx2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = kWaves * 64;
 constexpr int kTile = 32;  // tokens a wave takes at a time
-constexpr int kFan = 16, kLevels = 3;  // parts joined at a time, how often: kFan^kLevels workgroups at most
 constexpr int kWhole = 16;  // tiles of a list that is not split: four a wave
+
+// A list's parts: the workgroup of the first, how many; none where the list is whole.
+struct ListParts {
+    int first, count;
+};
 
 struct AttnShape {
     int group;      // query heads of a key-value head
@@ -58,8 +61,9 @@ struct AttnShape {
     int64_t units;  // key-value heads * parts: a request's lists of tiles
     int64_t positions;  // of a table row
     int grid_log2;  // workgroups
-    float *partials;
-    unsigned *counters;
+    int part_floats;  // of a part: 16-head part's values, maxima and sums
+    float *partials;  // two parts a workgroup
+    ListParts *lists;  // [batch][units], or nullptr: no list can be long enough to be split
 };
 
 // Values alike in every lane, for the compiler to keep in scalar registers.
@@ -97,6 +101,15 @@ __device__ __forceinline__ Span span_of(const PagedAttentionArgs &a, const AttnS
 // What a part whose maximum is m is multiplied with where the whole's is top.  A
 // part without a maximum holds zeros, or the NaN of scores that are none.
 __device__ __forceinline__ float rescale(float m, float top) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+
+// Elements d and d + 1 of a head's output.
+template <int QT>
+__device__ __forceinline__ void store_result(const PagedAttentionArgs &a, int64_t b, int64_t head, int d, srv_f32x2 sum, float sum_l) {
+    const float r = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
+    const int64_t to = b * a.out_stride + head * a.head_dim + d;
+    srv_store1(QT, a.out, to, sum[0] * r);
+    srv_store1(QT, a.out, to + 1, sum[1] * r);
+}
 
 template <int CT>
 __device__ __forceinline__ floatx4 mma16(const srv_u32x4 &x, const srv_u32x4 &y, floatx4 c) {
@@ -146,8 +159,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
 
     __shared__ __align__(16) int64_t row_off[kWaves][kTile];
     __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
-    __shared__ float part_m[kFan][16], part_l[kFan][16];
-    __shared__ unsigned arrived;
     TML_DYNAMIC_LDS(floatx4, dyn);
     float *const wave_o = (float *)dyn;  // [wave][head][DP]
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
@@ -174,8 +185,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
     auto span_at = [&](int64_t r) { return span_of(a, sh, uniform(a.seq_len[r])); };
     if (__builtin_amdgcn_ballot_w64(none) != 0)  // requests with nothing to look at
         for (int64_t r = blockIdx.x; r < a.batch; r += gridDim.x)
-            if (span_at(r).tiles == 0)
+            if (span_at(r).tiles == 0) {
+                if (sh.lists != nullptr)
+                    for (int64_t i = threadIdx.x; i < sh.units; i += kThreads) sh.lists[r * sh.units + i] = ListParts{0, 0};
                 for (int i = threadIdx.x; i < (int)(a.q_heads * D); i += kThreads) srv_store1(QT, a.out, r * a.out_stride + i, 0.0f);
+            }
     const int64_t total = uniform(wave_at64(upto, 63)) * sh.units;
     if (total == 0) return;
     // Lists of so few tiles that a part costs more to join than to read stay whole:
@@ -274,33 +288,34 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
         for (int j = 0; j < kOut; ++j) o[j] = floatx4{0, 0, 0, 0};
 
         // ---- the tiles: lane % 32 looks up a token's row
-        auto block_of = [&](int t) {
-            const int64_t tok = sp.first + (int64_t)t * kTile + (lane & 31);
-            if (t >= t1 || tok >= sp.len) return -1;
-            return a.block_table[b * a.table_stride + (uint32_t)tok / (uint32_t)P];
+        auto block_of = [&](int tile) {
+            const int64_t tok = sp.first + (int64_t)tile * kTile + (lane & 31);
+            return a.block_table[b * a.table_stride + (uint32_t)min(tok, sp.len - 1) / (uint32_t)P];
         };
-        int block = block_of(t0 + wave);
-        for (int t = t0 + wave; t < t1; t += kWaves) {
-            const uint32_t tok = (uint32_t)(sp.first + (int64_t)t * kTile + (lane & 31));
-            const bool live = block >= 0 && block < a.n_blocks;
-            const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(live);
+        // the byte offset of each token's row to LDS; which of the 32 may be looked at
+        auto rows_of = [&](int tile, int in_block) {
+            const int64_t tok = sp.first + (int64_t)tile * kTile + (lane & 31);
+            const bool live = tile < t1 && tok < sp.len && in_block >= 0 && in_block < a.n_blocks;
             // (a token no one may look at reads the cache's first row)
-            const int64_t off = live ? (block * a.block_stride + (int64_t)(tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes : 0;
+            const int64_t off = live ? (in_block * a.block_stride + (int64_t)((uint32_t)tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes : 0;
             row_off[wave][lane & 31] = off;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            block = block_of(t + kWaves);
-
-            srv_u32x4 k[2][kChunks], v[8][kHalves];
+            return (uint32_t)__builtin_amdgcn_ballot_w64(live);
+        };
+        srv_u32x4 kr[2][kChunks], vr[8][kHalves];
+        auto load_k = [&]() {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const char *row = (const char *)a.k_cache + row_off[wave][16 * h + l16];
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
                     const int d = c * kChunk + (kChunk / 4) * c4;
-                    k[h][c] = *(const srv_u32x4 *)(row + (d < D ? d : 0) * kBytes);
+                    kr[h][c] = *(const srv_u32x4 *)(row + (d < D ? d : 0) * kBytes);
                 }
             }
+        };
+        auto load_v = [&]() {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const char *row = (const char *)a.v_cache + row_off[wave][16 * (e / 4) + 4 * c4 + e % 4];
@@ -309,16 +324,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                     const int d = f * 16 * E + E * l16;
                     const char *at = row + (d < D ? d : 0) * kBytes;
                     if constexpr (E * kBytes == 16) {
-                        v[e][f] = *(const srv_u32x4 *)at;
+                        vr[e][f] = *(const srv_u32x4 *)at;
                     } else {
-                        const srv_u32x2 w = *(const srv_u32x2 *)at;
-                        v[e][f] = srv_u32x4{w[0], w[1], 0, 0};
+                        const srv_u32x2 half = *(const srv_u32x2 *)at;
+                        vr[e][f] = srv_u32x4{half[0], half[1], 0, 0};
                     }
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+        };
 
+        // Keys of the next tile are under way from this tile's scores on, values from
+        // its sums on, each into the registers just read.  (No branch around these
+        // loads, or the wait for one would be a wait for all: past the last tile they
+        // read the cache's first row.)
+        int t = t0 + wave;
+        uint32_t seen = rows_of(t, block_of(t));
+        load_k();
+        int block = block_of(t + kWaves);  // (in the loop's order)
+        __builtin_amdgcn_sched_barrier(0);
+        load_v();
+        while (t < t1) {
             // scores
             float s[8];
 #pragma unroll
@@ -329,15 +356,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                     if constexpr (kF32) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h][c][e]), __uint_as_float(q[0][c][e]), acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[h][c][e]), __uint_as_float(q[0][c][e]), acc, 0, 0, 0);
                     } else {
 #pragma unroll
-                        for (int n = 0; n < NQ; ++n) acc = mma16<CT>(k[h][c], q[n][c], acc);
+                        for (int n = 0; n < NQ; ++n) acc = mma16<CT>(kr[h][c], q[n][c], acc);
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * h + i] = (seen >> (16 * h + 4 * c4 + i) & 1) ? acc[i] * to_log2 : -INFINITY;
             }
+            t += kWaves;
+            const uint32_t seen_now = seen;
+            seen = rows_of(t, block);
+            load_k();
+            block = block_of(t + kWaves);
             float most = s[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
@@ -359,12 +391,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                 l += p[e];
             }
             // what no one may look at can be anything, and zero times NaN is NaN
-            if (seen != 0xFFFFFFFFu) {
+            if (seen_now != 0xFFFFFFFFu) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if ((seen >> (16 * (e / 4) + 4 * c4 + e % 4) & 1) == 0)
+                    if ((seen_now >> (16 * (e / 4) + 4 * c4 + e % 4) & 1) == 0)
 #pragma unroll
-                        for (int f = 0; f < kHalves; ++f) v[e][f] = srv_u32x4{0, 0, 0, 0};
+                        for (int f = 0; f < kHalves; ++f) vr[e][f] = srv_u32x4{0, 0, 0, 0};
             }
             if constexpr (kF32) {
 #pragma unroll
@@ -373,7 +405,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                     for (int j = 0; j < E; ++j)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            o[f * E + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e][f][j]), p[e], o[f * E + j], 0, 0, 0);
+                            o[f * E + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[e][f][j]), p[e], o[f * E + j], 0, 0, 0);
             } else {
                 srv_u32x4 w[NP];
                 to_terms<CT, NP>(p, w);
@@ -384,11 +416,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                         srv_u32x4 vt;  // d = .. + j of the eight tokens
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            vt[e] = __builtin_amdgcn_perm(v[2 * e + 1][f][j / 2], v[2 * e][f][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+                            vt[e] = __builtin_amdgcn_perm(vr[2 * e + 1][f][j / 2], vr[2 * e][f][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                         for (int n = 0; n < NP; ++n) o[f * E + j] = mma16<CT>(vt, w[n], o[f * E + j]);
                     }
             }
+            load_v();
         }
 
         // ---- the waves' parts
@@ -415,76 +448,34 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                 }
         }
         __syncthreads();
+        // The whole list's result goes to the output, a part's to the workspace: [heads][D]
+        // values, then each head's maximum and sum.  The workgroup that a list begins in
+        // has it in its second slot, those it goes on in in their first.
         const bool whole = t1 - t0 == sp.tiles;
-        const int slot_floats = sh.heads * (int)(D + 2);
-        // this unit's tiles are [u - t0, u - t0 + tiles) of the list; a workgroup's first part
-        // that began before its share has its first slot, one that goes on past it the second
-        const int64_t u_first = u - t0;
-        auto slot_of = [&](int64_t w) { return 2 * w + (u_first < w * share ? 0 : 1); };
-        // a value of the unit's result: to the output, or as a part to the workspace
-        auto put = [&](bool last, float *part, int g, int d, float v, float sum_m, float sum_l) {
-            if (last) {
-                srv_store1(QT, a.out, b * a.out_stride + (head0 + g) * D + d, sum_l == 0.0f ? 0.0f : v / sum_l);
-            } else {
-                xchg_store(part + g * (int)D + d, v);
-                if (d == 0) {
-                    xchg_store(part + sh.heads * (int)D + 2 * g, sum_m);
-                    xchg_store(part + sh.heads * (int)D + 2 * g + 1, sum_l);
-                }
-            }
-        };
-        float *part = sh.partials + slot_of(blockIdx.x) * slot_floats;
-        for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
-            const int g = (int)((uint32_t)i / (uint32_t)D), d = i - g * (int)D;
-            float sum_m = wave_m[0][g], sum_l = 0.0f, v = 0.0f;
+        const int row2 = (int)D / 2;
+        float *const part = sh.partials + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * sh.part_floats;
+        for (int i = threadIdx.x; i < gn * row2; i += kThreads) {
+            const int g = (int)((uint32_t)i / (uint32_t)row2), d = 2 * (i - g * row2);
+            float sum_m = wave_m[0][g], sum_l = 0.0f;
+            srv_f32x2 sum = {0.0f, 0.0f};
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) sum_m = fmaxf(sum_m, wave_m[w][g]);
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                v += wave_o[(w * sh.heads + g) * DP + d];
+                sum += *(const srv_f32x2 *)(wave_o + (w * sh.heads + g) * DP + d);
                 sum_l += wave_l[w][g] * rescale(wave_m[w][g], sum_m);
             }
-            put(whole, part, g, d, v, sum_m, sum_l);
-        }
-        if (!whole) {
-            // Parts are joined in groups of kFan, the groups' sums in groups again: what
-            // one workgroup reads, parts and heads alike, is a few round trips.
-            const int64_t w_first = div_short(u_first, share);
-            int n = (int)(div_short(u_first + sp.tiles - 1, share) - w_first + 1), at = (int)(blockIdx.x - w_first), stride = 1;
-            for (int level = 0; n > 1; ++level) {
-                const int first = at / kFan * kFan, size = min(kFan, n - first);
-                auto part_at = [&](int k) { return sh.partials + slot_of(w_first + (int64_t)(first + k) * stride) * slot_floats; };
-                unsigned *counter = sh.counters + ((int64_t)level << (sh.grid_log2 + 1)) + slot_of(w_first + (int64_t)first * stride);
-                if (xchg_arrive(counter, &arrived) != (unsigned)(size - 1)) break;
-                xchg_reset(counter);
-                for (int i = threadIdx.x; i < size * gn; i += kThreads) {
-                    const int k = (int)((uint32_t)i / (uint32_t)gn), g = i - k * gn;
-                    const float *from = part_at(k) + sh.heads * (int)D + 2 * g;
-                    part_m[k][g] = xchg_load(from);
-                    part_l[k][g] = xchg_load(from + 1);
-                }
-                __syncthreads();
-                n = (n + kFan - 1) / kFan;
-                at /= kFan;
-                part = part_at(0);
-                for (int i = threadIdx.x; i < gn * (int)D; i += kThreads) {
-                    const int g = (int)((uint32_t)i / (uint32_t)D), d = i - g * (int)D;
-                    float o_part[kFan], sum_m = -INFINITY, sum_l = 0.0f, v = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < kFan; ++k) o_part[k] = xchg_load(part_at(min(k, size - 1)) + g * (int)D + d);
-                    for (int k = 0; k < size; ++k) sum_m = fmaxf(sum_m, part_m[k][g]);
-#pragma unroll
-                    for (int k = 0; k < kFan; ++k)
-                        if (k < size) {
-                            const float r = rescale(part_m[k][g], sum_m);
-                            sum_l += r * part_l[k][g];
-                            v += r * o_part[k];
-                        }
-                    put(n == 1, part, g, d, v, sum_m, sum_l);
-                }
-                stride *= kFan;
+            if (whole) {
+                store_result<QT>(a, b, head0 + g, d, sum, sum_l);
+            } else {
+                *(srv_f32x2 *)(part + g * (int)D + d) = sum;
+                if (d == 0) *(srv_f32x2 *)(part + sh.heads * (int)D + 2 * g) = srv_f32x2{sum_m, sum_l};
             }
         }
+        // where the list's parts are, for the kernel that joins them
+        if (sh.lists != nullptr && t0 == 0 && threadIdx.x == 0)
+            sh.lists[b * sh.units + unit] = whole ? ListParts{0, 0} : ListParts{(int)blockIdx.x, (int)(div_short(u + sp.tiles - 1, share) - blockIdx.x) + 1};
+
         // ---- the next list
         u += lists ? 1 : t1 - t0;
         if (u >= u_end) return;
@@ -498,11 +489,58 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
     }
 }
 
-// Workgroups: a power of two, the largest of which two fit each CU.
-int workgroups_log2() {
-    const unsigned n = 2 * (unsigned)std::max(1, device_cus());
-    return std::min(31 - __builtin_clz(n), 4 * kLevels);
+// Adds a list's parts up, in their order; a wave a query head, its lanes first the
+// parts' maxima and sums, 64 at a time, then pairs of d.
+constexpr int kJoinWaves = 4, kJoinBatch = 16;
+template <int QT>
+__global__ __launch_bounds__(64 * kJoinWaves) void paged_attention_join_kernel(PagedAttentionArgs a, AttnShape sh) {
+    const int lane = threadIdx.x & 63;
+    const int head = (int)blockIdx.x * kJoinWaves + uniform((int)(threadIdx.x >> 6));
+    const int64_t b = blockIdx.y;
+    if (head >= (int)a.q_heads) return;
+    const int kv = (int)((uint32_t)head / (uint32_t)sh.group), in_group = head - kv * sh.group, g = in_group & 15;
+    const ListParts list = sh.lists[b * sh.units + kv * sh.parts + (in_group >> 4)];
+    const int count = uniform(list.count), D = (int)a.head_dim;
+    if (count == 0) return;
+    const float *const first = sh.partials + (2 * (int64_t)uniform(list.first) + 1) * sh.part_floats;
+    // (later parts are in their workgroups' first slots)
+    auto part_of = [&](int i) { return i == 0 ? first : first + (2 * (int64_t)i - 1) * sh.part_floats; };
+    float sum_m = -INFINITY, sum_l = 0.0f;
+    srv_f32x2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};  // pairs lane and lane + 64
+    for (int i0 = 0; i0 < count; i0 += 64) {
+        const int n = min(64, count - i0);
+        const srv_f32x2 ml = *(const srv_f32x2 *)(part_of(i0 + min(lane, n - 1)) + sh.heads * D + 2 * g);
+        float peak = fmaxf(ml[0], sum_m);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+        const float before = rescale(sum_m, peak), r = lane < n ? rescale(ml[0], peak) : 0.0f;
+        sum_m = peak;
+        sum_l = sum_l * before + (lane < n ? r * ml[1] : 0.0f);  // (a lane's own parts)
+        sum[0] *= before;
+        sum[1] *= before;
+        for (int i = 0; i < n; i += kJoinBatch) {  // (past the last part: its values again, times zero)
+            srv_f32x2 v[kJoinBatch];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (128 * half >= D) break;
+                const int d = 2 * lane + 128 * half;
+#pragma unroll
+                for (int j = 0; j < kJoinBatch; ++j)
+                    v[j] = *(const srv_f32x2 *)(part_of(i0 + min(i + j, n - 1)) + g * D + (d < D ? d : 0));
+#pragma unroll
+                for (int j = 0; j < kJoinBatch; ++j)
+                    sum[half] += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(r), i + j)) * v[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum_l += __shfl_xor(sum_l, o);
+    if (2 * lane < D) store_result<QT>(a, b, head, 2 * lane, sum[0], sum_l);
+    if (2 * lane + 128 < D) store_result<QT>(a, b, head, 2 * lane + 128, sum[1], sum_l);
 }
+
+// Workgroups: a power of two, the largest of which two fit each CU.
+int workgroups_log2() { return 31 - __builtin_clz(2 * (unsigned)std::max(1, device_cus())); }
 int64_t workgroups() { return (int64_t)1 << workgroups_log2(); }
 
 AttnShape shape_of(const PagedAttentionArgs &a) {
@@ -513,11 +551,18 @@ AttnShape shape_of(const PagedAttentionArgs &a) {
     sh.units = a.kv_heads * sh.parts;
     sh.positions = a.table_width * a.block_size;
     sh.grid_log2 = workgroups_log2();
+    sh.part_floats = sh.heads * (int)(a.head_dim + 2);
     return sh;
 }
 
 bool attn_empty(const PagedAttentionArgs &a) {
     return a.batch <= 0 || a.q_heads <= 0 || a.kv_heads <= 0 || a.head_dim <= 0;
+}
+
+// Whether a list may be long enough to be split.
+bool may_split(const PagedAttentionArgs &a) {
+    const int64_t positions = a.table_width * a.block_size;
+    return (a.window > 0 ? std::min(positions, a.window) : positions) > kWhole * kTile;
 }
 
 template <int CT, int QT>
@@ -528,6 +573,9 @@ Status launch_dim(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t 
     if (dp == 64) paged_attention_kernel<CT, QT, 64><<<grid, block, lds, s>>>(a, sh);
     else if (dp == 128) paged_attention_kernel<CT, QT, 128><<<grid, block, lds, s>>>(a, sh);
     else paged_attention_kernel<CT, QT, 256><<<grid, block, lds, s>>>(a, sh);
+    TML_HIP_TRY(hipGetLastError());
+    if (sh.lists == nullptr) return Status::Ok();
+    paged_attention_join_kernel<QT><<<dim3((unsigned)((a.q_heads + kJoinWaves - 1) / kJoinWaves), (unsigned)a.batch), dim3(64 * kJoinWaves), 0, s>>>(a, sh);
     TML_HIP_TRY(hipGetLastError());
     return Status::Ok();
 }
@@ -546,9 +594,9 @@ Status check_paged_attention(const PagedAttentionArgs &a) {
     if (a.head_dim % 8 != 0 || a.head_dim > 256)
         return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: the head size must be a multiple of 8, at most 256");
     const int64_t most = (int64_t)1 << 31;
-    if (a.n_blocks >= most || a.block_size >= most || a.batch >= (1 << 20) || a.q_heads >= (1 << 16) ||
+    if (a.n_blocks >= most || a.block_size >= most || a.batch >= (1 << 16) || a.q_heads >= (1 << 16) ||
         a.table_width >= most || a.table_width * a.block_size > most)
-        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: at most 2^20 requests, 2^16 heads and 2^31 positions of a table");
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: at most 2^16 requests, 2^16 heads and 2^31 positions of a table");
     if (a.q == nullptr || a.out == nullptr || a.seq_len == nullptr || (a.n_blocks > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) ||
         (a.table_width > 0 && a.block_table == nullptr))
         return Status::Err(TML_ERR_INVALID_ARG, "null pointer");
@@ -563,12 +611,10 @@ Status check_paged_attention(const PagedAttentionArgs &a) {
     return Status::Ok();
 }
 
-void paged_attention_workspace_need(const PagedAttentionArgs &a, size_t *partial_floats, size_t *counters) {
-    *partial_floats = *counters = 0;
-    if (attn_empty(a)) return;
+size_t paged_attention_workspace_floats(const PagedAttentionArgs &a) {
+    if (attn_empty(a) || !may_split(a)) return 0;
     const AttnShape sh = shape_of(a);
-    *partial_floats = (size_t)(2 * workgroups() * sh.heads * (a.head_dim + 2));
-    *counters = (size_t)(kLevels * 2 * workgroups());
+    return (size_t)(2 * workgroups() * sh.part_floats + 2 * a.batch * sh.units);
 }
 
 Status launch_paged_attention(const PagedAttentionArgs &in, const Workspace &ws, hipStream_t s) {
@@ -576,11 +622,12 @@ Status launch_paged_attention(const PagedAttentionArgs &in, const Workspace &ws,
     if (attn_empty(a)) return Status::Ok();
     if (a.n_blocks == 0) a.table_width = 0;  // no cache: nothing to look at
     AttnShape sh = shape_of(a);
-    size_t pf, nc;
-    paged_attention_workspace_need(a, &pf, &nc);
-    if (ws.partial_floats < pf || ws.counter_count < nc) return Status::Err(TML_ERR_INVALID_ARG, "paged attention: workspace too small");
-    sh.partials = ws.partials;
-    sh.counters = ws.counters;
+    if (may_split(a)) {
+        if (ws.partial_floats < paged_attention_workspace_floats(a))
+            return Status::Err(TML_ERR_INVALID_ARG, "paged attention: workspace too small");
+        sh.partials = ws.partials;
+        sh.lists = (ListParts *)(ws.partials + 2 * workgroups() * sh.part_floats);
+    }
     if (a.cache_type == TML_TYPE_F32) return launch_dim<TML_TYPE_F32, TML_TYPE_F32>(a, sh, s);
     if (a.cache_type == TML_TYPE_F16)
         return a.q_type == TML_TYPE_F32 ? launch_dim<TML_TYPE_F16, TML_TYPE_F32>(a, sh, s) : launch_dim<TML_TYPE_F16, TML_TYPE_F16>(a, sh, s);

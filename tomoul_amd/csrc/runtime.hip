@@ -306,29 +306,20 @@ Status ensure_workspace(DeviceCtx *c, MatmulArgs &m, hipStream_t s, Workspace *w
     return Status::Ok();
 }
 
-// The same for the paged attention's parts.
+// The same for the paged attention's parts, which need no counters.
 Status attention_workspace(DeviceCtx *c, const PagedAttentionArgs &a, hipStream_t s, Workspace *ws) {
-    size_t pf = 0, nc = 0;
-    paged_attention_workspace_need(a, &pf, &nc);
-    const bool grow_ctr = nc * sizeof(unsigned) > c->counters.bytes;
-    if (pf * sizeof(float) > c->ws.bytes || grow_ctr) {
+    const size_t bytes = paged_attention_workspace_floats(a) * sizeof(float);
+    if (bytes > c->ws.bytes) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
         TML_HIP_TRY(hipStreamIsCapturing(s, &cap));
         if (cap != hipStreamCaptureStatusNone)
             return Status::Err(TML_ERR_INVALID_ARG,
                                "the workspace must grow during stream capture: run this call once eagerly (outside "
                                "capture) before capturing it");
-        TML_TRY(c->ws.ensure(pf * sizeof(float)));
-        if (grow_ctr) {
-            TML_TRY(c->counters.ensure(nc * sizeof(unsigned)));
-            TML_HIP_TRY(hipMemsetAsync(c->counters.p, 0, c->counters.bytes, s));
-            TML_HIP_TRY(hipStreamSynchronize(s));
-        }
+        TML_TRY(c->ws.ensure(bytes));
     }
     ws->partials = (float *)c->ws.p;
     ws->partial_floats = c->ws.bytes / sizeof(float);
-    ws->counters = (unsigned *)c->counters.p;
-    ws->counter_count = c->counters.bytes / sizeof(unsigned);
     return Status::Ok();
 }
 

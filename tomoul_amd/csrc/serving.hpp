@@ -157,7 +157,7 @@ struct PagedAttentionArgs {
     int64_t out_stride;
 };
 Status check_paged_attention(const PagedAttentionArgs &a);
-void paged_attention_workspace_need(const PagedAttentionArgs &a, size_t *partial_floats, size_t *counters);
+size_t paged_attention_workspace_floats(const PagedAttentionArgs &a);
 Status launch_paged_attention(const PagedAttentionArgs &a, const Workspace &ws, hipStream_t s);
 
 }  // namespace tml
