@@ -33,6 +33,12 @@
 // workgroup's share is some whole heads and at most two parts of one; its waves take
 // the tiles in turn and join in LDS.  Parts go to the workspace, and a second, small
 // kernel adds them up in their order.
+//
+// Measured on MI355X (launches in a graph): bf16, 64 requests of up to 4096 tokens, 32
+// heads on 8 of 128 112 us (4.8 TB/s); f16, two of 40k to 65k tokens 68 us (5.5 TB/s); f32 q,
+// f16 cache, one of 448 tokens, 20 heads of 64 8.2 us, of 1500 14.1 us; one of 20 tokens
+// 5.4 us.  Long ones are bound by memory, short ones by the chain of dependent loads:
+// lengths, table, rows.
 #include "serving.hpp"
 
 #include <algorithm>
@@ -141,10 +147,18 @@ __device__ __forceinline__ void to_terms(float (&v)[8], srv_u32x4 (&t)[N]) {
         }
 }
 
+// 16 bytes of the cache.  ONCE: with the streaming policy, which leaves the
+// caches to others.
+template <bool ONCE>
+__device__ __forceinline__ srv_u32x4 load_cache(const char *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load((const srv_u32x4 *)p);
+    else return *(const srv_u32x4 *)p;
+}
+
 // CT: the cache's type.  QT: q's and the output's (CT or f32).  DP: the head size
 // rounded up to 64, 128 or 256.
-template <int CT, int QT, int DP>
-__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttentionArgs a, AttnShape sh) {
+template <int CT, int QT, int DP, bool ONCE>
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void paged_attention_kernel(PagedAttentionArgs a, AttnShape sh) {
     constexpr bool kF32 = CT == TML_TYPE_F32;
     constexpr int kBytes = kF32 ? 4 : 2;
     constexpr int NQ = QT == CT ? 1 : CT == TML_TYPE_F16 ? 2 : 3;
@@ -311,7 +325,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
                     const int d = c * kChunk + (kChunk / 4) * c4;
-                    kr[h][c] = *(const srv_u32x4 *)(row + (d < D ? d : 0) * kBytes);
+                    kr[h][c] = load_cache<ONCE>(row + (d < D ? d : 0) * kBytes);
                 }
             }
         };
@@ -324,7 +338,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
                     const int d = f * 16 * E + E * l16;
                     const char *at = row + (d < D ? d : 0) * kBytes;
                     if constexpr (E * kBytes == 16) {
-                        vr[e][f] = *(const srv_u32x4 *)at;
+                        vr[e][f] = load_cache<ONCE>(at);
                     } else {
                         const srv_u32x2 half = *(const srv_u32x2 *)at;
                         vr[e][f] = srv_u32x4{half[0], half[1], 0, 0};
@@ -565,14 +579,26 @@ bool may_split(const PagedAttentionArgs &a) {
     return (a.window > 0 ? std::min(positions, a.window) : positions) > kWhole * kTile;
 }
 
+// A cache past the GPU's last-level cache is read with the streaming policy, a
+// smaller one so that the next step may find it there.  Measured, plain / streaming:
+// 64 requests of up to 4096 tokens (533 MB) 118 / 112 us, two of 40k to 65k (377 MB) 76 /
+// 68; eight of 2k (72 MB) 25.1 / 26.6, one of 1500 with 20 heads of 64 (8 MB) 14.1 / 14.7.
+constexpr int64_t kLastLevel = (int64_t)256 << 20;
+
+template <int CT, int QT, int DP>
+void launch_kernel(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
+    const size_t lds = (size_t)kWaves * sh.heads * DP * 4;
+    const dim3 grid((unsigned)workgroups()), block(kThreads);
+    const double bytes = 2.0 * type_bytes(CT) * a.n_blocks * a.block_size * a.kv_heads * a.head_dim;
+    if (bytes > kLastLevel) paged_attention_kernel<CT, QT, DP, true><<<grid, block, lds, s>>>(a, sh);
+    else paged_attention_kernel<CT, QT, DP, false><<<grid, block, lds, s>>>(a, sh);
+}
+
 template <int CT, int QT>
 Status launch_dim(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
-    const int dp = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
-    const size_t lds = (size_t)kWaves * sh.heads * dp * 4;
-    const dim3 grid((unsigned)workgroups()), block(kThreads);
-    if (dp == 64) paged_attention_kernel<CT, QT, 64><<<grid, block, lds, s>>>(a, sh);
-    else if (dp == 128) paged_attention_kernel<CT, QT, 128><<<grid, block, lds, s>>>(a, sh);
-    else paged_attention_kernel<CT, QT, 256><<<grid, block, lds, s>>>(a, sh);
+    if (a.head_dim <= 64) launch_kernel<CT, QT, 64>(a, sh, s);
+    else if (a.head_dim <= 128) launch_kernel<CT, QT, 128>(a, sh, s);
+    else launch_kernel<CT, QT, 256>(a, sh, s);
     TML_HIP_TRY(hipGetLastError());
     if (sh.lists == nullptr) return Status::Ok();
     paged_attention_join_kernel<QT><<<dim3((unsigned)((a.q_heads + kJoinWaves - 1) / kJoinWaves), (unsigned)a.batch), dim3(64 * kJoinWaves), 0, s>>>(a, sh);
