@@ -386,9 +386,10 @@ int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const 
  * on the order in which workgroups run.  A tensor is read and written inside
  * the call's stream order only: on another stream than its maker's, order
  * the streams first.  tml_hip_paged_attention_dev takes the device's
- * workspace, with the rules of tml_hip_gemm_dev (grown on first use, refused
- * while captured, one stream at a time); the others need none and can be
- * captured at once. */
+ * workspace where a table row holds more than 512 positions (and no window of
+ * at most 512 is given), with the rules of tml_hip_gemm_dev: grown on first use,
+ * refused while captured, one stream at a time.  The others need none and can
+ * be captured at once. */
 
 /* Block tables and slot maps.  Request r has ctx_len[r] tokens in the cache
  * and new_len[r] coming (a negative length counts as 0).  With B =
@@ -440,7 +441,8 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
  *            q_type: F32 or the cache's type
  *   caches   as in tml_hip_kv_store_dev; rows start on 16-byte boundaries
  *            (pointers and strides), else TML_ERR_INVALID_ARG
- *   head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads
+ *   head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads;
+ *            batch and q_heads below 2^16, table_width * block_size at most 2^31
  * The call shares the tiles of the whole batch among the GPU's workgroups by
  * the lengths as they are in seq_len, so one long request, many short ones
  * and any mixture take their bytes' time. */

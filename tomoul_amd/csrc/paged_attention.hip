@@ -622,7 +622,7 @@ Status check_paged_attention(const PagedAttentionArgs &a) {
     const int64_t most = (int64_t)1 << 31;
     if (a.n_blocks >= most || a.block_size >= most || a.batch >= (1 << 16) || a.q_heads >= (1 << 16) ||
         a.table_width >= most || a.table_width * a.block_size > most)
-        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: at most 2^16 requests, 2^16 heads and 2^31 positions of a table");
+        return Status::Err(TML_ERR_INVALID_SHAPE, "paged attention: requests and heads must be below 2^16, a table's positions at most 2^31");
     if (a.q == nullptr || a.out == nullptr || a.seq_len == nullptr || (a.n_blocks > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) ||
         (a.table_width > 0 && a.block_table == nullptr))
         return Status::Err(TML_ERR_INVALID_ARG, "null pointer");
