@@ -533,6 +533,34 @@ def test_paged_attention_streams_and_graph():
     assert torch.equal(long, p.gl) and torch.equal(eager, first)
 
 
+def test_paged_attention_growth_refused_during_capture():
+    # a fresh library context has no workspace: a call that may split must not allocate inside a capture
+    import torch
+    p = Attn(F32, F16, 8, 2, 64, 16, [900, 33], seed=19)
+    short = Attn(F32, F16, 8, 2, 64, 16, [300, 33], seed=20)
+    torch.cuda.synchronize()
+    _abi.shutdown()
+    _abi.init()
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError) as e:
+        with torch.cuda.graph(g, stream=side):
+            _abi.paged_attention_dev(*p.args(), stream=side.cuda_stream)
+    assert "eagerly" in str(e.value)
+    del g
+    torch.cuda.synchronize()
+    # rows of at most 512 positions need none
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        _abi.paged_attention_dev(*short.args(), stream=side.cuda_stream)
+    for _ in range(3):
+        short.out.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        close(short.out[:, :512].reshape(2, 8, 64), short.ref, short.tol)
+    p.check()
+
+
 def test_paged_attention_refusals():
     p = Attn(F32, F16, 4, 2, 64, 16, [40])
     ok = list(p.args())

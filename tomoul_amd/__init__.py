@@ -4,7 +4,8 @@
   tomoul_amd.quantization  Q8_0 / Q8_K / Q4_0 containers, quantizers and
                            weight-only matmuls
   tomoul_amd.dispatch      matmulWithWeight[Bias] (the weight-type dispatch)
-  tomoul_amd._abi          ctypes binding of include/tomoul_hip.h
+  tomoul_amd._abi          ctypes binding of include/tomoul_hip.h, the serving
+                           operators' device-pointer calls among it
   tomoul_amd.build         builds libtomoul_hip.so with hipcc
 
 All compute runs in libtomoul_hip.so; importing an op module does not load

@@ -8,7 +8,8 @@
 //
 // One pass: a row's h stays in registers between its sum of squares and the
 // output, so x and the residual are read once and sum and y written once.
-// Bound by memory past a few hundred rows, by latency below.  A lane holds
+// Bound by memory past a few hundred rows, by latency below: 8192 x 5120 bf16 to 8
+// bits 52.6 us on MI355X (294 MB, 5.6 TB/s), one row of 1280 f32 2.9 us.  A lane holds
 // runs of eight columns (16-byte accesses of 16-bit types), NV of them; a row
 // belongs to one wave (no barrier, four rows a workgroup) or to a workgroup.
 // A row's last run is moved back to end with the row: the columns it shares

@@ -5,6 +5,8 @@
 //   M >  8            -> gemm_mfma.hip (LDS-tiled fp32 MFMA, compute-bound)
 // The host-pointer entry points wrap the device-pointer one: upload operands
 // (or reuse a registered weight), launch, download C, synchronise.
+// The serving operators (serving.hpp) are device-pointer entry points that check
+// their arguments in their launchers.
 // tml_hip_gemm_ex_dev_noalloc is the device-pointer entry point for callers
 // that cannot allocate: its split-K scratch is a static device array.
 #include <unistd.h>
