@@ -142,18 +142,27 @@ __device__ __forceinline__ MvRaw<KIND> mv_load_x(const void *x, int64_t i) {
     }
     return r;
 }
-// `live` of them from element i, the others zero.
+// `live` of them from element i, the others zero.  (The last one again in their
+// place: eight loads without a branch are one wait.)
 template <int KIND>
 __device__ __forceinline__ MvRaw<KIND> mv_load_few(const void *x, int64_t i, int live) {
+    uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (live > 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t at = i + min(e, live - 1);
+            v[e] = mv_int(KIND) ? ((const uint8_t *)x)[at] : KIND == MV_F32 ? ((const uint32_t *)x)[at] : ((const uint16_t *)x)[at];
+        }
+    }
     MvRaw<KIND> r;
 #pragma unroll
     for (int j = 0; j < (KIND == MV_F32 ? 2 : 1); ++j) r.d[j] = srv_u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        if (e >= live) continue;
-        if constexpr (mv_int(KIND)) r.d[0][e / 4] |= (uint32_t)((const uint8_t *)x)[i + e] << (8 * (e % 4));
-        else if constexpr (KIND == MV_F32) r.d[e / 4][e % 4] = ((const uint32_t *)x)[i + e];
-        else r.d[0][e / 2] |= (uint32_t)((const uint16_t *)x)[i + e] << (16 * (e % 2));
+        const uint32_t u = e < live ? v[e] : 0u;
+        if constexpr (mv_int(KIND)) r.d[0][e / 4] |= u << (8 * (e % 4));
+        else if constexpr (KIND == MV_F32) r.d[e / 4][e % 4] = u;
+        else r.d[0][e / 2] |= u << (16 * (e % 2));
     }
     return r;
 }
@@ -208,7 +217,7 @@ __device__ __forceinline__ void mv_put(const MvRaw<KIND> &raw, char *to, int row
 
 // ANY: weight rows on any address, and x in as many fills of LDS as it takes.
 template <int KIND, int SETS, bool ANY>
-__global__ __launch_bounds__(SETS == 4 ? 512 : 1024) void matvec_q4g_kernel(Matvec4Args a, MvShape sh) {
+__global__ __launch_bounds__(SETS > 2 ? 512 : 1024) void matvec_q4g_kernel(Matvec4Args a, MvShape sh) {
     constexpr int kTerms = mv_terms(KIND), kRows = SETS * 4 / kTerms, kItems = mv_items(KIND);
     TML_DYNAMIC_LDS(srv_u32x4, dyn);
     char *const lds = (char *)dyn;
@@ -454,7 +463,7 @@ Status launch_sets(const Matvec4Args &a, MvShape sh, bool wide, hipStream_t s) {
     // 16 / 8 waves: 8-bit x, 8 rows, 14336 x 4096 12.0 / 13.1 us; bf16, 4 rows, 51866 x
     // 1280 10.6 / 11.5; f32, 1 row, 1280 x 5120 7.2 / 6.7; splits one power of two more
     // or less there 16.5, 16.8 (of 12.0), 8.1 (of 6.7).
-    const int nw = tiles * gy >= 2 * cus && SETS < 4 ? 16 : 8;
+    const int nw = tiles * gy >= 2 * cus && SETS < 3 ? 16 : 8;
     int ks = 1;
     while (ks < nw && tiles * gy * ks * 2 <= (int64_t)cus * nw && ks * 2 <= sh.runs) ks *= 2;
     const int tiles_wg = nw / ks;
@@ -488,6 +497,7 @@ Status launch_kind(const Matvec4Args &a, const MvShape &sh, bool wide, hipStream
     const int64_t rows = a.M * mv_terms(KIND);
     if (rows <= 4) return launch_sets<KIND, 1>(a, sh, wide, s);
     if (rows <= 8) return launch_sets<KIND, 2>(a, sh, wide, s);
+    if (rows <= 12) return launch_sets<KIND, 3>(a, sh, wide, s);  // (5 rows of f32 x, 3091 x 4950: 18.2 us as four sets, 10.4)
     return launch_sets<KIND, 4>(a, sh, wide, s);
 }
 
