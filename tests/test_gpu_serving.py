@@ -717,6 +717,30 @@ def test_matvec_q4g_infinities_nan():
         close(got[:1], y, tol)
 
 
+@pytest.mark.parametrize("k,group", [(200, 32), (130, 64), (129, 128), (640, 96)])
+def test_matvec_q4g_scales_that_are_no_numbers(k, group):
+    # an infinite or NaN scale touches its own column and group alone, chunks past K not at all
+    import torch
+    q, s = weights(36, 40, k, group)
+    q[q == 0] = 3  # (an infinite scale times nothing is a NaN of its own)
+    s[2, -1], s[5, 0], s[9, -1] = float("inf"), float("nan"), -float("inf")
+    for xt in (F32, F16, I8):
+        x, xs = make_x(xt, 37, 2, k, 32 if xt == I8 else 0)
+        x = x.abs() + 1 if xt != I8 else x.clamp(min=1)  # one sign: sums of infinities stay infinite or are NaN by q alone
+        got = run_matvec(xt, x, xs, q, s, group, 32 if xt == I8 else 0)
+        for n in (2, 5, 9):
+            lo = 0 if n == 5 else (s.shape[1] - 1) * group
+            part = q[n, lo:lo + group]
+            if n == 5 or bool((part > 0).any() and (part < 0).any()):
+                # (of both signs: the group's sum comes first, and its sign decides)
+                assert torch.isnan(got[:, n]).all() if n == 5 else not torch.isfinite(got[:, n]).any()
+            else:
+                assert torch.isinf(got[:, n]).all()
+        rest = [n for n in range(40) if n not in (2, 5, 9)]
+        y, tol = matvec_ref(xt, x, xs, q, torch.where(torch.isfinite(s), s, 1.0), group, 32)
+        close(got[:, rest], y[:, rest], tol[:, rest])
+
+
 def test_matvec_q4g_bits_do_not_vary():
     import torch
     x, _ = make_x(F32, 32, 3, 4096)

@@ -318,10 +318,10 @@ __global__ __launch_bounds__(SETS > 2 ? 512 : 1024) void matvec_q4g_kernel(Matve
             const int first_group = group_of((run0 + c) * 4);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                // (chunks past K's take zeros for x)
-                const int g = group_of(min((run0 + min(c + u, c1 - 1)) * 4 + c4, sh.chunks - 1));
+                const int chunk = (run0 + min(c + u, c1 - 1)) * 4 + c4, g = group_of(min(chunk, sh.chunks - 1));
                 if constexpr (ANY) cs[u] = s_row[g];
                 else cs[u] = s_lds[n16 * kScaleRow + g - first_group];
+                if (chunk >= sh.chunks) cs[u] = 0.0f;  // (past K there is nothing, whatever the last group's scale is)
             }
             if constexpr (!ANY) {
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
