@@ -49,7 +49,6 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef int64_t offx2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = kWaves * 64;
 constexpr int kTile = 32;  // tokens a wave takes at a time
