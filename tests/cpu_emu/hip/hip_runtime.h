@@ -114,8 +114,13 @@ inline hipError_t hipGetDevice(int *d) {
     return hipSuccess;
 }
 inline hipError_t hipSetDevice(int) { return hipSuccess; }
+// Compute units: 256, or EMU_CUS.
+inline int tml_emu_cus() {
+    const char *v = std::getenv("EMU_CUS");
+    return v != nullptr ? std::atoi(v) : 256;
+}
 inline hipError_t hipDeviceGetAttribute(int *v, hipDeviceAttribute_t, int) {
-    *v = 256;
+    *v = tml_emu_cus();
     return hipSuccess;
 }
 inline hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) {

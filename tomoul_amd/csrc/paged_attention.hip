@@ -466,7 +466,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void paged_attention_k
         // has it in its second slot, those it goes on in in their first.
         const bool whole = t1 - t0 == sp.tiles;
         const int row2 = (int)D / 2;
-        float *const part = sh.partials + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * sh.part_floats;
+        const int64_t part_at = (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * sh.part_floats;
         for (int i = threadIdx.x; i < gn * row2; i += kThreads) {
             const int g = (int)((uint32_t)i / (uint32_t)row2), d = 2 * (i - g * row2);
             float sum_m = wave_m[0][g], sum_l = 0.0f;
@@ -481,6 +481,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void paged_attention_k
             if (whole) {
                 store_result<QT>(a, b, head0 + g, d, sum, sum_l);
             } else {
+                float *const part = sh.partials + part_at;
                 *(srv_f32x2 *)(part + g * (int)D + d) = sum;
                 if (d == 0) *(srv_f32x2 *)(part + sh.heads * (int)D + 2 * g) = srv_f32x2{sum_m, sum_l};
             }
