@@ -436,7 +436,9 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
  * position the output is zeros; whatever lies in other positions, NaN among
  * it, is not looked at.  seq_len counts the new token, stored before the call;
  * a negative one counts as 0, and one past table_width * block_size as that.
- * Scores that are NaN or +inf, and infinite values, give NaN.
+ * A score of -inf, of an infinite key say, weighs nothing, and where there are no
+ * others the output is zeros too; a score that is NaN or +inf makes its head NaN,
+ * and an infinite value its element.
  *   q, out   [batch, q_heads, head_dim], rows q_stride / out_stride apart, of
  *            q_type: F32 or the cache's type
  *   caches   as in tml_hip_kv_store_dev; rows start on 16-byte boundaries

@@ -339,9 +339,11 @@ def attention_ref(a):
         q = values(a["q"][r], qt)
         with np.errstate(invalid="ignore", over="ignore"):
             s = np.einsum("hd,thd->ht", q, key) * a["scale"]
-            p = np.exp(s - s.max(1, keepdims=True))
-            p /= p.sum(1, keepdims=True)
-            err = ((2.0 ** -21 + 4 * np.sqrt(dim) * U) * np.einsum("hd,thd->ht", np.abs(q), np.where(np.isfinite(key), np.abs(key), 0.0)) * a["scale"]).max(1)
+            top = s.max(1, keepdims=True)
+            p = np.exp(s - np.where(top == -np.inf, 0.0, top))
+            total = p.sum(1, keepdims=True)
+            p /= np.where(total == 0, 1.0, total)
+            err = ((2.0 ** -21 + 4 * np.sqrt(dim) * U) * np.einsum("hd,thd->ht", np.abs(q), np.where(np.isfinite(key), np.abs(key), 0.0)) * abs(a["scale"])).max(1)
             ref[r] = np.einsum("ht,thd->hd", p, val)
             tol[r] = (2 * err[:, None] + term + 8 * np.sqrt(length) * U) * np.einsum("ht,thd->hd", p, np.abs(val))
     return ref, np.nan_to_num(tol) + HALF_ULP[qt] * 1.001 * np.nan_to_num(np.abs(ref)) + (2.0 ** -25 if qt == F16 else 1e-30)
@@ -397,6 +399,36 @@ def test_paged_attention_window_and_missing_blocks(lanes, types):
     attention_check(lanes, attention_problem(*types, 2, 1, 64, 16, [29, 1500], window=700), reverse=True)
     got = attention_check(lanes, attention_problem(*types, 4, 2, 40, 8, [100, 300, 16, 9], holes=(0, 1, 5, 6, 7, 8, 20), widen=3))
     assert (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("types", PAIRS, ids=pair)
+@pytest.mark.parametrize("dim,length", [(64, 50), (80, 50), (40, 33), (128, 600), (136, 40)])
+def test_paged_attention_infinite_keys_and_queries(lanes, types, dim, length):
+    # a score of -inf weighs nothing, one of +inf or NaN makes the head NaN, whatever
+    # the head size and the types; nothing but scores of -inf: zeros
+    inf = np.inf
+    for scale in (0.125, -0.125):
+        a = attention_problem(*types, 6, 2, dim, 16, [length, length, 1, length], seed=21)
+        a["scale"], low = scale, -np.sign(scale)
+        qt, ct = types
+        q = np.abs(values(a["q"], qt)) + 0.1  # all of one sign, in d 0 and the last one of both
+        q[:, 1, 0] *= -1
+        q[1, 2, dim - 1] *= -1
+        q[1, 3, 5] = 0
+        q[1, 4, 5] = 1e-30 if qt == F32 else 1e-3  # (little next to the others, but something)
+        q[3, 0, 7], q[3, 1, 7], q[3, 4, 7] = inf, -inf, np.nan
+        a["q"] = stored(q, qt)
+        puts = [(0, 7, 0, 0, low * inf), (0, 20, 1, dim - 1, low * inf), (1, 3, 0, dim - 1, low * inf), (1, 32, 1, 5, low * inf), (1, 4, 1, 0, low * inf),
+                (2, 0, 0, 3, low * inf), (2, 0, 1, 3, -low * inf), (3, 9, 1, 8, low * inf)]
+        sb, st, sh = a["strides"]
+        for r, tok, h, d, v in puts:
+            a["rows"][r][0][tok, h, d] = stored([v], ct)[0]
+            a["caches"][0][a["table"][r, tok // 16] * sb + tok % 16 * st + h * sh + d] = stored([v], ct)[0]
+        ref, tol = attention_ref(a)
+        assert np.isnan(ref[0, 1]).all() and np.isfinite(ref[0, 0]).all() and np.isfinite(ref[0, 3:]).all()
+        assert np.isnan(ref[1, 2]).all() and np.isnan(ref[1, 3]).all() and np.isfinite(ref[1, [0, 1, 4, 5]]).all()
+        assert (ref[2, [0, 2]] == 0).all() and np.isnan(ref[2, 3:]).all()
+        close(attention_run(lanes, a), ref, tol, (scale,))
 
 
 @pytest.mark.parametrize("cus", [1, 4, 16, 256])

@@ -1,0 +1,79 @@
+"""Corners of the serving operators on the GPU: infinite keys and queries, groups of
+more heads than a workgroup of the attention takes, the sizes that need the most LDS,
+lengths that advance in place, more rows than one launch has room for.
+
+Tolerances are those of test_gpu_serving.py, whose problems these build on.
+"""
+import math
+
+import pytest
+
+from test_gpu_serving import BF16, F16, F32, HALF_ULP, TYPES, U, Attn, close, dt, pair
+from tomoul_amd import _abi
+
+pytestmark = pytest.mark.gpu
+
+
+# -------------------------------------------------------- paged attention
+def attention_ref(p):
+    """The result and its tolerance for the cache, q and scale as they are on the GPU now."""
+    import torch
+    inf = math.inf
+    ref, tol = (torch.zeros(p.batch, p.heads, p.dim, dtype=torch.float64) for _ in range(2))
+    term = 2.0 ** -16 if p.ct == BF16 and p.qt == BF16 else 2.0 ** -20
+    for r, length in enumerate(p.lens):
+        pages = p.table[r, :-(-length // p.block)].long().cuda()
+        key, val = (c[pages].reshape(-1, p.kv, p.dim)[:length].double().cpu().repeat_interleave(p.heads // p.kv, 1) for c in (p.k, p.v))
+        q = p.gq[r].view(p.heads, p.dim).double().cpu()
+        s = (q * key).sum(2).T * p.scale
+        top = s.amax(1, keepdim=True)
+        e = torch.exp(s - torch.where(top == -inf, 0.0, top))
+        total = e.sum(1, keepdim=True)
+        w = e / torch.where(total == 0, 1.0, total)
+        ref[r] = (w.T[:, :, None] * val).sum(0)
+        finite = torch.nan_to_num(q, 0.0, 0.0, 0.0).abs() * torch.nan_to_num(key, 0.0, 0.0, 0.0).abs()
+        err = ((2.0 ** -21 + 4 * math.sqrt(p.dim) * U) * finite.sum(2).T * abs(p.scale)).amax(1)
+        tol[r] = (2 * err[:, None] + term + 8 * math.sqrt(max(length, 1)) * U) * (w.T[:, :, None] * val.abs()).sum(0)
+    tol = torch.nan_to_num(tol) + HALF_ULP[p.qt] * 1.001 * torch.nan_to_num(ref).abs() + (2.0 ** -25 if p.qt == F16 else 1e-30)
+    return ref, tol
+
+
+@pytest.mark.parametrize("types", TYPES, ids=pair)
+@pytest.mark.parametrize("dim,length", [(64, 50), (80, 50), (40, 33), (128, 900), (136, 40), (256, 30)])
+def test_paged_attention_infinite_keys_and_queries(types, dim, length):
+    # a score of -inf weighs nothing, one of +inf or NaN makes the head NaN, whatever
+    # the head size and the types; nothing but scores of -inf: zeros
+    import torch
+    inf = math.inf
+    for scale in (0.125, -0.125):
+        p = Attn(*types, 6, 2, dim, 16, [length, length, 1, length], seed=21)
+        p.scale, low = scale, -math.copysign(1.0, scale)
+        q = p.q.double().abs() + 0.1  # all of one sign, in d 0 and the last one of both
+        q[:, 1, 0] *= -1
+        q[1, 2, dim - 1] *= -1
+        q[1, 3, 5] = 0
+        q[1, 4, 5] = 1e-30 if types[0] == F32 else 1e-3  # (little next to the others, but something)
+        q[3, 0, 7], q[3, 1, 7], q[3, 4, 7] = inf, -inf, math.nan
+        p.gq = q.to(dt(types[0])).reshape(p.batch, -1).cuda()
+        for r, tok, h, d, v in ((0, 7, 0, 0, low * inf), (0, 20, 1, dim - 1, low * inf), (1, 3, 0, dim - 1, low * inf), (1, 25, 1, 5, low * inf),
+                                (1, 4, 1, 0, low * inf), (2, 0, 0, 3, low * inf), (2, 0, 1, 3, -low * inf), (3, 9, 1, 8, low * inf)):
+            p.k[int(p.table[r, tok // 16]), tok % 16, h, d] = v
+        ref, tol = attention_ref(p)
+        assert torch.isnan(ref[0, 1]).all() and torch.isfinite(ref[0, 0]).all() and torch.isfinite(ref[0, 3:]).all()
+        assert torch.isnan(ref[1, 2]).all() and torch.isnan(ref[1, 3]).all() and torch.isfinite(ref[1, [0, 1, 4, 5]]).all()
+        assert (ref[2, [0, 2]] == 0).all() and torch.isnan(ref[2, 3:]).all()
+        close(p.run(), ref, tol, (dim, scale))
+
+
+def test_paged_attention_infinite_key_against_the_least_query():
+    # q's elements that f16 and bf16 cannot hold next to the others still give an infinite key its sign
+    import torch
+    for ct in (F16, BF16):
+        for least in (1e-12, 1e-30, 1e-39, -1e-39):
+            p = Attn(F32, ct, 2, 1, 64, 16, [40], seed=23)
+            p.gq = p.gq.abs() + 0.5
+            p.gq[:, 3] = p.gq[:, 64 + 3] = least
+            p.k[int(p.table[0, 1]), 2, 0, 3] = -math.copysign(math.inf, least)
+            ref, tol = attention_ref(p)
+            assert torch.isfinite(ref).all()
+            close(p.run(), ref, tol, (ct, least))

@@ -22,7 +22,8 @@
 //            product's rows
 // Precision: scores and sums are fp32.  q goes in as terms of the cache's type
 // (itself where it has that type; two f16 terms scaled by a power of two, or three
-// bf16 terms, where it is f32), and so do the weights: two terms (2^-22 of f16,
+// bf16 terms, where it is f32; an infinite key meets the first of them alone), and so
+// do the weights: two terms (2^-22 of f16,
 // 2^-16 of bf16), three bf16 terms where the output is f32.  An f32 cache runs on
 // the fp32 matrix cores.
 //
@@ -36,8 +37,8 @@
 //
 // Measured on MI355X (launches in a graph): bf16, 64 requests of up to 4096 tokens, 32
 // heads on 8 of 128 112 us (4.8 TB/s); f16, two of 40k to 65k tokens 68 us (5.5 TB/s); f32 q,
-// f16 cache, one of 448 tokens, 20 heads of 64 8.2 us, of 1500 14.1 us; one of 20 tokens
-// 5.4 us.  Long ones are bound by memory, short ones by the chain of dependent loads:
+// f16 cache, one of 448 tokens, 20 heads of 64 8.4 us, of 1500 14.2 us; one of 20 tokens
+// 5.6 us.  Long ones are bound by memory, short ones by the chain of dependent loads:
 // lengths, table, rows.
 #include "serving.hpp"
 
@@ -144,6 +145,36 @@ __device__ __forceinline__ void to_terms(float (&v)[8], srv_u32x4 (&t)[N]) {
                 v[e + 1] -= CT == TML_TYPE_F16 ? tml_half_bits(d >> 16) : __uint_as_float(d & 0xFFFF0000u);
             }
         }
+}
+
+// q's terms.  The sum over first terms has to be infinite or NaN where the score is,
+// so the first is infinite or NaN where the element is, and of its sign otherwise:
+//   f16   (|v| < 2^15) the element moved away from zero by f16's smallest number,
+//         rounded; a v of 2^-136 still has a sign then
+//   bf16  the element cut off, which cannot overflow
+template <int CT, int N>
+__device__ __forceinline__ void to_query_terms(float (&v)[8], srv_u32x4 (&t)[N]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        if constexpr (CT == TML_TYPE_F16) {
+            const float x = v[e] + __builtin_amdgcn_fmed3f(v[e] * 0x1p112f, -0x1p-24f, 0x1p-24f);
+            const float y = v[e + 1] + __builtin_amdgcn_fmed3f(v[e + 1] * 0x1p112f, -0x1p-24f, 0x1p-24f);
+            const uint32_t d = srv_pack_f16(x, y);
+            t[0][e / 2] = d;
+            v[e] -= tml_half_bits(d & 0xFFFFu);
+            v[e + 1] -= tml_half_bits(d >> 16);
+        } else {
+            // (canonical: any NaN has the bit that the cut leaves)
+            const uint32_t x = __float_as_uint(__builtin_canonicalizef(v[e])), y = __float_as_uint(__builtin_canonicalizef(v[e + 1]));
+            t[0][e / 2] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            v[e] -= __uint_as_float(x & 0xFFFF0000u);
+            v[e + 1] -= __uint_as_float(y & 0xFFFF0000u);
+        }
+    }
+    srv_u32x4 rest[N - 1];
+    to_terms<CT, N - 1>(v, rest);
+#pragma unroll
+    for (int n = 1; n < N; ++n) t[n] = rest[n - 1];
 }
 
 // 16 bytes of the cache.  ONCE: with the streaming policy, which leaves the
@@ -289,7 +320,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void paged_attention_k
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
                 srv_u32x4 t[NQ];
-                to_terms<CT, NQ>(v[c], t);
+                to_query_terms<CT, NQ>(v[c], t);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) q[n][c] = t[n];
             }
@@ -359,25 +390,49 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void paged_attention_k
         __builtin_amdgcn_sched_barrier(0);
         load_v();
         while (t < t1) {
-            // scores
-            float s[8];
+            // (past the head size there are keys again, and they may be infinite: q's zeros must not meet them)
+            if (D < DP) {
+#pragma unroll
+                for (int c = DP == 64 ? 0 : kChunks / 2; c < kChunks; ++c)
+                    if (c * kChunk + (kChunk / 4) * c4 >= D) kr[0][c] = kr[1][c] = srv_u32x4{0, 0, 0, 0};
+            }
+            // scores: sums over q's first terms, and over the others
+            floatx4 lead[2], rest[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                floatx4 acc = {0, 0, 0, 0};
+                lead[h] = rest[h] = floatx4{0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
                     if constexpr (kF32) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[h][c][e]), __uint_as_float(q[0][c][e]), acc, 0, 0, 0);
+                            lead[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[h][c][e]), __uint_as_float(q[0][c][e]), lead[h], 0, 0, 0);
                     } else {
+                        lead[h] = mma16<CT>(kr[h][c], q[0][c], lead[h]);
 #pragma unroll
-                        for (int n = 0; n < NQ; ++n) acc = mma16<CT>(kr[h][c], q[n][c], acc);
+                        for (int n = 1; n < NQ; ++n) rest[h] = mma16<CT>(kr[h][c], q[n][c], rest[h]);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * h + i] = (seen >> (16 * h + 4 * c4 + i) & 1) ? acc[i] * to_log2 : -INFINITY;
             }
+            if constexpr (NQ > 1) {
+                // an infinite first sum is the score: the others only add infinities of any sign to it
+                float peak = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) peak = fmaxf(peak, fabsf(lead[i / 4][i % 4]));
+                if (__builtin_amdgcn_ballot_w64(peak == INFINITY) != 0) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (fabsf(lead[i / 4][i % 4]) == INFINITY) rest[i / 4][i % 4] = 0.0f;
+                }
+            }
+            float s[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float score = NQ > 1 ? lead[h][i] + rest[h][i] : lead[h][i];
+                    s[4 * h + i] = (seen >> (16 * h + 4 * c4 + i) & 1) ? score * to_log2 : -INFINITY;
+                }
             t += kWaves;
             const uint32_t seen_now = seen;
             seen = rows_of(t, block);
