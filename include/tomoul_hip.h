@@ -461,8 +461,8 @@ int tml_hip_paged_attention_dev(int q_type, int cache_type, int64_t batch, int64
  * made of the unrounded h.  residual, sum and weight (ones) may be NULL; sum
  * may be x or residual.  out is of out_type: F32, F16, BF16, or I8 with
  *   scales[row, g] = max|out| / 127 over columns [g * group, (g + 1) * group)
- * (group 0: one scale a row; the last group may be short) and q = the nearest
- * integer to out / scale.  A group whose largest magnitude is below 2^-118 has
+ * (group 0: one scale a row; the last group may be short) and q = out / scale,
+ * divided in fp32 and rounded to the nearest integer, halves to the even one.  A group whose largest magnitude is below 2^-118 has
  * scale 1 and zeros; one that holds an infinity or a NaN has that as its scale
  * and zeros.  scales: [rows, ceil(cols / group)], at most 16384 a row; it is
  * written for I8 only. */

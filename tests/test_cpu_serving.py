@@ -144,6 +144,39 @@ def test_rmsnorm_8_bits(lanes, t, rows, cols, group):
     norm_program(lanes, t, rows, cols, I8, group=group, cus=1, reverse=True)
 
 
+def tie_weights(cols, most, seed):
+    """Values at and next to the halves between the steps of a group whose largest is `most`."""
+    rng = np.random.default_rng(seed)
+    step = np.float32(most) / np.float32(127)
+    w = ((rng.integers(-127, 127, cols) + 0.5) * np.float64(step)).astype(np.float32)
+    w = (w.view(np.int32) + rng.integers(-2, 3, cols)).astype(np.int32).view(np.float32)
+    w[rng.integers(cols)] = most
+    return w
+
+
+@pytest.mark.parametrize("cols,group", [(1280, 0), (1280, 128), (1237, 0), (1237, 96), (7, 0), (33000, 0)])
+def test_rmsnorm_8_bits_at_the_halves(lanes, cols, group):
+    # x of ones and no epsilon: out is the weight itself, so the quotient is known to its last bit
+    rng = np.random.default_rng(17)
+    width = group or cols
+    w = np.concatenate([tie_weights(min(width, cols - g), np.float32(m), g) for g, m in
+                        zip(range(0, cols, width), np.exp(rng.uniform(-8, 8, -(-cols // width))))])
+    groups = -(-cols // width)
+    p = lanes.Program()
+    bx, bw = p.buf(np.ones(cols, np.float32)), p.buf(w)
+    bo, bs = p.buf(np.zeros(cols, np.int8)), p.buf(np.zeros(groups, np.float32))
+    p.call("rmsnorm", F32, 1, cols, ("b", bx), cols, None, 0, ("b", bw), 0.0, None, 0, I8, ("b", bo), cols, ("b", bs), group, None)
+    got = p.run()
+    assert p.codes == [0], p.messages
+    for g in range(groups):
+        part = w[g * width:(g + 1) * width]
+        scale = np.abs(part).max() / np.float32(127)
+        assert got[bs][g] == scale
+        want = np.rint(part / scale)
+        wrong = got[bo][g * width:(g + 1) * width] != want
+        assert not wrong.any(), (g, int(wrong.sum()), part[wrong][:3] / scale, want[wrong][:3])
+
+
 @pytest.mark.parametrize("what", ["x", "residual", "weight", "sum", "out", "scales"])
 def test_rmsnorm_short_operand_is_reported(lanes, what):
     with pytest.raises(lanes.Fault):

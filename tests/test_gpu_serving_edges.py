@@ -6,9 +6,10 @@ Tolerances are those of test_gpu_serving.py, whose problems these build on.
 """
 import math
 
+import numpy as np
 import pytest
 
-from test_gpu_serving import BF16, F16, F32, HALF_ULP, TYPES, U, Attn, close, dt, pair
+from test_gpu_serving import BF16, F16, F32, HALF_ULP, I8, TYPES, U, Attn, close, dt, pair
 from tomoul_amd import _abi
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +78,27 @@ def test_paged_attention_infinite_key_against_the_least_query():
             ref, tol = attention_ref(p)
             assert torch.isfinite(ref).all()
             close(p.run(), ref, tol, (ct, least))
+
+
+# ---------------------------------------------------------------- rmsnorm
+@pytest.mark.parametrize("rows,cols,group", [(1, 1280, 0), (1100, 1280, 128), (1, 1280, 128), (1100, 1237, 0), (3, 1237, 96), (2, 7, 0), (2, 33000, 0), (2, 9000, 64)])
+def test_rmsnorm_8_bits_at_the_halves(rows, cols, group):
+    # x of ones and no epsilon: out is the weight itself, so the quotient is known to its last bit
+    rng = np.random.default_rng(17)
+    width = group or cols
+    w = np.empty(cols, np.float32)
+    for g in range(0, cols, width):
+        most = np.float32(np.exp(rng.uniform(-8, 8)))
+        part = ((rng.integers(-127, 127, min(width, cols - g)) + 0.5) * np.float64(most / np.float32(127))).astype(np.float32)
+        part = (part.view(np.int32) + rng.integers(-2, 3, len(part))).astype(np.int32).view(np.float32)
+        part[rng.integers(len(part))] = most
+        w[g:g + width] = part
+    import torch
+    x, gw = torch.ones(rows, cols, device="cuda"), torch.from_numpy(w).cuda()
+    q, scales = torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), torch.zeros(rows, -(-cols // width), device="cuda")
+    _abi.rmsnorm_dev(F32, rows, cols, x.data_ptr(), cols, gw.data_ptr(), 0.0, I8, q.data_ptr(), cols, scales_ptr=scales.data_ptr(), group=group)
+    torch.cuda.synchronize()
+    scale = np.array([np.abs(w[g:g + width]).max() / np.float32(127) for g in range(0, cols, width)], np.float32)
+    want = np.rint(w / np.repeat(scale, width)[:cols])
+    assert (scales.cpu().numpy() == scale).all()
+    assert (q.cpu().numpy() == want).all()

@@ -35,20 +35,40 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v, int width) {
     return v;
 }
 
-// scale of a group whose largest magnitude has the bits `most`, and what y is
-// multiplied with.  A group of (nearly) zeros has scale 1 and q = 0; one that
-// holds an infinity or a NaN has that as its scale and q = 0, so that what is
-// made of it is no number either.
-__device__ __forceinline__ float group_scale(uint32_t most, float *inv) {
+// scale of a group whose largest magnitude has the bits `most`.  A group of (nearly)
+// zeros has scale 1; one that holds an infinity or a NaN has that as its scale.
+constexpr uint32_t kLeast = (127u - 118u) << 23;  // 2^-118: m / 127 and 127 / m are normal numbers from it on
+__device__ __forceinline__ float group_scale(uint32_t most) {
     const float m = __uint_as_float(most);
-    *inv = 0.0f;
-    if (most >= 0x7F800000u) return m;
-    if (m < 0x1p-118f) return 1.0f;  // 127 / m and m / 127 stay normal numbers above it
-    *inv = 127.0f / m;
-    return m / 127.0f;
+    return most >= 0x7F800000u ? m : most < kLeast ? 1.0f : m / 127.0f;
 }
-__device__ __forceinline__ int quantum(float y, float inv) {
-    return (int)__builtin_rintf(__builtin_amdgcn_fmed3f(inv == 0.0f ? 0.0f : y * inv, -127.0f, 127.0f));
+// rint(y / scale), and 0 where the scale is no number.
+__device__ __forceinline__ int quantum(float y, float scale) {
+    const float q = y / scale;
+    return scale < INFINITY ? (int)__builtin_rintf(q) : 0;
+}
+// The same for eight columns of one group, whose largest magnitude is `most`.  A
+// product with 127 / most, off by less than 2^-22 of 127, goes the other way at some of
+// the halves between two integers: a wave that has a product so near to one divides
+// (8192 x 5120 bf16, groups of 128: divisions alone 65 us, this 61, products alone 60).
+__device__ __forceinline__ srv_u32x2 quanta(const float (&y)[8], uint32_t most, float scale) {
+    const float inv = most < 0x7F800000u && most >= kLeast ? 127.0f / __uint_as_float(most) : 0.0f;
+    int n[8];
+    float off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float q = inv == 0.0f ? 0.0f : y[e] * inv, r = __builtin_rintf(q);
+        off = fmaxf(off, fabsf(q - r));
+        n[e] = (int)r;
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(off > 0.5f - 0x1p-14f) != 0, 0)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n[e] = quantum(y[e], scale);
+    }
+    srv_u32x2 d = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e / 4] |= (uint32_t)(n[e] & 0xFF) << (8 * (e % 4));
+    return d;
 }
 
 // TPR threads a row, NV runs of eight columns a thread.
@@ -146,16 +166,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(RmsNormA
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) m = max(m, part_m[w]);
         }
-        float inv;
-        const float s = group_scale(m, &inv);
+        const float s = group_scale(m);
         if (t == 0) a.scales[row] = s;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (skip[v] >= 8) continue;
-            uint32_t d[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e / 4] |= (uint32_t)(quantum(h[v][e], inv) & 0xFF) << (8 * (e % 4));
-            *(srv_u32x2_any *)((int8_t *)a.out + row * a.out_stride + off[v]) = srv_u32x2{d[0], d[1]};
+            const srv_u32x2 d = quanta(h[v], m, s);
+            if (skip[v] < 8) *(srv_u32x2_any *)((int8_t *)a.out + row * a.out_stride + off[v]) = d;
         }
         return;
     }
@@ -177,28 +193,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(RmsNormA
         if constexpr (kWaves > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         for (int i = t; i < ngroups; i += TPR) {
-            float inv;
-            a.scales[row * ngroups + i] = group_scale(lds_most[i], &inv);
+            const float s = group_scale(lds_most[i]);
+            a.scales[row * ngroups + i] = s;
+            lds_most[i] = __float_as_uint(s);
         }
+        if constexpr (kWaves > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        uint32_t d[2] = {0, 0};
+        srv_u32x2 d = {0, 0};
         if (by_lanes) {
-            float inv;
-            const float s = group_scale(wave_max(most[v], group / 8), &inv);
+            const uint32_t m = wave_max(most[v], group / 8);
+            const float s = group_scale(m);
             if (off[v] % group == 0 && skip[v] == 0) a.scales[row * ngroups + off[v] / group] = s;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e / 4] |= (uint32_t)(quantum(h[v][e], inv) & 0xFF) << (8 * (e % 4));
+            d = quanta(h[v], m, s);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float inv;
-                (void)group_scale(lds_most[(off[v] + e) / group], &inv);
-                d[e / 4] |= (uint32_t)(quantum(h[v][e], inv) & 0xFF) << (8 * (e % 4));
-            }
+            for (int e = 0; e < 8; ++e)
+                d[e / 4] |= (uint32_t)(quantum(h[v][e], __uint_as_float(lds_most[(off[v] + e) / group])) & 0xFF) << (8 * (e % 4));
         }
-        if (skip[v] < 8) *(srv_u32x2_any *)((int8_t *)a.out + row * a.out_stride + off[v]) = srv_u32x2{d[0], d[1]};
+        if (skip[v] < 8) *(srv_u32x2_any *)((int8_t *)a.out + row * a.out_stride + off[v]) = d;
     }
 }
 
@@ -235,17 +250,17 @@ __global__ __launch_bounds__(1024) void rmsnorm_any_kernel(RmsNormArgs a) {
         for (int64_t c = t; c < a.cols; c += 1024) atomicMax(&lds_most[c / a.group], mag(norm_at(c, sum_at(c))));
         __syncthreads();
         for (int i = t; i < ngroups; i += 1024) {
-            float inv;
-            a.scales[row * ngroups + i] = group_scale(lds_most[i], &inv);
+            const float s = group_scale(lds_most[i]);
+            a.scales[row * ngroups + i] = s;
+            lds_most[i] = __float_as_uint(s);
         }
+        __syncthreads();
     }
     for (int64_t c = t; c < a.cols; c += 1024) {
         const float h = sum_at(c), y = norm_at(c, h);
         if (a.sum != nullptr) srv_store1(a.type, a.sum, row * a.sum_stride + c, h);
         if (i8) {
-            float inv;
-            (void)group_scale(lds_most[c / a.group], &inv);
-            ((int8_t *)a.out)[row * a.out_stride + c] = (int8_t)quantum(y, inv);
+            ((int8_t *)a.out)[row * a.out_stride + c] = (int8_t)quantum(y, __uint_as_float(lds_most[c / a.group]));
         } else {
             srv_store1(a.out_type, a.out, row * a.out_stride + c, y);
         }
