@@ -15,7 +15,7 @@
 //
 // LDS arrays keep what the workgroup before left in them, and a launch's dynamic
 // LDS starts as that pattern.  With EMU_REVERSE=1 the blocks of a grid run from the
-// last to the first and so do the waves of a block.  Launches that HIP refuses
+// last to the first and so do the waves of a block.  Launches that HIP refuses or cuts
 // (2^32 work items or more in a dimension, over 1024 threads a block, over 160 KiB of
 // dynamic LDS) do not run and are reported by hipGetLastError.
 //

@@ -102,3 +102,30 @@ def test_rmsnorm_8_bits_at_the_halves(rows, cols, group):
     want = np.rint(w / np.repeat(scale, width)[:cols])
     assert (scales.cpu().numpy() == scale).all()
     assert (q.cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("t,rows,cols", [(F32, (1 << 22) + 3, 3), (F16, (1 << 26) + 5, 8)], ids=str)
+def test_rmsnorm_more_rows_than_a_launch_has_room_for(t, rows, cols):
+    import torch
+    free, _ = torch.cuda.mem_get_info()
+    if free < 12 << 30:
+        pytest.skip("needs 12 GiB")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x = torch.empty(rows, cols, dtype=dt(t), device="cuda").normal_(generator=g)
+    q, s = torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    total, out = torch.zeros_like(x), torch.zeros_like(x)
+    _abi.rmsnorm_dev(t, rows, cols, x.data_ptr(), cols, None, 1e-6, t, out.data_ptr(), cols, residual_ptr=x.data_ptr(), residual_stride=cols,
+                     sum_ptr=total.data_ptr(), sum_stride=cols)
+    _abi.rmsnorm_dev(t, rows, cols, x.data_ptr(), cols, None, 1e-6, I8, q.data_ptr(), cols, scales_ptr=s.data_ptr())
+    torch.cuda.synchronize()
+    step = 1 << 22
+    for r in range(0, rows, step):
+        part = x[r:r + step].float()
+        assert torch.equal(total[r:r + step], (2 * part).to(dt(t)))  # (exact: twice a number)
+        y = part * torch.rsqrt((part * part).mean(1, keepdim=True) + 1e-6)
+        most = y.abs().amax(1)
+        assert ((s[r:r + step] - most / 127).abs() <= 60 * U * most / 127).all()
+        assert ((q[r:r + step] * s[r:r + step, None] - y).abs() <= (0.5 + 127 * 140 * U) * most[:, None] / 127).all()
+        y2 = 2 * part * torch.rsqrt((4 * part * part).mean(1, keepdim=True) + 1e-6)
+        assert ((out[r:r + step].float() - y2).abs() <= (HALF_ULP[t] * 1.001 + 60 * U) * y2.abs() + 2.0 ** -25 * (t == F16)).all()

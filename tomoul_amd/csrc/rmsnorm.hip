@@ -269,40 +269,58 @@ __global__ __launch_bounds__(1024) void rmsnorm_any_kernel(RmsNormArgs a) {
 
 constexpr int64_t kMaxGroups = 16384;  // maxima in LDS, 64 KiB
 
+// Rows of one launch, of workgroups of `threads` that take rows_wg rows each: a
+// grid has fewer than 2^32 threads (a larger one is cut without an error).
+int64_t launch_rows(int threads, int rows_wg) { return (int64_t)(0xFFFFFFFFu / (unsigned)threads) * rows_wg; }
+
+RmsNormArgs rows_from(const RmsNormArgs &a, int64_t r0, int64_t rows) {
+    RmsNormArgs p = a;
+    const int64_t size = type_bytes(a.type), groups = a.out_type == TML_TYPE_I8 ? (a.cols + a.group - 1) / a.group : 0;
+    p.rows = rows;
+    p.x = (const char *)a.x + r0 * a.x_stride * size;
+    if (a.residual != nullptr) p.residual = (const char *)a.residual + r0 * a.residual_stride * size;
+    if (a.sum != nullptr) p.sum = (char *)a.sum + r0 * a.sum_stride * size;
+    p.out = (char *)a.out + r0 * a.out_stride * type_bytes(a.out_type);
+    if (groups > 0) p.scales = a.scales + r0 * groups;
+    return p;
+}
+
 template <int T>
-Status launch_type(const RmsNormArgs &a, hipStream_t s) {
-    const int64_t groups = a.out_type == TML_TYPE_I8 ? (a.cols + a.group - 1) / a.group : 0;
-    const int64_t runs = (a.cols + 7) / 8;
-    if (a.cols < 8 || runs > 4 * 1024) {
-        rmsnorm_any_kernel<<<dim3((unsigned)a.rows), dim3(1024), (size_t)groups * 4, s>>>(a);
-        TML_HIP_TRY(hipGetLastError());
-        return Status::Ok();
-    }
+Status launch_type(const RmsNormArgs &all, hipStream_t s) {
+    const int64_t groups = all.out_type == TML_TYPE_I8 ? (all.cols + all.group - 1) / all.group : 0;
+    const int64_t runs = (all.cols + 7) / 8;
+    const bool any = all.cols < 8 || runs > 4 * 1024;
     // A wave a row where that leaves enough waves to fill the GPU; otherwise a
     // workgroup a row, whose four waves share its latency.
-    const bool wave = runs <= 64 || (runs <= 256 && a.rows >= 4 * (int64_t)device_cus());
-    const int tpr = wave ? 64 : runs <= 1024 ? 256 : 1024;
-    const int nv = (int)((runs + tpr - 1) / tpr);
-    const unsigned rows_wg = wave ? 4 : 1;
-    const dim3 grid((unsigned)((a.rows + rows_wg - 1) / rows_wg)), block(tpr < 256 ? 256 : tpr);
-    const size_t lds = groups > 1 ? (size_t)groups * rows_wg * 4 : 0;
+    const bool wave = runs <= 64 || (runs <= 256 && all.rows >= 4 * (int64_t)device_cus());
+    const int tpr = any ? 1024 : wave ? 64 : runs <= 1024 ? 256 : 1024;
+    const int nv = (int)((runs + tpr - 1) / tpr), rows_wg = tpr == 64 ? 4 : 1;
+    const dim3 block(tpr < 256 ? 256 : tpr);
+    const size_t lds = any || groups > 1 ? (size_t)groups * rows_wg * 4 : 0;
+    const int64_t most = launch_rows((int)block.x, rows_wg);
+    for (int64_t r0 = 0; r0 < all.rows; r0 += most) {
+        const RmsNormArgs a = rows_from(all, r0, std::min(most, all.rows - r0));
+        const dim3 grid((unsigned)((a.rows + rows_wg - 1) / rows_wg));
 #define TML_NORM(TPR, NV) rmsnorm_kernel<T, TPR, NV><<<grid, block, lds, s>>>(a)
-    if (tpr == 64) {
-        if (nv == 1) TML_NORM(64, 1);
-        else if (nv == 2) TML_NORM(64, 2);
-        else if (nv == 3) TML_NORM(64, 3);
-        else TML_NORM(64, 4);
-    } else if (tpr == 256) {
-        if (nv == 1) TML_NORM(256, 1);
-        else if (nv == 2) TML_NORM(256, 2);
-        else if (nv == 3) TML_NORM(256, 3);
-        else TML_NORM(256, 4);
-    } else {
-        if (nv <= 2) TML_NORM(1024, 2);
-        else TML_NORM(1024, 4);
-    }
+        if (any) {
+            rmsnorm_any_kernel<<<grid, block, lds, s>>>(a);
+        } else if (tpr == 64) {
+            if (nv == 1) TML_NORM(64, 1);
+            else if (nv == 2) TML_NORM(64, 2);
+            else if (nv == 3) TML_NORM(64, 3);
+            else TML_NORM(64, 4);
+        } else if (tpr == 256) {
+            if (nv == 1) TML_NORM(256, 1);
+            else if (nv == 2) TML_NORM(256, 2);
+            else if (nv == 3) TML_NORM(256, 3);
+            else TML_NORM(256, 4);
+        } else {
+            if (nv <= 2) TML_NORM(1024, 2);
+            else TML_NORM(1024, 4);
+        }
 #undef TML_NORM
-    TML_HIP_TRY(hipGetLastError());
+        TML_HIP_TRY(hipGetLastError());
+    }
     return Status::Ok();
 }
 
