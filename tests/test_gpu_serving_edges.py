@@ -129,3 +129,26 @@ def test_rmsnorm_more_rows_than_a_launch_has_room_for(t, rows, cols):
         assert ((q[r:r + step] * s[r:r + step, None] - y).abs() <= (0.5 + 127 * 140 * U) * most[:, None] / 127).all()
         y2 = 2 * part * torch.rsqrt((4 * part * part).mean(1, keepdim=True) + 1e-6)
         assert ((out[r:r + step].float() - y2).abs() <= (HALF_ULP[t] * 1.001 + 60 * U) * y2.abs() + 2.0 ** -25 * (t == F16)).all()
+
+
+# ------------------------------------------------------------- matvec_q4g
+def test_matvec_q4g_more_columns_than_a_launch_has_room_for():
+    # two k a column, so that 2^30 columns stay small: rows of a byte
+    import torch
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    n = (1 << 30) + 7
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    w = torch.randint(0, 256, (n,), generator=g, device="cuda", dtype=torch.uint8)
+    scales, y = torch.ones(n, device="cuda"), torch.full((n,), 99.0, dtype=torch.float16, device="cuda")
+    scales[-9:] = 2.0
+    x = torch.tensor([[3.0, 0.5]], dtype=torch.float16, device="cuda")
+    _abi.matvec_q4g_dev(F16, 1, n, 2, x.data_ptr(), 2, w.data_ptr(), 1, scales.data_ptr(), 32, F16, y.data_ptr(), n)
+    torch.cuda.synchronize()
+    step = 1 << 27
+    for at in range(0, n, step):
+        u = w[at:at + step].to(torch.int16)
+        want = ((u & 15 ^ 8) - 8).half() * 3 + ((u >> 4 ^ 8) - 8).half() * 0.5  # (exact)
+        assert torch.equal(y[at:at + step], want * scales[at:at + step].half())

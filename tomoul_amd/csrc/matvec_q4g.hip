@@ -502,6 +502,9 @@ Status launch_kind(const Matvec4Args &a, const MvShape &sh, bool wide, hipStream
 }
 
 constexpr int64_t kMostK = (int64_t)1 << 20;
+// Columns of a launch: four threads each, and a grid has fewer than 2^32 (a larger one
+// is cut without an error).
+constexpr int64_t kMostN = (int64_t)1 << 29;
 
 }  // namespace
 
@@ -527,6 +530,19 @@ Status launch_matvec_q4g(const Matvec4Args &in, hipStream_t s) {
     if ((a.M > 1 && (a.x_stride < a.K || a.y_stride < a.N)) || (a.N > 1 && a.w_stride < row))
         return Status::Err(TML_ERR_INVALID_SHAPE, "matvec_q4g: a row stride is shorter than the row");
     a.group = std::min(a.group, std::max<int64_t>(a.K, 1));
+    if (a.N > kMostN) {  // the last columns in a launch of their own
+        a.N = kMostN;
+        Status first = launch_matvec_q4g(a, s);
+        if (!first.ok()) return first;
+        a.N = in.N - kMostN;
+        if (a.K > 0) {
+            a.w += kMostN * a.w_stride;
+            a.w_scales += kMostN * ((a.K + a.group - 1) / a.group);
+        }
+        if (a.bias != nullptr) a.bias += kMostN;
+        a.y = (char *)a.y + kMostN * type_bytes(a.y_type);
+        return launch_matvec_q4g(a, s);
+    }
     MvShape sh{};
     sh.chunks = (int)((a.K + 31) / 32);
     sh.runs = (sh.chunks + 3) / 4;
