@@ -385,7 +385,8 @@ int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const 
  * of fewer bits is rounded once, to nearest even.  The results do not depend
  * on the order in which workgroups run.  A tensor is read and written inside
  * the call's stream order only: on another stream than its maker's, order
- * the streams first.  tml_hip_paged_attention_dev takes the device's
+ * the streams first.  Outputs overlap neither inputs nor each other, except where
+ * it says so below.  tml_hip_paged_attention_dev takes the device's
  * workspace where a table row holds more than 512 positions (and no window of
  * at most 512 is given), with the rules of tml_hip_gemm_dev: grown on first use,
  * refused while captured, one stream at a time.  The others need none and can
@@ -408,7 +409,9 @@ int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const 
  *   totals         [3] new tokens, blocks taken from the free list (more
  *                  than n_free: the rest got -1), requests whose length does
  *                  not fit table_width (their row takes what fits)
- * The outputs after `slots` may be NULL.  If totals[0] exceeds max_tokens the
+ * The outputs after `slots` may be NULL.  seq_len may be ctx_len or new_len itself,
+ * lengths that advance in place; any other output that overlaps an input is
+ * refused with TML_ERR_INVALID_ARG.  If totals[0] exceeds max_tokens the
  * plan is incomplete: tokens past it were neither mapped nor given blocks. */
 int tml_hip_kv_plan_dev(int64_t requests, int64_t block_size, const int *ctx_len, const int *new_len,
                         const int *free_blocks, int64_t n_free, int *block_table, int64_t table_width,

@@ -226,7 +226,7 @@ def plan_inputs(n, block, ctx_most, new_most, short, narrow=0):
     return ctx, new, pool[:max(0, len(pool) - 40 - short)], table
 
 
-def plan_program(lanes, block, ctx, new, free, table, max_tokens, gap=2, reverse=False, short=None):
+def plan_program(lanes, block, ctx, new, free, table, max_tokens, gap=2, reverse=False, short=None, in_place=None):
     n, width = len(ctx), len(table[0])
     p = lanes.Program(reverse=reverse)
     i32, i64 = np.int32, np.int64
@@ -239,6 +239,8 @@ def plan_program(lanes, block, ctx, new, free, table, max_tokens, gap=2, reverse
     bs = make("slots", np.full(max_tokens, -9, i64))
     outs = [make(name, np.full(k, -9, i32)) for name, k in (("request", max_tokens), ("position", max_tokens), ("seq_len", n), ("query_start", n + 1))]
     bl = make("totals", np.full(3, -9, i64))
+    if in_place is not None:
+        outs[2] = {"ctx": bc, "new": bn}[in_place]
     p.call("kv_plan", n, block, ("b", bc), ("b", bn), ("b", bf) if free else None, len(free), ("b", bt), width, width + gap, max_tokens, ("b", bs),
            *[("b", o) for o in outs], ("b", bl), None)
     got = p.run()
@@ -255,6 +257,42 @@ def test_kv_plan(lanes, n, block, ctx_most, new_most, pad, short):
         got = plan_program(lanes, block, ctx, new, free, table, tokens, reverse=reverse)
         for what, g, r in zip(("table", "slots", "request", "position", "seq_len", "query_start", "totals"), got, ref):
             assert g == [list(v) for v in r] if what == "table" else g == list(r), what
+
+
+@pytest.mark.parametrize("n,block,ctx_most,new_most,pad,short", PLANS)
+@pytest.mark.parametrize("which", ["ctx", "new"])
+def test_kv_plan_lengths_in_place(lanes, which, n, block, ctx_most, new_most, pad, short):
+    # seq_len over one of the lengths it is made of: no workgroup may read it after it was written
+    ctx, new, free, table = plan_inputs(n, block, ctx_most, new_most, short, 2 if n == 33 else 0)
+    tokens = sum(max(v, 0) for v in new) + pad
+    ref = plan_ref(block, ctx, new, free, table, tokens)
+    for reverse in (False, True):
+        got = plan_program(lanes, block, ctx, new, free, table, tokens, reverse=reverse, in_place=which)
+        for what, g, r in zip(("table", "slots", "request", "position", "seq_len", "query_start", "totals"), got, ref):
+            assert g == [list(v) for v in r] if what == "table" else g == list(r), what
+
+
+def test_kv_plan_refuses_outputs_over_inputs(lanes):
+    # one buffer of ints: ctx at 0, new at 8, free blocks at 16, a table of 2 x 3 with rows 8 apart at 32, the outputs behind
+    n, tokens = 2, 4
+    good = dict(ctx=0, new=8, free=16, table=32, slots=64, request=80, position=88, seq_len=96, query_start=104, totals=112)
+
+    def code(**over):
+        at = {**good, **over}
+        p = lanes.Program()
+        b = p.buf(np.concatenate([[5, 3], np.zeros(6), [3, 1], np.zeros(6), np.arange(16), np.zeros(128)]).astype(np.int32))
+        a = {k: ("b", b, 4 * v) for k, v in at.items()}
+        p.call("kv_plan", n, 4, a["ctx"], a["new"], a["free"], 5, a["table"], 3, 8, tokens, a["slots"], a["request"], a["position"], a["seq_len"],
+               a["query_start"], a["totals"], None)
+        p.run()
+        return p.codes[0]
+
+    assert code() == 0 and code(seq_len=0) == 0 and code(seq_len=8) == 0
+    assert code(free=35) == 0 and code(ctx=36, new=44) == 0  # (between the table's rows)
+    for over in (dict(seq_len=1), dict(seq_len=7), dict(seq_len=17), dict(query_start=0), dict(query_start=6), dict(query_start=20), dict(slots=2),
+                 dict(slots=10), dict(request=1), dict(position=9), dict(position=13 + 5), dict(totals=4), dict(totals=6), dict(free=34), dict(free=38),
+                 dict(ctx=41), dict(new=31), dict(new=34), dict(table=1), dict(table=18)):
+        assert code(**over) == -5, over
 
 
 def test_kv_plan_more_tokens_than_room(lanes):

@@ -9,7 +9,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_serving import BF16, F16, F32, HALF_ULP, I8, TYPES, U, Attn, close, dt, pair
+from test_gpu_serving import BF16, F16, F32, HALF_ULP, I8, TYPES, U, Attn, close, dt, gen, pair
 from tomoul_amd import _abi
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +152,60 @@ def test_matvec_q4g_more_columns_than_a_launch_has_room_for():
         u = w[at:at + step].to(torch.int16)
         want = ((u & 15 ^ 8) - 8).half() * 3 + ((u >> 4 ^ 8) - 8).half() * 0.5  # (exact)
         assert torch.equal(y[at:at + step], want * scales[at:at + step].half())
+
+
+# ---------------------------------------------------------------- kv_plan
+@pytest.mark.parametrize("n,new_most", [(64, 1), (500, 40), (3, 3000), (2000, 3)])
+def test_kv_plan_lengths_in_place(n, new_most):
+    # the lengths advance over themselves, step after step, eagerly and as a graph
+    import torch
+    block, steps = 16, 3
+    width = -(-steps * max(new_most, 1) // block) + 1
+    i32 = dict(dtype=torch.int32, device="cuda")
+    new = torch.randint(0, new_most + 1, (n,), generator=gen(5)).to(torch.int32)
+    tokens = int(new.sum()) + 7
+    free = torch.randperm(n * width, generator=gen(6)).to(torch.int32).cuda()
+    ctx, gnew = torch.zeros(n, **i32), new.cuda()
+    table = torch.full((n, width), -1, **i32)
+    slots, pos = torch.zeros(tokens, dtype=torch.int64, device="cuda"), torch.zeros(tokens, **i32)
+    req, totals = torch.zeros(tokens, **i32), torch.zeros(3, dtype=torch.int64, device="cuda")
+
+    def plan(stream):
+        _abi.kv_plan_dev(n, block, ctx.data_ptr(), gnew.data_ptr(), free.data_ptr(), free.numel(), table.data_ptr(), width, width, tokens,
+                         slots.data_ptr(), token_request_ptr=req.data_ptr(), positions_ptr=pos.data_ptr(), seq_len_ptr=ctx.data_ptr(),
+                         totals_ptr=totals.data_ptr(), stream=stream)
+
+    owner = torch.repeat_interleave(torch.arange(n), new.long())
+    first = torch.cat([torch.arange(int(v)) for v in new]) if tokens > 7 else torch.zeros(0, dtype=torch.long)
+    side = torch.cuda.Stream()
+    graph = None
+    handed = 0
+    for step in range(2 * steps):
+        if step == steps:  # the same again from the start, replayed
+            ctx.zero_()
+            table.fill_(-1)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                plan(side.cuda_stream)
+            handed = 0
+        pool = torch.roll(torch.arange(n * width, dtype=torch.int32), -handed).cuda()
+        free.copy_(pool)
+        torch.cuda.synchronize()
+        if graph is None:
+            plan(None)
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        done = (step % steps) * new.long()
+        assert torch.equal(ctx.cpu().long(), done + new.long())
+        assert torch.equal(req[:-7].cpu().long(), owner) and (req[-7:] == -1).all()
+        where = done[owner] + first
+        assert torch.equal(pos[:-7].cpu().long(), where)
+        page = table.cpu().long()[owner, where // block]
+        assert (page >= 0).all() and torch.equal(slots[:-7].cpu(), page * block + where % block)
+        need = int((-(-(done + new.long()) // block) - -(-done // block)).sum())
+        assert totals.tolist() == [tokens - 7, need, 0]
+        handed += need
+        used = table[table >= 0]
+        assert used.unique().numel() == used.numel() == handed

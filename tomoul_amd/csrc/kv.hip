@@ -23,7 +23,9 @@ namespace {
 // the slice since empty ones are left out; a token finds its request there by
 // bisection.  A block is written into the table by the token that is first in
 // it, so every entry has one writer, and entries that a token reads (of blocks
-// it found) nobody writes.  Launches in a graph: 64 requests of a token 3.9 us, 512 of
+// it found) nobody writes.  The lengths are read by all workgroups and seq_len is
+// written by the first, so lengths that advance in place take a launch after the
+// plan's where that has several workgroups.  Launches in a graph: 64 requests of a token 3.9 us, 512 of
 // up to 256 tokens 5.7 us (slices of 512 and 1024 tokens: 6.2, 7.8; workgroups of 1024
 // threads, one step of sums for two: 19.3), one of 200000 tokens 3.6.
 constexpr int kPlanThreads = 256;
@@ -144,6 +146,12 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(KvPlanArgs a) {
     }
 }
 
+// Lengths that advance in place while the plan runs in several workgroups: after it.
+__global__ __launch_bounds__(256) void kv_lengths_kernel(int64_t requests, const int *ctx_len, const int *new_len, int *seq_len) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r < requests) seq_len[r] = (int)min((int64_t)max(ctx_len[r], 0) + max(new_len[r], 0), (int64_t)0x7FFFFFFF);
+}
+
 // -------------------------------------------------------------- kv_store
 // A thread moves eight elements of one token's keys and the same eight of its
 // values, `runs` threads a token.  Bound by memory: each row is read and
@@ -201,6 +209,21 @@ void launch_store(const KvStoreArgs &a, const StoreShape &sh, dim3 grid, hipStre
     else kv_store_kernel<TS, TML_TYPE_BF16><<<grid, dim3(256), 0, s>>>(a, sh);
 }
 
+// Bytes [p, p + bytes); rows > 1: the same every `stride` bytes.
+struct Bytes {
+    const void *p;
+    int64_t bytes;
+    int64_t rows = 1, stride = 0;
+};
+bool meet(const Bytes &a, const Bytes &b) {  // b: one row
+    if (a.p == nullptr || b.p == nullptr || a.bytes <= 0 || b.bytes <= 0 || a.rows <= 0) return false;
+    const intptr_t off = (intptr_t)b.p - (intptr_t)a.p;  // b's start in a
+    if (off + b.bytes <= 0 || off >= (a.rows - 1) * a.stride + a.bytes) return false;
+    if (off < 0 || a.rows == 1) return true;
+    const intptr_t in_row = off % a.stride;
+    return in_row < a.bytes || in_row + b.bytes > a.stride;
+}
+
 }  // namespace
 
 Status launch_kv_plan(const KvPlanArgs &a, hipStream_t s) {
@@ -214,9 +237,31 @@ Status launch_kv_plan(const KvPlanArgs &a, hipStream_t s) {
     if ((a.requests > 0 && (a.ctx_len == nullptr || a.new_len == nullptr)) || (a.n_free > 0 && a.free_blocks == nullptr) ||
         (a.requests > 0 && a.table_width > 0 && a.block_table == nullptr) || (a.max_tokens > 0 && a.slots == nullptr))
         return Status::Err(TML_ERR_INVALID_ARG, "null pointer");
+    // Workgroups read all lengths while the first one writes: only seq_len may lie over
+    // what it is made of, element on element.
+    const int64_t width = std::min(a.table_width, (int64_t)1 << 32);  // (no length reaches further)
+    const int64_t free_read = std::min(a.n_free, a.requests * width);
+    const Bytes ins[3] = {{a.ctx_len, a.requests * 4}, {a.new_len, a.requests * 4}, {a.free_blocks, free_read * 4}};
+    const Bytes outs[6] = {{a.block_table, width * 4, a.requests, a.requests > 1 ? a.table_stride * 4 : 0}, {a.slots, a.max_tokens * 8}, {a.token_request, a.max_tokens * 4},
+                           {a.positions, a.max_tokens * 4}, {a.query_start, (a.requests + 1) * 4}, {a.totals, 24}};
+    const Bytes lengths{a.seq_len, a.requests * 4};
+    bool bad = false;
+    for (const Bytes &in : ins) {
+        for (const Bytes &out : outs) bad |= meet(out, in);
+        bad |= (in.p != a.seq_len || in.p == a.free_blocks) && meet(lengths, in);
+    }
+    if (bad)
+        return Status::Err(TML_ERR_INVALID_ARG, "kv plan: an output overlaps an input (seq_len alone may be ctx_len or new_len itself)");
     const int64_t slices = std::max<int64_t>(1, (a.max_tokens + kSlice - 1) / kSlice);
-    kv_plan_kernel<<<dim3((unsigned)slices), dim3(kPlanThreads), 0, s>>>(a);
+    const bool after = slices > 1 && a.requests > 0 && a.seq_len != nullptr && (a.seq_len == a.ctx_len || a.seq_len == a.new_len);
+    KvPlanArgs plan = a;
+    if (after) plan.seq_len = nullptr;
+    kv_plan_kernel<<<dim3((unsigned)slices), dim3(kPlanThreads), 0, s>>>(plan);
     TML_HIP_TRY(hipGetLastError());
+    if (after) {
+        kv_lengths_kernel<<<dim3((unsigned)((a.requests + 255) / 256)), dim3(256), 0, s>>>(a.requests, a.ctx_len, a.new_len, a.seq_len);
+        TML_HIP_TRY(hipGetLastError());
+    }
     return Status::Ok();
 }
 
