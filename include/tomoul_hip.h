@@ -30,7 +30,7 @@
  * callers: one model-forward thread, src/core/ops.zig:485).  All calls on
  * one device share that device's split-K workspace, so "_dev" calls issued
  * concurrently on different streams of the same device race; issue them on
- * one stream.
+ * one stream.  (The serving operators say for themselves what they share.)
  */
 #ifndef TOMOUL_HIP_H
 #define TOMOUL_HIP_H
@@ -386,11 +386,12 @@ int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const 
  * on the order in which workgroups run.  A tensor is read and written inside
  * the call's stream order only: on another stream than its maker's, order
  * the streams first.  Outputs overlap neither inputs nor each other, except where
- * it says so below.  tml_hip_paged_attention_dev takes the device's
- * workspace where a table row holds more than 512 positions (and no window of
- * at most 512 is given), with the rules of tml_hip_gemm_dev: grown on first use,
- * refused while captured, one stream at a time.  The others need none and can
- * be captured at once. */
+ * it says so below.  tml_hip_paged_attention_dev takes a workspace where a table row
+ * holds more than 512 positions (and no window of at most 512 is given).  It is
+ * not the products', so an attention may run beside them on another stream; its own
+ * calls share it, with the rules of tml_hip_gemm_dev: grown on first use, refused while
+ * captured, one stream at a time.  The others need none and can be captured at
+ * once. */
 
 /* Block tables and slot maps.  Request r has ctx_len[r] tokens in the cache
  * and new_len[r] coming (a negative length counts as 0).  With B =

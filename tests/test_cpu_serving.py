@@ -509,6 +509,23 @@ def test_paged_attention_splits(lanes, cus):
     attention_check(lanes, attention_problem(BF16, BF16, 2, 2, 8, 16, [(i * 37) % 60 for i in range(70)]), cus=cus, reverse=True)
 
 
+def test_paged_attention_has_a_workspace_of_its_own(lanes):
+    # an attention on one stream must not write where a split GEMM's sums are on another
+    a = attention_problem(F16, F16, 2, 1, 64, 16, [700])
+    p = lanes.Program(cus=4)
+    p.env["TML_GEMM_SPLIT"] = "4"
+    gemm = [p.buf(np.zeros(n, np.float32)) for n in (32 * 2048, 2048 * 64, 32 * 64)]
+    b = [p.buf(v) for v in (a["q"], a["caches"][0], a["caches"][1], a["table"], np.array(a["lens"], np.int32), np.zeros_like(a["q"]))]
+    for _ in range(2):
+        p.call("gemm", 0, 32, 64, 2048, ("b", gemm[0]), ("b", gemm[1]), 1.0, None, 0, None, ("b", gemm[2]), 1.0, 0.0, None)
+        p.call("paged_attention", F16, F16, 1, 2, 1, 64, ("b", b[0]), 128, ("b", b[1]), ("b", b[2]), a["n_blocks"], 16, *a["strides"], ("b", b[3]),
+               a["width"], a["width"], ("b", b[4]), 0, a["scale"], ("b", b[5]), 128, None)
+    p.run()
+    assert p.codes == [0] * 4, p.messages
+    first, second, third, fourth = p.allocations
+    assert second == first + 1 and second == third == fourth, p.allocations
+
+
 @pytest.mark.parametrize("what", ["q", "k", "v", "table", "lens", "out"])
 def test_paged_attention_short_operand_is_reported(lanes, what):
     a = attention_problem(F32, F16, 4, 2, 40, 8, [90, 96])

@@ -198,6 +198,7 @@ struct DeviceCtx {
     std::vector<hipEvent_t> chunk_done;  // ... and the chunks of its downloads
     GrowBuf qtmp, tl_raw, tl_scales, tr;  // quantizer partials, .tl payload staging, transpose temporary
     GrowBuf ws, counters;                // split-K workspace (gemv, gemm)
+    GrowBuf attention;                   // the paged attention's parts
     DevBuf zero;                         // kZeroBlockBytes of zeros
     std::unordered_map<const void *, Registered> weights;
 };
@@ -308,20 +309,21 @@ Status ensure_workspace(DeviceCtx *c, MatmulArgs &m, hipStream_t s, Workspace *w
     return Status::Ok();
 }
 
-// The same for the paged attention's parts, which need no counters.
+// The same for the paged attention's parts, which need no counters.  They have a buffer
+// of their own: an attention and a split GEMM may run on two streams.
 Status attention_workspace(DeviceCtx *c, const PagedAttentionArgs &a, hipStream_t s, Workspace *ws) {
     const size_t bytes = paged_attention_workspace_floats(a) * sizeof(float);
-    if (bytes > c->ws.bytes) {
+    if (bytes > c->attention.bytes) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
         TML_HIP_TRY(hipStreamIsCapturing(s, &cap));
         if (cap != hipStreamCaptureStatusNone)
             return Status::Err(TML_ERR_INVALID_ARG,
                                "the workspace must grow during stream capture: run this call once eagerly (outside "
                                "capture) before capturing it");
-        TML_TRY(c->ws.ensure(bytes));
+        TML_TRY(c->attention.ensure(bytes));
     }
-    ws->partials = (float *)c->ws.p;
-    ws->partial_floats = c->ws.bytes / sizeof(float);
+    ws->partials = (float *)c->attention.p;
+    ws->partial_floats = c->attention.bytes / sizeof(float);
     return Status::Ok();
 }
 
@@ -774,6 +776,7 @@ void tml_hip_shutdown(void) {
         }
         c->a.release(); c->b.release(); c->c.release(); c->bias.release(); c->res.release();
         c->scales.release(); c->qtmp.release(); c->ws.release(); c->counters.release();
+        c->attention.release();
         c->tl_raw.release(); c->tl_scales.release(); c->tr.release();
         c->pin_in.release(); c->pin_out.release();
         for (hipEvent_t e : c->chunk_done) (void)hipEventDestroy(e);
@@ -1135,7 +1138,7 @@ int tml_hip_transpose_requant_dev(int fmt, int64_t rows, int64_t cols, const voi
     return report(run());
 }
 
-// ------------------------------------------------------------ .tl files
+// ---------------------------------------------------- serving operators
 int tml_hip_kv_plan_dev(int64_t requests, int64_t block_size, const int *ctx_len, const int *new_len,
                         const int *free_blocks, int64_t n_free, int *block_table, int64_t table_width,
                         int64_t table_stride, int64_t max_tokens, int64_t *slots, int *token_request, int *positions,
@@ -1212,6 +1215,7 @@ int tml_hip_quantize_groups_dev(int64_t N, int64_t K, int64_t group, const float
     return report(launch_quantize_groups(N, K, group, w, w_stride, q, q_stride, scales, (hipStream_t)stream));
 }
 
+// ------------------------------------------------------------ .tl files
 int tml_tl_open(const char *path, tml_tl_t *out) {
     if (out == nullptr) return report(Status::Err(TML_ERR_INVALID_ARG, "null handle pointer"));
     TlFile *f = nullptr;
