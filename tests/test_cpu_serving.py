@@ -634,7 +634,8 @@ def quantize_program(lanes, n, k, group, short=None):
         assert (np.abs(q[:, g * group:(g + 1) * group] * scale[:, None].astype(np.float64) - part) <= scale[:, None] * (0.5 + 1e-5)).all()
 
 
-@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 33, 32), (5, 200, 64), (2, 700, 128), (9, 96, 96), (4, 50, 2)])
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 33, 32), (5, 200, 64), (2, 700, 128), (9, 96, 96), (4, 50, 2),
+                                       (3, 50, 2 ** 63 - 1), (2, 51, 2 ** 63 - 1)])
 def test_quantize_groups(lanes, n, k, group):
     quantize_program(lanes, n, k, group)
 

@@ -209,3 +209,18 @@ def test_kv_plan_lengths_in_place(n, new_most):
         handed += need
         used = table[table >= 0]
         assert used.unique().numel() == used.numel() == handed
+
+
+# -------------------------------------------------------- quantize_groups
+@pytest.mark.parametrize("k", [50, 51, 4096])
+def test_quantize_groups_any_group_past_k(k):
+    import torch
+    w = torch.randn(3, k, generator=gen(9)).cuda()
+    outs = []
+    for group in (k, 2 ** 63 - 1):
+        q, s = torch.zeros(3, (k + 1) // 2, dtype=torch.uint8, device="cuda"), torch.zeros(3, device="cuda")
+        _abi.quantize_groups_dev(3, k, group, w.data_ptr(), k, q.data_ptr(), (k + 1) // 2, s.data_ptr())
+        torch.cuda.synchronize()
+        outs.append((q.cpu(), s.cpu()))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert torch.equal(outs[0][1], w.abs().amax(1).cpu() / 7)

@@ -573,6 +573,7 @@ Status launch_quantize_groups(int64_t N, int64_t K, int64_t group, const float *
     if (group <= 0) return Status::Err(TML_ERR_INVALID_ARG, "group quantizer: the group must be positive");
     if (group % 2 != 0 && group < K) return Status::Err(TML_ERR_INVALID_SHAPE, "group quantizer: the group must be even");
     if (N == 0 || K == 0) return Status::Ok();
+    group = std::min(group, K);
     if (w == nullptr || q == nullptr || scales == nullptr) return Status::Err(TML_ERR_INVALID_ARG, "null pointer");
     if (N > 1 && (w_stride < K || q_stride < (K + 1) / 2))
         return Status::Err(TML_ERR_INVALID_SHAPE, "group quantizer: a row stride is shorter than the row");
