@@ -491,7 +491,9 @@ int tml_hip_rmsnorm_dev(int type, int64_t rows, int64_t cols, const void *x, int
  * Arithmetic: f32 x is split into two f16 terms a chunk of 32 (2^-23 of each
  * element, 2^-39 of the chunk's largest), bf16 and f16 x and 8-bit x are exact
  * but for that 2^-39 of bf16; products and sums are fp32, integers exact.  A
- * group's scale multiplies the group's finished sum. */
+ * group's scale multiplies the finished sum of each 32 of its columns (of f32 x, of
+ * each of its two terms), so an infinite scale gives an infinity only where these
+ * have one sign, and NaN otherwise. */
 int tml_hip_matvec_q4g_dev(int x_type, int64_t M, int64_t N, int64_t K, const void *x, int64_t x_stride,
                            const float *x_scales, int64_t x_group, const uint8_t *w, int64_t w_stride,
                            const float *w_scales, int64_t group, const float *bias, int y_type, void *y,

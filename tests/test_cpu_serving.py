@@ -600,6 +600,28 @@ def test_matvec_q4g_rows_anywhere(lanes, xt, k, width, offset):
     matvec_program(lanes, xt, 3, 21, k, 32, 32 if xt == I8 else 0, width=width, offset=offset)
 
 
+@pytest.mark.parametrize("xt", [F32, F16, BF16, I8], ids=tname)
+@pytest.mark.parametrize("group", [32, 64, 96, 128, 256])
+def test_matvec_q4g_infinite_scales(lanes, xt, group):
+    # a scale multiplies the sum over each 32 of its group's columns (of f32 x, of each of
+    # its terms), and these are added then
+    k, n = 256, 18
+
+    def edit(q, s):
+        s[3, 0], s[7, -1] = np.inf, -np.inf
+
+    y, q, s, x = matvec_program(lanes, xt, 2, n, k, group, bias=False, edit=edit)
+    with np.errstate(invalid="ignore"):
+        parts = np.einsum("mck,nck->mnc", x.reshape(2, k // 32, 32), q.reshape(n, k // 32, 32).astype(np.float64))
+        want = (parts * s.astype(np.float64)[:, np.arange(k // 32) * 32 // group]).sum(2)
+    assert not np.isfinite(want[:, [3, 7]]).any() and (group == 256 or np.isinf(want[:, [3, 7]]).any() or np.isnan(want).any())
+    ok = np.isfinite(want)
+    assert np.array_equal(np.isfinite(y), ok)
+    if xt != F32:
+        assert np.array_equal(np.isnan(y), np.isnan(want)) and np.array_equal(y[np.isinf(want)], want[np.isinf(want)])
+    assert (np.abs(y - want)[ok] <= 1e-4 * np.abs(want[ok]) + 1e-3).all()
+
+
 @pytest.mark.parametrize("width", [None, 501])
 @pytest.mark.parametrize("what", ["x", "x_scales", "w", "w_scales", "bias", "y"])
 def test_matvec_q4g_short_operand_is_reported(lanes, width, what):
