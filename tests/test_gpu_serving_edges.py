@@ -224,3 +224,28 @@ def test_quantize_groups_any_group_past_k(k):
         outs.append((q.cpu(), s.cpu()))
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
     assert torch.equal(outs[0][1], w.abs().amax(1).cpu() / 7)
+
+
+# ----------------------------------------- paged attention, sizes past the usual
+@pytest.mark.parametrize("types", TYPES, ids=pair)
+@pytest.mark.parametrize("heads,kv,dim,block,lens,layout,widen", [
+    (34, 2, 96, 16, [260, 900, 1], "htd", 0), (48, 1, 64, 16, [1300, 0, 600], "thd", 3),  # groups of more than 16 heads, split
+    (16, 1, 256, 16, [70, 1030], "thd", 0), (40, 1, 256, 32, [5, 700], "htd", 0),  # the most LDS a workgroup takes
+    (8, 8, 64, 16, [40, 3, 448], "thd", 300), (8, 2, 128, 16, [0, 513, 17], "htd", 1000)])  # a table far wider than its requests
+def test_paged_attention_large_groups_and_wide_tables(types, heads, kv, dim, block, lens, layout, widen):
+    Attn(*types, heads, kv, dim, block, lens, layout, widen=widen, seed=31).check()
+
+
+@pytest.mark.parametrize("cols,group", [(49152, 3), (32768, 2), (131072, 8)])
+def test_rmsnorm_8_bits_the_most_groups(cols, group):
+    # 16384 group maxima in LDS, 64 KiB of them
+    import torch
+    x = torch.randn(2, cols, generator=gen(41)).cuda()
+    q, scales = torch.zeros(2, cols, dtype=torch.int8, device="cuda"), torch.zeros(2, 16384, device="cuda")
+    _abi.rmsnorm_dev(F32, 2, cols, x.data_ptr(), cols, None, 1e-6, I8, q.data_ptr(), cols, scales_ptr=scales.data_ptr(), group=group)
+    torch.cuda.synchronize()
+    y = x.double() / torch.sqrt(x.double().square().mean(1, keepdim=True) + 1e-6)
+    most = y.view(2, 16384, group).abs().amax(2)
+    assert ((scales - most / 127).abs() <= 40 * U * most / 127).all()
+    # (the scale's own error, and half a step)
+    assert ((q.view(2, 16384, group) * scales[:, :, None].double() - y.view(2, 16384, group)).abs() <= (0.5 + 127 * 80 * U) * most[:, :, None] / 127).all()
