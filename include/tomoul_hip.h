@@ -426,7 +426,7 @@ int tml_hip_kv_plan_dev(int64_t requests, int64_t block_size, const int *ctx_len
  * with slot = slots[t]; v alike, the caches having the same strides.  The
  * strides say whether tokens or heads come first in a block.  A slot that is
  * negative or not below n_blocks * block_size is skipped.  Two tokens with the
- * same slot: one of them is stored, either. */
+ * same slot: what lies there afterwards is made of both. */
 int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k,
                          const void *v, int64_t k_stride, int64_t v_stride, const int64_t *slots, void *k_cache,
                          void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
@@ -449,6 +449,11 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
  *            (pointers and strides), else TML_ERR_INVALID_ARG
  *   head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads;
  *            batch and q_heads below 2^16, table_width * block_size at most 2^31
+ * Arithmetic: products and sums are fp32, of q and of the weights e^(s - max) as terms
+ * of the cache's type.  f32 q on a 16-bit cache: two f16 terms (2^-22 of each element,
+ * 2^-39 of its head's largest) or three bf16 terms (2^-24).  Weights: two f16 terms
+ * (2^-22 of each, 2^-39 of the largest), two bf16 terms (2^-16), three (2^-24) where
+ * the output is f32.  An f32 cache is all fp32.
  * The call shares the tiles of the whole batch among the GPU's workgroups by
  * the lengths as they are in seq_len, so one long request, many short ones
  * and any mixture take their bytes' time. */
@@ -479,9 +484,13 @@ int tml_hip_rmsnorm_dev(int type, int64_t rows, int64_t cols, const void *x, int
  * w is N rows of K two's-complement nibbles, even k in the low one, row n at
  * w + n * w_stride (bytes; the buffer holds N * w_stride of them, and what
  * follows a row's K nibbles may be anything); w_scales is [N, ceil(K / group)].
- * group: a multiple of 32, or at least K.  Rows that start on 16-byte
- * boundaries with w_stride >= ceil(K / 32) * 16 are read in wide loads; others
- * are read too, slower.
+ * group: a multiple of 32, or at least K.  Fastest are rows that start on 16-byte
+ * boundaries with w_stride >= ceil(K / 32) * 16, and a K at which the rows of x of one
+ * pass fit LDS together: to 16000 for 1 or 2 rows of f32 or 4 of 16 bits, to 3968 for
+ * the 8 or 16 of a full pass, to 7680 for 16 of 8 bits.  Other rows and other K are
+ * taken too, their scales read one by one: 65536 x 4096, 1 row of f32, 36 us, with
+ * weight rows of 2049 bytes 78; 4096 outputs, 8 rows of f32, K = 4096 and 4224, 11.3
+ * and 13.5.
  *   x   [M, K], rows x_stride apart: F32, F16, BF16, or I8 with x_scales [M]
  *       (x_group 0) or [M, ceil(K / x_group)] (x_group a multiple of 32), as
  *       tml_hip_rmsnorm_dev leaves them

@@ -5,10 +5,10 @@
 //
 // over the positions t of [max(0, len - window), len) whose block is in the
 // cache; none of them: zeros.  Query heads h of a group share a key-value head.
-// Keys and values are read once, 2 * len * dim elements a key-value head, for
-// 4 * group operations an element, so memory bounds it from some 100 KB up; the
-// kernel is laid out to have loads in flight, and the matrix cores do the
-// arithmetic because they cost nothing next to that, at a group of one too.
+// Keys and values are read once for each 16 query heads of a group, 2 * len * dim
+// elements a key-value head, for 4 * group operations an element, so memory bounds it
+// from some 100 KB up; the kernel is laid out to have loads in flight, and the matrix
+// cores do the arithmetic because they cost nothing next to that, at a group of one too.
 //
 // One pass with a running maximum and sum.  A wave takes 32 tokens at a time:
 //   scores   S = K q^T: 16 tokens are the MFMA's rows, up to 16 query heads its
@@ -37,9 +37,12 @@
 //
 // Measured on MI355X (launches in a graph): bf16, 64 requests of up to 4096 tokens, 32
 // heads on 8 of 128 112 us (4.8 TB/s); f16, two of 40k to 65k tokens 68 us (5.5 TB/s); f32 q,
-// f16 cache, one of 448 tokens, 20 heads of 64 8.4 us, of 1500 14.2 us; one of 20 tokens
-// 5.6 us.  Long ones are bound by memory, short ones by the chain of dependent loads:
-// lengths, table, rows.
+// f16 cache, one of 448 tokens, 20 heads of 64 8.4 us (10.0 with a table for 4096: the
+// second kernel is launched by the table's width and finds nothing to do), of 1500
+// 14.2 us; one of 20 tokens 5.6 us; eight of 2k, 32 heads on 8 of 256, bf16 46 us (3.1
+// TB/s), f32 112 us (2.6 TB/s).  Long ones are bound by memory, short ones by the chain
+// of dependent loads: lengths, table, rows.  The f32 kernel for heads past 128 keeps 36
+// vector registers of a lane in scratch, the one for 128 two, the others none.
 #include "serving.hpp"
 
 #include <algorithm>
@@ -637,7 +640,9 @@ bool may_split(const PagedAttentionArgs &a) {
 // A cache past the GPU's last-level cache is read with the streaming policy, a
 // smaller one so that the next step may find it there.  Measured, plain / streaming:
 // 64 requests of up to 4096 tokens (533 MB) 118 / 112 us, two of 40k to 65k (377 MB) 76 /
-// 68; eight of 2k (72 MB) 25.1 / 26.6, one of 1500 with 20 heads of 64 (8 MB) 14.1 / 14.7.
+// 68; eight of 2k (72 MB) 25.2 / 27.1, one of 1500 with 20 heads of 64 (8 MB) 14.3 / 14.6.
+// The rule goes by the whole pool, the lengths being on the GPU: few short requests in
+// a large pool are read with the streaming policy too, at the last two's loss.
 constexpr int64_t kLastLevel = (int64_t)256 << 20;
 
 template <int CT, int QT, int DP>
