@@ -451,7 +451,7 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
  *            batch and q_heads below 2^16, table_width * block_size at most 2^31
  * Arithmetic: products and sums are fp32, of q and of the weights e^(s - max) as terms
  * of the cache's type.  f32 q on a 16-bit cache: two f16 terms (2^-22 of each element,
- * 2^-39 of its head's largest) or three bf16 terms (2^-24).  Weights: two f16 terms
+ * 2^-39 of its head's largest or of 2^-100) or three bf16 terms (2^-24).  Weights: two f16 terms
  * (2^-22 of each, 2^-39 of the largest), two bf16 terms (2^-16), three (2^-24) where
  * the output is f32.  An f32 cache is all fp32.
  * The call shares the tiles of the whole batch among the GPU's workgroups by
@@ -498,7 +498,7 @@ int tml_hip_rmsnorm_dev(int type, int64_t rows, int64_t cols, const void *x, int
  * Made for few rows, up to 16 of which share one pass over the weight (8 of F32
  * x); more rows take more passes.  K is at most 2^20, M at most 131070.
  * Arithmetic: f32 x is split into two f16 terms a chunk of 32 (2^-23 of each
- * element, 2^-39 of the chunk's largest), bf16 and f16 x and 8-bit x are exact
+ * element, 2^-39 of the chunk's largest or of 2^-100), bf16 and f16 x and 8-bit x are exact
  * but for that 2^-39 of bf16; products and sums are fp32, integers exact.  A
  * group's scale multiplies the finished sum of each 32 of its columns (of f32 x, of
  * each of its two terms), so an infinite scale gives an infinity only where these

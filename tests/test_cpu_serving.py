@@ -10,9 +10,10 @@ derivation before the first run:
   attention  scores (2^-21 + 4 sqrt(D) u) sum |q k| * scale, weights 2^-16 (16-bit output
              of a bf16 cache) or 2^-20, sums 8 sqrt(len) u, of sum p |v|
 
-CPU only; needs /opt/rocm/llvm/bin/clang++ (skipped without it).
+CPU only; needs /opt/rocm/llvm/bin/clang++ and an x86-64 (skipped without them).
 """
 import os
+import platform
 import sys
 
 import numpy as np
@@ -20,7 +21,7 @@ import pytest
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CLANG = "/opt/rocm/llvm/bin/clang++"
-pytestmark = pytest.mark.skipif(not os.path.exists(CLANG), reason="no clang++ for the CPU build")
+pytestmark = pytest.mark.skipif(not os.path.exists(CLANG) or platform.machine() != "x86_64", reason="no clang++ for the CPU build, or not x86-64")
 
 U = 2.0 ** -24
 F32, F16, BF16, I8 = 0, 1, 2, 3
