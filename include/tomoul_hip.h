@@ -441,8 +441,8 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
  * it, is not looked at.  seq_len counts the new token, stored before the call;
  * a negative one counts as 0, and one past table_width * block_size as that.
  * A score of -inf, of an infinite key say, weighs nothing, and where there are no
- * others the output is zeros too; a score that is NaN or +inf makes its head NaN,
- * and an infinite value its element.
+ * others the output is zeros too; a score that is NaN or +inf makes its head NaN.
+ * An infinite value makes its element infinite or NaN.
  *   q, out   [batch, q_heads, head_dim], rows q_stride / out_stride apart, of
  *            q_type: F32 or the cache's type
  *   caches   as in tml_hip_kv_store_dev; rows start on 16-byte boundaries
