@@ -374,8 +374,9 @@ int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const 
 /* ---------------------------------------------------- serving operators
  * What a decoder step needs around its products, without the host in
  * between: block tables and slot maps from request lengths, new keys and
- * values to their slots, attention over the paged cache, the norm that
- * feeds a product, and the product with 4-bit weights and group scales.  No
+ * values to their slots, attention of single tokens and of prompts over the paged cache
+ * (of floats, or in 4 bits), the norm that feeds a product, the product with 4-bit weights
+ * and group scales, and the scores of tokens.  No
  * counterpart in the reference (its cache is one contiguous run a request,
  * src/core/cache.zig:1-30, on the host).
  *
@@ -386,9 +387,10 @@ int tml_hip_gemm_prepared_ex(tml_prepared_t w, int64_t M, const float *A, const 
  * on the order in which workgroups run.  A tensor is read and written inside
  * the call's stream order only: on another stream than its maker's, order
  * the streams first.  Outputs overlap neither inputs nor each other, except where
- * it says so below.  tml_hip_paged_attention_dev takes a workspace where a table row
+ * it says so below.  The attentions of one new token (tml_hip_paged_attention_dev, _ex_dev,
+ * _q4_dev) take a workspace where a table row
  * holds more than 512 positions (and no window of at most 512 is given).  It is
- * not the products', so an attention may run beside them on another stream; its own
+ * not the products', so an attention may run beside them on another stream; their own
  * calls share it, with the rules of tml_hip_gemm_dev: grown on first use, refused while
  * captured, one stream at a time.  The others need none and can be captured at
  * once. */
@@ -463,6 +465,111 @@ int tml_hip_paged_attention_dev(int q_type, int cache_type, int64_t batch, int64
                                 int64_t token_stride, int64_t head_stride, const int *block_table,
                                 int64_t table_width, int64_t table_stride, const int *seq_len, int64_t window,
                                 float scale, void *out, int64_t out_stride, void *stream);
+
+/* tml_hip_paged_attention_dev with other scores s_t in the place of scale * q . k_t:
+ *   s_t = cap * tanh(scale * q . k_t / cap) - slopes[h] * (seq_len - 1 - t)
+ * cap: 0 for none, or from 2^-100 to 2^100.  slopes: q_heads floats of a bias that grows
+ * with the distance, or NULL.  With neither it is that call.  An infinite product is
+ * capped to +-cap, where there is one. */
+int tml_hip_paged_attention_ex_dev(int q_type, int cache_type, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                   int64_t head_dim, const void *q, int64_t q_stride, const void *k_cache,
+                                   const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                                   int64_t token_stride, int64_t head_stride, const int *block_table,
+                                   int64_t table_width, int64_t table_stride, const int *seq_len, int64_t window,
+                                   float scale, float cap, const float *slopes, void *out, int64_t out_stride,
+                                   void *stream);
+
+/* Attention of prompts over the paged cache: any number of new tokens a request, whose
+ * keys and values were stored before the call (tml_hip_kv_plan_dev's query_start and
+ * seq_len, tml_hip_kv_store_dev).  Token i of request r is row query_start[r] + i of q and
+ * out and stands at position pos = seq_len[r] - new + i, new = query_start[r + 1] -
+ * query_start[r].  It sees the positions t of its request with
+ *   t < seq_len[r]  and  (t <= pos or t < prefix_len[r])  and  (window == 0 or t > pos - window)
+ * whose block is in the cache; other requests (documents of one batch) never.
+ * prefix_len NULL: causal.  A prefix of the whole length: every token sees every other, as
+ * in an encoder.  The scores are
+ *   s_t = cap * tanh(scale * q . k_t / cap) - slopes[h] * |pos - t|
+ * with cap and slopes as in tml_hip_paged_attention_ex_dev; a token that sees nothing gets
+ * zeros, and what lies in other positions, NaN among it, is not looked at.
+ *   tokens       rows of q and out; those at query_start[requests] and after are left as they
+ *                were.  Starts and lengths that do not fit (negative, past tokens, past the
+ *                table) count as the nearest that do
+ *   other arguments, types, heads and alignment as in tml_hip_paged_attention_dev; tokens
+ *   below 2^24, tokens * q_heads / 128 + requests * kv_heads at most 2^23
+ * Arithmetic: products and sums are fp32, of q and of the weights e^(s - max) as terms of the
+ * cache's type: q as there (an infinite element of f32 q on a 16-bit cache makes its
+ * head's outputs NaN); weights one term where out has 16 bits (2^-8 of each for bf16, 2^-11
+ * for f16), two of f16 (2^-22) or three of bf16 (2^-24) where it is f32.  An f32 cache is
+ * all fp32.  Needs no workspace.
+ * One new token a request is taken too (a mixed batch), but a request's 128 (token, head)
+ * rows go through its cache one after another: tml_hip_paged_attention_ex_dev shares long
+ * caches among the GPU's workgroups. */
+int tml_hip_prompt_attention_dev(int q_type, int cache_type, int64_t tokens, int64_t requests, int64_t q_heads,
+                                 int64_t kv_heads, int64_t head_dim, const void *q, int64_t q_stride,
+                                 const void *k_cache, const void *v_cache, int64_t n_blocks, int64_t block_size,
+                                 int64_t block_stride, int64_t token_stride, int64_t head_stride,
+                                 const int *block_table, int64_t table_width, int64_t table_stride,
+                                 const int *query_start, const int *seq_len, const int *prefix_len, int64_t window,
+                                 float scale, float cap, const float *slopes, void *out, int64_t out_stride,
+                                 void *stream);
+
+/* A paged cache in 4 bits.  A row (a token's head) holds, for each 32 consecutive elements
+ * x, the f16 minimum z = f16(min x), the f16 step s = f16((max x - min x) / 15) and
+ *   n = round((x - z) / s), in fp32, halves to even, 0 .. 15 (0 where s is 0);  x ~ n * s + z
+ * 5 bits an element.  |x - (n s + z)| <= s / 2 + 2^-11 (|min x| + max x - min x) + 2^-21.
+ * Elements past +-65504 count as that; a group that holds an infinity or a NaN is NaN.
+ * head_dim = 32 G, a multiple of 32, at most 256.  A row is 20 G bytes, starting on a 4-byte boundary:
+ *   key    element d: nibble d % 8 (bits 4 (d % 8) and up) of the 32-bit little-endian
+ *          word (d % 32 / 8) * G + d / 32
+ *   value  element d: nibble d / 16 of the G bytes from byte (d % 16) * G
+ *   both   from byte 16 G on, a word for each 32 elements: s in the low half, z in the high
+ * The strides of the caches (of these calls and of tml_hip_paged_attention_q4_dev) count
+ * BYTES and are multiples of 4. */
+#define TML_Q4_ROW_BYTES(head_dim) ((head_dim) / 32 * 20)
+
+/* New keys and values to their slots, as tml_hip_kv_store_dev, in 4 bits. */
+int tml_hip_kv_store_q4_dev(int type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k, const void *v,
+                            int64_t k_stride, int64_t v_stride, const int64_t *slots, void *k_cache, void *v_cache,
+                            int64_t n_blocks, int64_t block_size, int64_t block_stride, int64_t token_stride,
+                            int64_t head_stride, void *stream);
+
+/* The other way: the rows n * s + z of slots[t], rounded to `type`, to element d of head h of
+ * token t at k + t * k_stride + h * head_dim + d, and v alike.  A token whose slot is negative
+ * or not in the cache is left as it was.  A slot may be asked for more than once. */
+int tml_hip_kv_load_q4_dev(int type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k_cache,
+                           const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                           int64_t token_stride, int64_t head_stride, const int64_t *slots, void *k, void *v,
+                           int64_t k_stride, int64_t v_stride, void *stream);
+
+/* Attention of one new token a request over a paged cache in 4 bits: that of
+ * tml_hip_paged_attention_ex_dev over the values n * s + z, with its workspace.
+ *   q, out   F32, F16 or BF16
+ * Arithmetic: products and sums are fp32, of the nibbles as they are, of q as two f16 terms
+ * (2^-22 of each element, 2^-35 of its head's largest or of 2^-100) and of the weights
+ * times the values' steps as two f16 terms (2^-22 of each, 2^-38 of the largest step's).
+ * An infinite or NaN element of q makes its head's outputs NaN. */
+int tml_hip_paged_attention_q4_dev(int q_type, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   const void *q, int64_t q_stride, const void *k_cache, const void *v_cache,
+                                   int64_t n_blocks, int64_t block_size, int64_t block_stride, int64_t token_stride,
+                                   int64_t head_stride, const int *block_table, int64_t table_width,
+                                   int64_t table_stride, const int *seq_len, int64_t window, float scale, float cap,
+                                   const float *slopes, void *out, int64_t out_stride, void *stream);
+
+/* What logits say of tokens.  For each row of logits (`type`: F32, F16 or BF16, rows
+ * logits_stride apart), with log p = x - log sum e^x in fp32:
+ *   logprobs[row]      log p of tokens[row]; 0 where that is no column (padding).  tokens
+ *                      and logprobs are given together or both NULL
+ *   entropy[row]       - sum p log p, or NULL
+ *   top_ids[row, i], top_logprobs[row, i]   the `top` (0 to 64) most likely columns and their
+ *                      log p, by value, equal ones by the lower column; one of the two may
+ *                      be NULL.  NaN logits are never among them; past the last column -1
+ *                      and -inf
+ * A logit of -inf has probability 0.  A row of nothing else: -inf, entropy 0.  A NaN or +inf
+ * makes its row's values NaN (its ids are those of the logits that are no NaN).
+ * Columns below 2^31. */
+int tml_hip_token_logprobs_dev(int type, int64_t rows, int64_t cols, const void *logits, int64_t logits_stride,
+                               const int *tokens, float *logprobs, float *entropy, int64_t top, int *top_ids,
+                               float *top_logprobs, void *stream);
 
 /* Root-mean-square norm with the residual's addition:
  *   h = x + residual;  sum = h;  out = h / sqrt(mean(h^2) + eps) * weight

@@ -89,6 +89,12 @@ pub extern "c" fn tml_hip_paged_attention_dev(q_type: c_int, cache_type: c_int, 
 pub extern "c" fn tml_hip_rmsnorm_dev(elem_type: c_int, rows: i64, cols: i64, x: *const anyopaque, x_stride: i64, residual: ?*const anyopaque, residual_stride: i64, weight: ?[*]const f32, eps: f32, sum: ?*anyopaque, sum_stride: i64, out_type: c_int, out: *anyopaque, out_stride: i64, scales: ?[*]f32, group: i64, stream: ?*anyopaque) c_int;
 pub extern "c" fn tml_hip_matvec_q4g_dev(x_type: c_int, M: i64, N: i64, K: i64, x: *const anyopaque, x_stride: i64, x_scales: ?[*]const f32, x_group: i64, w: [*]const u8, w_stride: i64, w_scales: [*]const f32, group: i64, bias: ?[*]const f32, y_type: c_int, y: *anyopaque, y_stride: i64, stream: ?*anyopaque) c_int;
 pub extern "c" fn tml_hip_quantize_groups_dev(N: i64, K: i64, group: i64, w: [*]const f32, w_stride: i64, q: [*]u8, q_stride: i64, scales: [*]f32, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_paged_attention_ex_dev(q_type: c_int, cache_type: c_int, batch: i64, q_heads: i64, kv_heads: i64, head_dim: i64, q: *const anyopaque, q_stride: i64, k_cache: *const anyopaque, v_cache: *const anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, block_table: [*]const c_int, table_width: i64, table_stride: i64, seq_len: [*]const c_int, window: i64, scale: f32, cap: f32, slopes: ?[*]const f32, out: *anyopaque, out_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_prompt_attention_dev(q_type: c_int, cache_type: c_int, tokens: i64, requests: i64, q_heads: i64, kv_heads: i64, head_dim: i64, q: *const anyopaque, q_stride: i64, k_cache: *const anyopaque, v_cache: *const anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, block_table: [*]const c_int, table_width: i64, table_stride: i64, query_start: [*]const c_int, seq_len: [*]const c_int, prefix_len: ?[*]const c_int, window: i64, scale: f32, cap: f32, slopes: ?[*]const f32, out: *anyopaque, out_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_kv_store_q4_dev(elem_type: c_int, tokens: i64, kv_heads: i64, head_dim: i64, k: *const anyopaque, v: *const anyopaque, k_stride: i64, v_stride: i64, slots: [*]const i64, k_cache: *anyopaque, v_cache: *anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_kv_load_q4_dev(elem_type: c_int, tokens: i64, kv_heads: i64, head_dim: i64, k_cache: *const anyopaque, v_cache: *const anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, slots: [*]const i64, k: *anyopaque, v: *anyopaque, k_stride: i64, v_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_paged_attention_q4_dev(q_type: c_int, batch: i64, q_heads: i64, kv_heads: i64, head_dim: i64, q: *const anyopaque, q_stride: i64, k_cache: *const anyopaque, v_cache: *const anyopaque, n_blocks: i64, block_size: i64, block_stride: i64, token_stride: i64, head_stride: i64, block_table: [*]const c_int, table_width: i64, table_stride: i64, seq_len: [*]const c_int, window: i64, scale: f32, cap: f32, slopes: ?[*]const f32, out: *anyopaque, out_stride: i64, stream: ?*anyopaque) c_int;
+pub extern "c" fn tml_hip_token_logprobs_dev(elem_type: c_int, rows: i64, cols: i64, logits: *const anyopaque, logits_stride: i64, tokens: ?[*]const c_int, logprobs: ?[*]f32, entropy: ?[*]f32, top: i64, top_ids: ?[*]c_int, top_logprobs: ?[*]f32, stream: ?*anyopaque) c_int;
 
 // --------------------------------------------------------- .tl files
 pub extern "c" fn tml_tl_open(path: [*:0]const u8, out: *TlFile) c_int;

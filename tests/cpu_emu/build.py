@@ -95,7 +95,7 @@ OPTIMISED = {"gemm_dma", "gemm_mfma", "emu_main"}
 
 def _deps() -> list[str]:
     return [os.path.join(HERE, "hip", "hip_runtime.h"), os.path.join(CSRC, "tml_internal.hpp"),
-            os.path.join(CSRC, "host_copier.hpp"), os.path.join(CSRC, "serving.hpp"), os.path.join(ROOT, "include", "tomoul_hip.h"),
+            os.path.join(CSRC, "host_copier.hpp"), os.path.join(CSRC, "serving.hpp"), os.path.join(CSRC, "paged_split.hpp"), os.path.join(CSRC, "terms.hpp"), os.path.join(ROOT, "include", "tomoul_hip.h"),
             os.path.abspath(__file__)]
 
 

@@ -328,11 +328,16 @@ inline tml_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_f16(tml_emu_f16x8, tml_e
                                                            int) {
     return c;
 }
+typedef float tml_emu_f32x16 __attribute__((ext_vector_type(16)));
+inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x2f32(float, float, tml_emu_f32x16 c, int, int, int) { return c; }
+inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(tml_emu_bf16x8, tml_emu_bf16x8, tml_emu_f32x16 c, int, int, int) { return c; }
+inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(tml_emu_f16x8, tml_emu_f16x8, tml_emu_f32x16 c, int, int, int) { return c; }
 typedef int tml_emu_i32x4 __attribute__((ext_vector_type(4)));
 inline tml_emu_i32x4 __builtin_amdgcn_mfma_i32_16x16x64_i8(tml_emu_i32x4, tml_emu_i32x4, tml_emu_i32x4 c, int, int, int) {
     return c;
 }
 inline float __builtin_amdgcn_exp2f(float x) { return std::exp2(x); }
+inline float __builtin_amdgcn_rcpf(float x) { return 1.0f / x; }
 // Byte permute: selector 0-3 picks a byte of b, 4-7 one of a.
 inline uint32_t __builtin_amdgcn_perm(uint32_t a, uint32_t b, uint32_t sel) {
     const uint64_t both = (uint64_t)a << 32 | b;

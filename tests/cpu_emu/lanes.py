@@ -20,7 +20,7 @@ sys.path.insert(0, HERE)
 import build as emu_build  # noqa: E402  (tests/cpu_emu/build.py)
 
 EXE = os.path.join(emu_build.OUT_DIR, "emu_lanes")
-UNITS = ["rmsnorm", "kv", "matvec_q4g", "paged_attention"]
+UNITS = ["rmsnorm", "kv", "matvec_q4g", "paged_attention", "paged_attention_q4", "kv_q4", "prompt_attention", "logprobs"]
 HEADER = os.path.join(HERE, "lanes", "hip", "hip_runtime.h")
 
 

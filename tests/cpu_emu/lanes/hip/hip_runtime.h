@@ -36,6 +36,9 @@
 #define __builtin_amdgcn_mfma_f32_16x16x4f32 tml_emu_plain_mfma_f32
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16 tml_emu_plain_mfma_bf16
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16 tml_emu_plain_mfma_f16
+#define __builtin_amdgcn_mfma_f32_32x32x2f32 tml_emu_plain_mfma_f32_32
+#define __builtin_amdgcn_mfma_f32_32x32x16_bf16 tml_emu_plain_mfma_bf16_32
+#define __builtin_amdgcn_mfma_f32_32x32x16_f16 tml_emu_plain_mfma_f16_32
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8 tml_emu_plain_mfma_i8
 #define tml_emu_launcher tml_emu_plain_launcher
 #define tml_emu_launch tml_emu_plain_launch
@@ -54,6 +57,9 @@
 #undef __builtin_amdgcn_mfma_f32_16x16x4f32
 #undef __builtin_amdgcn_mfma_f32_16x16x32_bf16
 #undef __builtin_amdgcn_mfma_f32_16x16x32_f16
+#undef __builtin_amdgcn_mfma_f32_32x32x2f32
+#undef __builtin_amdgcn_mfma_f32_32x32x16_bf16
+#undef __builtin_amdgcn_mfma_f32_32x32x16_f16
 #undef __builtin_amdgcn_mfma_i32_16x16x64_i8
 #undef tml_emu_launcher
 #undef tml_emu_launch
@@ -192,4 +198,31 @@ TML_LANE_OP inline tml_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_f16(tml_emu_
 TML_LANE_OP inline tml_emu_i32x4 __builtin_amdgcn_mfma_i32_16x16x64_i8(tml_emu_i32x4 a, tml_emu_i32x4 b, tml_emu_i32x4 c, int, int, int) {
     const tml_lane_pair<tml_emu_i32x4> ab{a, b};
     return tml_lane_product<int8_t, tml_emu_i32x4, 16>(tml_lane_meet(__builtin_return_address(0), &ab, sizeof ab), c);
+}
+// The 32 x 32 ones: A row l % 32, B column l % 32, the k of half l / 32; rows
+// 8 j + 4 (l / 32) + i of column l % 32, in that order.
+template <typename E, int N>
+inline tml_emu_f32x16 tml_lane_product32(const tml_lane_meeting &m, tml_emu_f32x16 c) {
+    tml_lane_whole_wave(m);
+    const unsigned lane = tml_emu_lane();
+    for (unsigned i = 0; i < 16; ++i)
+        for (unsigned g = 0; g < 2; ++g) {
+            E a[N], b[N];
+            std::memcpy(a, m.data[32 * g + 8 * (i / 4) + 4 * (lane / 32) + i % 4], sizeof a);
+            std::memcpy(b, m.data[32 * g + lane % 32] + sizeof a, sizeof b);
+            for (int k = 0; k < N; ++k) c[i] += (float)a[k] * (float)b[k];
+        }
+    return c;
+}
+TML_LANE_OP inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float b, tml_emu_f32x16 c, int, int, int) {
+    const tml_lane_pair<float> ab{a, b};
+    return tml_lane_product32<float, 1>(tml_lane_meet(__builtin_return_address(0), &ab, sizeof ab), c);
+}
+TML_LANE_OP inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(tml_emu_bf16x8 a, tml_emu_bf16x8 b, tml_emu_f32x16 c, int, int, int) {
+    const tml_lane_pair<tml_emu_bf16x8> ab{a, b};
+    return tml_lane_product32<__bf16, 8>(tml_lane_meet(__builtin_return_address(0), &ab, sizeof ab), c);
+}
+TML_LANE_OP inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(tml_emu_f16x8 a, tml_emu_f16x8 b, tml_emu_f32x16 c, int, int, int) {
+    const tml_lane_pair<tml_emu_f16x8> ab{a, b};
+    return tml_lane_product32<_Float16, 8>(tml_lane_meet(__builtin_return_address(0), &ab, sizeof ab), c);
 }

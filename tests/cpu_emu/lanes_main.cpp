@@ -247,6 +247,12 @@ int main(int argc, char **argv) {
         if (name == "kv_plan") rc = call(tml_hip_kv_plan_dev, a);
         else if (name == "kv_store") rc = call(tml_hip_kv_store_dev, a);
         else if (name == "paged_attention") rc = call(tml_hip_paged_attention_dev, a);
+        else if (name == "paged_attention_ex") rc = call(tml_hip_paged_attention_ex_dev, a);
+        else if (name == "paged_attention_q4") rc = call(tml_hip_paged_attention_q4_dev, a);
+        else if (name == "prompt_attention") rc = call(tml_hip_prompt_attention_dev, a);
+        else if (name == "kv_store_q4") rc = call(tml_hip_kv_store_q4_dev, a);
+        else if (name == "kv_load_q4") rc = call(tml_hip_kv_load_q4_dev, a);
+        else if (name == "token_logprobs") rc = call(tml_hip_token_logprobs_dev, a);
         else if (name == "rmsnorm") rc = call(tml_hip_rmsnorm_dev, a);
         else if (name == "matvec_q4g") rc = call(tml_hip_matvec_q4g_dev, a);
         else if (name == "quantize_groups") rc = call(tml_hip_quantize_groups_dev, a);

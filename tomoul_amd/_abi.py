@@ -124,6 +124,21 @@ SIGNATURES = {
     "tml_hip_paged_attention_dev": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
                                                    _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _f,
                                                    _vp, _i64, _vp]),
+    "tml_hip_paged_attention_ex_dev": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
+                                                      _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                                                      _f, _f, _vp, _vp, _i64, _vp]),
+    "tml_hip_prompt_attention_dev": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
+                                                    _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                                    _vp, _i64, _f, _f, _vp, _vp, _i64, _vp]),
+    "tml_hip_kv_store_q4_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64,
+                                               _i64, _i64, _i64, _i64, _vp]),
+    "tml_hip_kv_load_q4_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                              _vp, _vp, _vp, _i64, _i64, _vp]),
+    "tml_hip_paged_attention_q4_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64,
+                                                      _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _f, _f, _vp,
+                                                      _vp, _i64, _vp]),
+    "tml_hip_token_logprobs_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp,
+                                                  _vp]),
     "tml_hip_rmsnorm_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i64,
                                            ctypes.c_int, _vp, _i64, _vp, _i64, _vp]),
     "tml_hip_matvec_q4g_dev": (ctypes.c_int, [ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
@@ -393,6 +408,82 @@ def paged_attention_dev(q_type: int, cache_type: int, batch: int, q_heads: int, 
                                             k_cache_ptr, v_cache_ptr, n_blocks, block_size, block_stride, token_stride,
                                             head_stride, block_table_ptr, table_width, table_stride, seq_len_ptr,
                                             window, scale, out_ptr, out_stride, stream))
+
+
+def paged_attention_ex_dev(q_type: int, cache_type: int, batch: int, q_heads: int, kv_heads: int, head_dim: int,
+                           q_ptr: int, q_stride: int, k_cache_ptr: int, v_cache_ptr: int, n_blocks: int,
+                           block_size: int, block_stride: int, token_stride: int, head_stride: int,
+                           block_table_ptr: int, table_width: int, table_stride: int, seq_len_ptr: int, scale: float,
+                           out_ptr: int, out_stride: int, *, window: int = 0, cap: float = 0.0,
+                           slopes_ptr: int | None = None, stream: int | None = None) -> None:
+    """paged_attention_dev with scores capped by a tanh and biased by distance."""
+    check(lib().tml_hip_paged_attention_ex_dev(q_type, cache_type, batch, q_heads, kv_heads, head_dim, q_ptr, q_stride,
+                                               k_cache_ptr, v_cache_ptr, n_blocks, block_size, block_stride,
+                                               token_stride, head_stride, block_table_ptr, table_width, table_stride,
+                                               seq_len_ptr, window, scale, cap, slopes_ptr, out_ptr, out_stride,
+                                               stream))
+
+
+def prompt_attention_dev(q_type: int, cache_type: int, tokens: int, requests: int, q_heads: int, kv_heads: int,
+                         head_dim: int, q_ptr: int, q_stride: int, k_cache_ptr: int, v_cache_ptr: int, n_blocks: int,
+                         block_size: int, block_stride: int, token_stride: int, head_stride: int, block_table_ptr: int,
+                         table_width: int, table_stride: int, query_start_ptr: int, seq_len_ptr: int, scale: float,
+                         out_ptr: int, out_stride: int, *, prefix_len_ptr: int | None = None, window: int = 0,
+                         cap: float = 0.0, slopes_ptr: int | None = None, stream: int | None = None) -> None:
+    """Attention of any number of new tokens a request over the paged cache: causal,
+    windowed and prefix masks, capped and biased scores."""
+    check(lib().tml_hip_prompt_attention_dev(q_type, cache_type, tokens, requests, q_heads, kv_heads, head_dim, q_ptr,
+                                             q_stride, k_cache_ptr, v_cache_ptr, n_blocks, block_size, block_stride,
+                                             token_stride, head_stride, block_table_ptr, table_width, table_stride,
+                                             query_start_ptr, seq_len_ptr, prefix_len_ptr, window, scale, cap,
+                                             slopes_ptr, out_ptr, out_stride, stream))
+
+
+def q4_row_bytes(head_dim: int) -> int:
+    """Bytes of a token's head in a 4-bit cache (TML_Q4_ROW_BYTES)."""
+    return head_dim // 32 * 20
+
+
+def kv_store_q4_dev(type_: int, tokens: int, kv_heads: int, head_dim: int, k_ptr: int, v_ptr: int, k_stride: int,
+                    v_stride: int, slots_ptr: int, k_cache_ptr: int, v_cache_ptr: int, n_blocks: int, block_size: int,
+                    block_stride: int, token_stride: int, head_stride: int, stream: int | None = None) -> None:
+    """New keys and values to their slots of a paged cache in 4 bits (cache strides in bytes)."""
+    check(lib().tml_hip_kv_store_q4_dev(type_, tokens, kv_heads, head_dim, k_ptr, v_ptr, k_stride, v_stride, slots_ptr,
+                                        k_cache_ptr, v_cache_ptr, n_blocks, block_size, block_stride, token_stride,
+                                        head_stride, stream))
+
+
+def kv_load_q4_dev(type_: int, tokens: int, kv_heads: int, head_dim: int, k_cache_ptr: int, v_cache_ptr: int,
+                   n_blocks: int, block_size: int, block_stride: int, token_stride: int, head_stride: int,
+                   slots_ptr: int, k_ptr: int, v_ptr: int, k_stride: int, v_stride: int,
+                   stream: int | None = None) -> None:
+    """The rows of given slots of a paged cache in 4 bits, as floats."""
+    check(lib().tml_hip_kv_load_q4_dev(type_, tokens, kv_heads, head_dim, k_cache_ptr, v_cache_ptr, n_blocks,
+                                       block_size, block_stride, token_stride, head_stride, slots_ptr, k_ptr, v_ptr,
+                                       k_stride, v_stride, stream))
+
+
+def paged_attention_q4_dev(q_type: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, q_ptr: int,
+                           q_stride: int, k_cache_ptr: int, v_cache_ptr: int, n_blocks: int, block_size: int,
+                           block_stride: int, token_stride: int, head_stride: int, block_table_ptr: int,
+                           table_width: int, table_stride: int, seq_len_ptr: int, scale: float, out_ptr: int,
+                           out_stride: int, *, window: int = 0, cap: float = 0.0, slopes_ptr: int | None = None,
+                           stream: int | None = None) -> None:
+    """Attention of one new token a request over a paged cache in 4 bits (cache strides in bytes)."""
+    check(lib().tml_hip_paged_attention_q4_dev(q_type, batch, q_heads, kv_heads, head_dim, q_ptr, q_stride, k_cache_ptr,
+                                               v_cache_ptr, n_blocks, block_size, block_stride, token_stride,
+                                               head_stride, block_table_ptr, table_width, table_stride, seq_len_ptr,
+                                               window, scale, cap, slopes_ptr, out_ptr, out_stride, stream))
+
+
+def token_logprobs_dev(type_: int, rows: int, cols: int, logits_ptr: int, logits_stride: int, *,
+                       tokens_ptr: int | None = None, logprobs_ptr: int | None = None, entropy_ptr: int | None = None,
+                       top: int = 0, top_ids_ptr: int | None = None, top_logprobs_ptr: int | None = None,
+                       stream: int | None = None) -> None:
+    """Log probabilities of given tokens (int32), the entropy, and the `top` most likely
+    columns with theirs, of each row of logits."""
+    check(lib().tml_hip_token_logprobs_dev(type_, rows, cols, logits_ptr, logits_stride, tokens_ptr, logprobs_ptr,
+                                           entropy_ptr, top, top_ids_ptr, top_logprobs_ptr, stream))
 
 
 def rmsnorm_dev(type_: int, rows: int, cols: int, x_ptr: int, x_stride: int, weight_ptr: int | None, eps: float,

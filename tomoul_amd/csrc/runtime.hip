@@ -309,10 +309,10 @@ Status ensure_workspace(DeviceCtx *c, MatmulArgs &m, hipStream_t s, Workspace *w
     return Status::Ok();
 }
 
-// The same for the paged attention's parts, which need no counters.  They have a buffer
+// The same for the paged attentions' parts, which need no counters.  They have a buffer
 // of their own: an attention and a split GEMM may run on two streams.
-Status attention_workspace(DeviceCtx *c, const PagedAttentionArgs &a, hipStream_t s, Workspace *ws) {
-    const size_t bytes = paged_attention_workspace_floats(a) * sizeof(float);
+Status attention_workspace(DeviceCtx *c, size_t floats, hipStream_t s, Workspace *ws) {
+    const size_t bytes = floats * sizeof(float);
     if (bytes > c->attention.bytes) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
         TML_HIP_TRY(hipStreamIsCapturing(s, &cap));
@@ -1164,24 +1164,115 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
                                   (hipStream_t)stream));
 }
 
+static int run_paged_attention(const PagedAttentionArgs &a, void *stream) {
+    auto run = [&]() -> Status {
+        DeviceCtx *c = nullptr;
+        TML_TRY(current_ctx(&c));
+        TML_TRY(check_paged_attention(a));
+        Workspace ws;
+        TML_TRY(attention_workspace(c, paged_attention_workspace_floats(a), (hipStream_t)stream, &ws));
+        return launch_paged_attention(a, ws, (hipStream_t)stream);
+    };
+    return report(run());
+}
+
 int tml_hip_paged_attention_dev(int q_type, int cache_type, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                 int64_t head_dim, const void *q, int64_t q_stride, const void *k_cache,
                                 const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
                                 int64_t token_stride, int64_t head_stride, const int *block_table,
                                 int64_t table_width, int64_t table_stride, const int *seq_len, int64_t window,
                                 float scale, void *out, int64_t out_stride, void *stream) {
-    const PagedAttentionArgs a{q_type, cache_type, batch, q_heads, kv_heads, head_dim, q, q_stride, k_cache, v_cache,
+    return run_paged_attention({q_type, cache_type, batch, q_heads, kv_heads, head_dim, q, q_stride, k_cache, v_cache,
+                                n_blocks, block_size, block_stride, token_stride, head_stride, block_table, table_width,
+                                table_stride, seq_len, window, scale, out, out_stride},
+                               stream);
+}
+
+int tml_hip_paged_attention_ex_dev(int q_type, int cache_type, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                   int64_t head_dim, const void *q, int64_t q_stride, const void *k_cache,
+                                   const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                                   int64_t token_stride, int64_t head_stride, const int *block_table,
+                                   int64_t table_width, int64_t table_stride, const int *seq_len, int64_t window,
+                                   float scale, float cap, const float *slopes, void *out, int64_t out_stride,
+                                   void *stream) {
+    return run_paged_attention({q_type, cache_type, batch, q_heads, kv_heads, head_dim, q, q_stride, k_cache, v_cache,
+                                n_blocks, block_size, block_stride, token_stride, head_stride, block_table, table_width,
+                                table_stride, seq_len, window, scale, out, out_stride, cap, slopes},
+                               stream);
+}
+
+int tml_hip_kv_store_q4_dev(int type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k, const void *v,
+                            int64_t k_stride, int64_t v_stride, const int64_t *slots, void *k_cache, void *v_cache,
+                            int64_t n_blocks, int64_t block_size, int64_t block_stride, int64_t token_stride,
+                            int64_t head_stride, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_kv_store_q4({type, tokens, kv_heads, head_dim, k, v, nullptr, nullptr, k_stride, v_stride, slots,
+                                      k_cache, v_cache, n_blocks, block_size, block_stride, token_stride, head_stride},
+                                     (hipStream_t)stream));
+}
+
+int tml_hip_kv_load_q4_dev(int type, int64_t tokens, int64_t kv_heads, int64_t head_dim, const void *k_cache,
+                           const void *v_cache, int64_t n_blocks, int64_t block_size, int64_t block_stride,
+                           int64_t token_stride, int64_t head_stride, const int64_t *slots, void *k, void *v,
+                           int64_t k_stride, int64_t v_stride, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_kv_load_q4({type, tokens, kv_heads, head_dim, nullptr, nullptr, k, v, k_stride, v_stride, slots,
+                                     const_cast<void *>(k_cache), const_cast<void *>(v_cache), n_blocks, block_size,
+                                     block_stride, token_stride, head_stride},
+                                    (hipStream_t)stream));
+}
+
+int tml_hip_paged_attention_q4_dev(int q_type, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   const void *q, int64_t q_stride, const void *k_cache, const void *v_cache,
+                                   int64_t n_blocks, int64_t block_size, int64_t block_stride, int64_t token_stride,
+                                   int64_t head_stride, const int *block_table, int64_t table_width,
+                                   int64_t table_stride, const int *seq_len, int64_t window, float scale, float cap,
+                                   const float *slopes, void *out, int64_t out_stride, void *stream) {
+    const PagedAttentionArgs a{q_type, q_type, batch, q_heads, kv_heads, head_dim, q, q_stride, k_cache, v_cache,
                                n_blocks, block_size, block_stride, token_stride, head_stride, block_table, table_width,
-                               table_stride, seq_len, window, scale, out, out_stride};
+                               table_stride, seq_len, window, scale, out, out_stride, cap, slopes};
     auto run = [&]() -> Status {
         DeviceCtx *c = nullptr;
         TML_TRY(current_ctx(&c));
-        TML_TRY(check_paged_attention(a));
+        TML_TRY(check_paged_attention_q4(a));
         Workspace ws;
-        TML_TRY(attention_workspace(c, a, (hipStream_t)stream, &ws));
-        return launch_paged_attention(a, ws, (hipStream_t)stream);
+        TML_TRY(attention_workspace(c, paged_attention_q4_workspace_floats(a), (hipStream_t)stream, &ws));
+        return launch_paged_attention_q4(a, ws, (hipStream_t)stream);
     };
     return report(run());
+}
+
+int tml_hip_prompt_attention_dev(int q_type, int cache_type, int64_t tokens, int64_t requests, int64_t q_heads,
+                                 int64_t kv_heads, int64_t head_dim, const void *q, int64_t q_stride,
+                                 const void *k_cache, const void *v_cache, int64_t n_blocks, int64_t block_size,
+                                 int64_t block_stride, int64_t token_stride, int64_t head_stride,
+                                 const int *block_table, int64_t table_width, int64_t table_stride,
+                                 const int *query_start, const int *seq_len, const int *prefix_len, int64_t window,
+                                 float scale, float cap, const float *slopes, void *out, int64_t out_stride,
+                                 void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_prompt_attention({q_type, cache_type, tokens, requests, q_heads, kv_heads, head_dim, q, q_stride,
+                                           k_cache, v_cache, n_blocks, block_size, block_stride, token_stride,
+                                           head_stride, block_table, table_width, table_stride, query_start, seq_len,
+                                           prefix_len, window, scale, cap, slopes, out, out_stride},
+                                          (hipStream_t)stream));
+}
+
+int tml_hip_token_logprobs_dev(int type, int64_t rows, int64_t cols, const void *logits, int64_t logits_stride,
+                               const int *tokens, float *logprobs, float *entropy, int64_t top, int *top_ids,
+                               float *top_logprobs, void *stream) {
+    DeviceCtx *c = nullptr;
+    Status s = current_ctx(&c);
+    if (!s.ok()) return report(s);
+    return report(launch_token_logprobs({type, rows, cols, logits, logits_stride, tokens, logprobs, entropy, top, top_ids,
+                                         top_logprobs},
+                                        (hipStream_t)stream));
 }
 
 int tml_hip_rmsnorm_dev(int type, int64_t rows, int64_t cols, const void *x, int64_t x_stride, const void *residual,

@@ -1,5 +1,5 @@
-// What the serving operators (rmsnorm.hip, kv.hip, matvec_q4g.hip,
-// paged_attention.hip) share: element types, eight elements at a time as
+// What the serving operators (rmsnorm.hip, kv.hip, kv_q4.hip, matvec_q4g.hip,
+// paged_attention.hip, paged_attention_q4.hip, prompt_attention.hip, logprobs.hip) share: element types, eight elements at a time as
 // floats, and the launchers' arguments.
 #pragma once
 
@@ -155,9 +155,76 @@ struct PagedAttentionArgs {
     float scale;
     void *out;
     int64_t out_stride;
+    float cap = 0.0f;               // of the scores: 0 for none
+    const float *slopes = nullptr;  // [q_heads] of the bias by distance, or nullptr
 };
 Status check_paged_attention(const PagedAttentionArgs &a);
 size_t paged_attention_workspace_floats(const PagedAttentionArgs &a);
 Status launch_paged_attention(const PagedAttentionArgs &a, const Workspace &ws, hipStream_t s);
+
+// The same over a cache in 4 bits: cache strides in bytes, cache_type unused.
+Status check_paged_attention_q4(const PagedAttentionArgs &a);
+size_t paged_attention_q4_workspace_floats(const PagedAttentionArgs &a);
+Status launch_paged_attention_q4(const PagedAttentionArgs &a, const Workspace &ws, hipStream_t s);
+
+constexpr float kLog2E = 1.44269504088896341f;
+
+// A cap of the scores: none, or one whose reciprocal is an ordinary number too.
+inline bool valid_cap(float cap) { return cap == 0.0f || (cap >= 0x1p-100f && cap <= 0x1p100f); }
+
+// cap * tanh(x / cap): past |z| = 0.35 (1 - t) / (1 + t) of t = e^(-2 |z|), below it the
+// series z - z^3 / 3 + 2 z^5 / 15 - .. to z^11 (the next term is below 2^-25 of z there),
+// since the first loses the bits that 1 - t does.
+__device__ __forceinline__ float cap_score(float x, float cap, float inv_cap) {
+    const float z = x * inv_cap, y = z * z;
+    const float t = __builtin_amdgcn_exp2f(fabsf(z) * -2.88539008177792681f);
+    const float far = __builtin_copysignf(cap * (1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+    const float series = -1.0f / 3 + y * (2.0f / 15 + y * (-17.0f / 315 + y * (62.0f / 2835 + y * (-1382.0f / 155925))));
+    return fabsf(z) < 0.35f ? x + x * (y * series) : far;
+}
+
+struct KvStore4Args {
+    int type;
+    int64_t tokens, kv_heads, head_dim;
+    const void *k, *v;  // (store)
+    void *k_out, *v_out;  // (load)
+    int64_t k_stride, v_stride;
+    const int64_t *slots;
+    void *k_cache, *v_cache;
+    int64_t n_blocks, block_size, block_stride, token_stride, head_stride;  // bytes
+};
+Status launch_kv_store_q4(const KvStore4Args &a, hipStream_t s);
+Status launch_kv_load_q4(const KvStore4Args &a, hipStream_t s);
+
+struct PromptAttentionArgs {
+    int q_type, cache_type;
+    int64_t tokens, requests, q_heads, kv_heads, head_dim;
+    const void *q;
+    int64_t q_stride;
+    const void *k_cache, *v_cache;
+    int64_t n_blocks, block_size, block_stride, token_stride, head_stride;
+    const int *block_table;
+    int64_t table_width, table_stride;
+    const int *query_start, *seq_len, *prefix_len;
+    int64_t window;
+    float scale, cap;
+    const float *slopes;
+    void *out;
+    int64_t out_stride;
+};
+Status launch_prompt_attention(const PromptAttentionArgs &a, hipStream_t s);
+
+struct LogprobsArgs {
+    int type;
+    int64_t rows, cols;
+    const void *logits;
+    int64_t stride;
+    const int *tokens;
+    float *logprobs, *entropy;
+    int64_t top;
+    int *top_ids;
+    float *top_logprobs;
+};
+Status launch_token_logprobs(const LogprobsArgs &a, hipStream_t s);
 
 }  // namespace tml
