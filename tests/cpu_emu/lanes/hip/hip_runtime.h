@@ -39,6 +39,7 @@
 #define __builtin_amdgcn_mfma_f32_32x32x2f32 tml_emu_plain_mfma_f32_32
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 tml_emu_plain_mfma_bf16_32
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16 tml_emu_plain_mfma_f16_32
+#define __builtin_amdgcn_ds_read_tr16_b64_v4i16 tml_emu_plain_read_tr
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8 tml_emu_plain_mfma_i8
 #define tml_emu_launcher tml_emu_plain_launcher
 #define tml_emu_launch tml_emu_plain_launch
@@ -60,6 +61,7 @@
 #undef __builtin_amdgcn_mfma_f32_32x32x2f32
 #undef __builtin_amdgcn_mfma_f32_32x32x16_bf16
 #undef __builtin_amdgcn_mfma_f32_32x32x16_f16
+#undef __builtin_amdgcn_ds_read_tr16_b64_v4i16
 #undef __builtin_amdgcn_mfma_i32_16x16x64_i8
 #undef tml_emu_launcher
 #undef tml_emu_launch
@@ -225,4 +227,19 @@ TML_LANE_OP inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(tml_em
 TML_LANE_OP inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(tml_emu_f16x8 a, tml_emu_f16x8 b, tml_emu_f32x16 c, int, int, int) {
     const tml_lane_pair<tml_emu_f16x8> ab{a, b};
     return tml_lane_product32<_Float16, 8>(tml_lane_meet(__builtin_return_address(0), &ab, sizeof ab), c);
+}
+// Lane i of 16 brings row i / 4, columns 4 (i % 4) and on, of a 4 x 16 block; gets column i.
+typedef short tml_emu_s16x4 __attribute__((ext_vector_type(4)));
+TML_LANE_OP inline tml_emu_s16x4 __builtin_amdgcn_ds_read_tr16_b64_v4i16(__attribute__((address_space(3))) tml_emu_s16x4 *p) {
+    const tml_emu_s16x4 mine = *(const tml_emu_s16x4 *)p;
+    const tml_lane_meeting &m = tml_lane_meet(__builtin_return_address(0), &mine, sizeof mine);
+    tml_lane_whole_wave(m);
+    const unsigned lane = tml_emu_lane();
+    tml_emu_s16x4 out;
+    for (unsigned j = 0; j < 4; ++j) {
+        tml_emu_s16x4 four;
+        std::memcpy(&four, m.data[(lane & ~15u) + 4 * j + lane % 16 / 4], sizeof four);
+        out[j] = four[lane % 4];
+    }
+    return out;
 }

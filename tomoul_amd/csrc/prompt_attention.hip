@@ -13,16 +13,17 @@
 // of the group at a token: row r is token r / group, head r % group, so short prompts
 // with grouped heads fill the matrix instructions and share each key.  Its four waves
 // have 32 rows each and go through the tiles of tokens that any of the rows sees, with a
-// running maximum and sum; keys and values of a tile are in LDS, those of the next on
-// their way to registers.
+// running maximum and sum.  Keys and values are copied straight to LDS, the next tile's
+// while this one is multiplied; one barrier a tile.
 //   scores   S^T = K Q^T, 32 tokens x 32 rows: a lane holds sixteen tokens of one row, so a
 //            row's maximum and sum need one exchange between two lanes
 //   weights  are the B operand of the next product as they lie if its k slots are numbered
 //            as the lane's tokens are: 8 j + 4 (lane / 32) + i
-//   values   O^T += V^T P^T: V goes to LDS transposed, its tokens in that order
-// 16-byte pieces of a row in LDS are exchanged by the row's number, so that lanes that
-// read the same piece of different rows use all banks.
-//
+//   values   O^T += V^T P^T: the LDS reads that transpose 4 x 16 blocks give a lane four
+//            tokens of its d
+// 16-byte pieces of a row in LDS are exchanged by the token's number, so that neither the
+// reads of one piece of 16 rows (keys) nor those of 64 bytes of four rows (values) meet in a
+// bank.
 // Precision: sums, maxima and the scores are fp32.  f32 queries go in as terms of the
 // cache's type (two of f16, scaled by a power of two, three of bf16), and so do the
 // weights where the output is f32; where it has 16 bits the weights are rounded to them
@@ -58,6 +59,24 @@ __device__ __forceinline__ floatx16 mma32(const srv_u32x4 &x, const srv_u32x4 &y
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
 }
 
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+#define TML_GPTR(p) ((__attribute__((address_space(1))) void *)(p))
+#define TML_LPTR(p) ((__attribute__((address_space(3))) void *)(p))
+// Lane i of a group of 16 reads four numbers, row i / 4 and columns 4 (i % 4) and on of a block
+// of 4 x 16; it gets the four rows of column i.
+__device__ __forceinline__ shortx4 read_turned(const shortx4 *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)p);
+}
+
+// A value that the compiler takes to be new here: what is made of it is made anew in every
+// tile instead of being kept in registers.
+__device__ __forceinline__ int anew(int v) {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+v"(v));
+#endif
+    return v;
+}
+
 // New tokens of request r: their first row of q, and how many (not past q's end).
 struct Request {
     int first, count;
@@ -68,14 +87,20 @@ __device__ __forceinline__ Request request_at(const PromptAttentionArgs &a, int6
 }
 __device__ __forceinline__ int64_t tiles_of(const PromptShape &sh, int count) { return ((int64_t)count * sh.group + kRows - 1) / kRows; }
 
-// Where piece `piece` of row `row` lies among the row's N pieces of 16 bytes (N a power of
-// two): 16 rows of neighbouring lanes meet each bank once.
+// What a token's pieces of 16 bytes are exchanged by in LDS, N of them a row: piece p is in
+// place p ^ this.
 template <int N>
-__device__ __forceinline__ int placed(int row, int piece) {
-    if constexpr (N >= 16) return piece ^ (row & 15);
-    else if constexpr (N == 8) return piece ^ ((row ^ row >> 3) & 7);
-    else return piece ^ (row >> 2 & 3);
+__device__ __forceinline__ int turn_of(int token) {
+    return N >= 16 ? (token & 3) << 2 | (token >> 2 & 3) : (token >> 1 & 1) << 2 | (token >> 2 & 3);
 }
+
+// Where a token's key and value are.
+struct alignas(16) RowAt {
+    const char *k, *v;
+};
+
+// Read in the place of what no one may look at, and of what is past the head size.
+__device__ srv_u32x4 zero_row[64];
 
 // CT: the cache's type.  QT: q's and the output's (CT or f32).  DP: the head size rounded
 // up to 64, 128 or 256.  FORM: the scores are capped or biased.
@@ -83,30 +108,34 @@ template <int CT, int QT, int DP, bool FORM>
 struct Prompt {
     static constexpr bool kF32 = CT == TML_TYPE_F32;
     static constexpr int kBytes = kF32 ? 4 : 2;
-    static constexpr int E = 16 / kBytes;                       // elements of a piece
     static constexpr int NQ = QT == CT ? 1 : CT == TML_TYPE_F16 ? 2 : 3;
     static constexpr int NP = QT == CT ? 1 : CT == TML_TYPE_F16 ? 2 : 3;
-    static constexpr int BN = kF32 || DP == 256 ? 32 : 64;       // tokens of a tile
-    static constexpr int KP = DP / E, VP = BN / E;               // pieces of a row of K, of V^T
-    static constexpr int kLoadsK = BN * KP / kThreads;           // pieces a thread moves
-    static constexpr int kItems = BN / 4 * KP;                   // V: four tokens of a piece each
-    static constexpr int kLoadsV = (kItems + kThreads - 1) / kThreads;
-    static constexpr int kQ = kF32 ? DP / 8 : DP / 16;           // 16 bytes of q a lane, each term
-    // registers of a lane: q, output, scores, tiles under way; two workgroups a CU where they fit half
-    static constexpr int kRegs = 4 * kQ * NQ + DP / 2 + BN / 2 + 4 * kLoadsK + 16 * kLoadsV + 16 * NP;
-    static constexpr int kPerCu = kRegs > 190 ? 1 : 2;
+    static constexpr int BN = kF32 || DP == 256 ? 32 : 64;  // tokens of a tile
+    static constexpr int KP = DP * kBytes / 16;              // pieces of a token's row
+    static constexpr int kOwn = BN / kWaves;                 // tokens that a wave copies
+    static constexpr int kCopies = kOwn * KP / 64;
+    static constexpr int kQ = kF32 ? DP / 8 : DP / 16;       // 16 bytes of q a lane, each term
+    // registers of a lane: q, output, scores and weights; two workgroups a CU where they leave room
+    static constexpr int kRegs = 4 * kQ * NQ + DP / 2 + BN / 2 + BN / 4 * NP;
+    static constexpr int kPerCu = kRegs > 180 ? 1 : 2;
 };
 
 template <int CT, int QT, int DP, bool FORM>
 __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void prompt_attention_kernel(PromptAttentionArgs a, PromptShape sh) {
     using C = Prompt<CT, QT, DP, FORM>;
     constexpr bool kF32 = C::kF32;
-    constexpr int kBytes = C::kBytes, E = C::E, NQ = C::NQ, NP = C::NP, BN = C::BN, KP = C::KP, VP = C::VP, kQ = C::kQ;
-    // base of the weights' exponent: f16 terms of e^(s - m) reach down to 2^-39 of the largest
-    constexpr float kUp = CT == TML_TYPE_F16 ? 14.0f : 0.0f;
+    constexpr int kBytes = C::kBytes, NQ = C::NQ, NP = C::NP, BN = C::BN, KP = C::KP, kQ = C::kQ, kOwn = C::kOwn;
+    // The maximum that weights are relative to may fall behind the row's by kBehind (in
+    // powers of two) before sums are scaled: with 32 rows one of them rises in most tiles.
+    // kUp: base of the weights' exponent, for f16's range; terms of them reach down to 2^-39
+    // (f32 outputs) or 2^-24 (one term, and the maximum behind) of the largest.
+    constexpr float kBehind = QT == TML_TYPE_F32 ? 0.0f : 8.0f;
+    constexpr float kUp = CT != TML_TYPE_F16 ? 0.0f : QT == TML_TYPE_F32 ? 14.0f : 7.0f;
 
-    __shared__ srv_u32x4 lds_k[BN * KP], lds_v[DP * VP];
-    __shared__ int64_t row_off[kWaves][BN];
+    // (arrays of their own: the compiler waits for copies to the array that it reads)
+    __shared__ srv_u32x4 lds_k0[BN * KP], lds_k1[BN * KP], lds_v0[BN * KP], lds_v1[BN * KP];
+    __shared__ RowAt row_at[kWaves][kOwn];
+    __shared__ uint64_t lds_live[2];  // of a tile's tokens
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
     const int l32 = lane & 31, half = lane >> 5;
     const int D = (int)a.head_dim;
@@ -153,11 +182,13 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
     const int64_t wave_first = ctx + token_of(wave0), wave_last = ctx + token_of(min(wave0 + 31, rows - 1));
     const int64_t row = min(row0 + 32 * wave + l32, rows - 1);
     const int64_t token = token_of(row), head = (int64_t)kv * sh.group + (row - token * sh.group);
-    const int64_t pos = ctx + token, low = low_of(pos), high = high_of(pos);
+    const int pos = (int)(ctx + token);
+    const uint32_t low = (uint32_t)low_of(pos), high = (uint32_t)max(high_of(pos), (int64_t)0);  // (at most 2^31)
 
     // ---- q: lane (row, half) has the k of its half
+    // (with the scale's sign, for maxima to be taken before the scale; a scale of 0 is a q of 0)
     srv_u32x4 q[NQ][kQ];
-    float to_score = a.scale;
+    float to_score = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
     {
         const int64_t at = (first + token) * a.q_stride + head * D;
         if constexpr (kF32) {
@@ -207,6 +238,13 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
             }
         }
     }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int c = 0; c < kQ; ++c) {
+            if (a.scale < 0.0f) q[n][c] ^= kF32 ? 0x80000000u : 0x80008000u;
+            if (a.scale == 0.0f) q[n][c] = srv_u32x4{0, 0, 0, 0};
+        }
     const float to_log2 = to_score * kLog2E;
     float slope = 0.0f, inv_cap = 0.0f;
     if constexpr (FORM) {
@@ -221,171 +259,196 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
 
-    // ---- the tiles' rows: lane % BN looks up a token's
+    // ---- copies: a wave's tokens are its share of the tile, lane % kOwn looks one up
     auto block_of = [&](int64_t k0) {
-        const int64_t tok = k0 + lane % BN;
+        const int64_t tok = k0 + wave * kOwn + lane % kOwn;
         return a.block_table[b * a.table_stride + (uint32_t)min(tok, len - 1) / (uint32_t)P];
     };
-    auto rows_of = [&](int64_t k0, int in_block) {
-        const int64_t tok = k0 + lane % BN;
+    auto copy_tile = [&](srv_u32x4 *to_k, srv_u32x4 *to_v, uint64_t *to_live, int64_t k0, int in_block) {
+        const int64_t tok = k0 + wave * kOwn + lane % kOwn;
         const bool live = tok < end && in_block >= 0 && in_block < a.n_blocks;
-        // (a token no one may look at reads the cache's first row)
-        const int64_t off = live ? (in_block * a.block_stride + (int64_t)((uint32_t)tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes : 0;
-        row_off[wave][lane % BN] = off;
+        const int64_t off = (in_block * a.block_stride + (int64_t)((uint32_t)tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes;
+        row_at[wave][lane % kOwn] = live ? RowAt{(const char *)a.k_cache + off, (const char *)a.v_cache + off} : RowAt{(const char *)zero_row, (const char *)zero_row};
+        const uint64_t all = __builtin_amdgcn_ballot_w64(live);
+        if (lane == 0) {
+            if constexpr (kOwn == 16) ((uint16_t *)to_live)[wave] = (uint16_t)all;
+            else ((uint8_t *)to_live)[wave] = (uint8_t)all;
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        return __builtin_amdgcn_ballot_w64(live);
-    };
-    srv_u32x4 kr[C::kLoadsK], vr[C::kLoadsV][4];
-    auto load_tile = [&]() {
+        const int copier = anew(lane);
 #pragma unroll
-        for (int i = 0; i < C::kLoadsK; ++i) {
-            const int at = i * kThreads + (int)threadIdx.x, tok = at / KP, d = at % KP * E;
-            kr[i] = *(const srv_u32x4 *)((const char *)a.k_cache + row_off[wave][tok] + (d < D ? d : 0) * kBytes);
-        }
-#pragma unroll
-        for (int i = 0; i < C::kLoadsV; ++i) {
-            const int at = min(i * kThreads + (int)threadIdx.x, C::kItems - 1), d = at % KP * E;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) vr[i][j] = *(const srv_u32x4 *)((const char *)a.v_cache + row_off[wave][at / KP * 4 + j] + (d < D ? d : 0) * kBytes);
+        for (int i = 0; i < C::kCopies; ++i) {
+            const int at = i * 64 + copier, t = at / KP, piece = (at % KP) ^ turn_of<KP>(wave * kOwn + t);
+            const RowAt row_here = row_at[wave][t];
+            const char *from_k = row_here.k + 16 * piece, *from_v = row_here.v + 16 * piece;
+            if (D < DP && piece * (16 / kBytes) >= D) from_k = from_v = (const char *)(zero_row + piece);
+            __builtin_amdgcn_global_load_lds(TML_GPTR(from_k), TML_LPTR(to_k + wave * kOwn * KP + i * 64), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(TML_GPTR(from_v), TML_LPTR(to_v + wave * kOwn * KP + i * 64), 16, 0, 0);
         }
     };
-    // To LDS: past the head size zeros (what is there may be infinite), and zeros for values no one may look at.
-    auto store_tile = [&](uint64_t live) {
+
+    // ---- a tile
+    auto multiply = [&](const srv_u32x4 *tile_k, const srv_u32x4 *tile_v, uint64_t live, int64_t k0) {
+        // rows of this wave that see none of the tile, or all of it
+        if (k0 >= high_of(wave_last) || k0 + BN <= low_of(wave_first)) return;
+        const bool whole = k0 + BN <= high_of(wave_first) && k0 >= low_of(wave_last) && (live & (~0ull >> (64 - BN))) == ~0ull >> (64 - BN);
+
+        // scores, before the scale (FORM: as powers of two)
+        float s[BN / 2];
+        floatx16 sum[BN / 32];
 #pragma unroll
-        for (int i = 0; i < C::kLoadsK; ++i) {
-            const int at = i * kThreads + (int)threadIdx.x, tok = at / KP, piece = at % KP;
-            if (D < DP && piece * E >= D) kr[i] = srv_u32x4{0, 0, 0, 0};
-            lds_k[tok * KP + placed<KP>(tok, piece)] = kr[i];
-        }
+        for (int u = 0; u < BN / 32; ++u)
 #pragma unroll
-        for (int i = 0; i < C::kLoadsV; ++i) {
-            const int at = i * kThreads + (int)threadIdx.x, quad = at / KP, d0 = at % KP * E;
-            if (C::kItems % kThreads != 0 && at >= C::kItems) break;
+            for (int i = 0; i < 16; ++i) sum[u][i] = 0.0f;
+        const int k_row = anew(l32);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if ((live >> (4 * quad + j) & 1) == 0) vr[i][j] = srv_u32x4{0, 0, 0, 0};
-            if constexpr (kF32) {  // a piece is four tokens
+        for (int c = 0; c < kQ; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) lds_v[(d0 + e) * VP + placed<VP>(d0 + e, quad)] = srv_u32x4{vr[i][0][e], vr[i][1][e], vr[i][2][e], vr[i][3][e]};
-            } else {  // a piece is four tokens and the four eight further on: quads 0 2 1 3 of sixteen tokens
-                const int spot = (quad & ~3) + ((quad & 1) << 1 | (quad >> 1 & 1));
-                srv_u32x2 *const to = (srv_u32x2 *)lds_v + (spot & 1);
+            for (int u = 0; u < BN / 32; ++u) {
+                const srv_u32x4 k = tile_k[32 * u * KP + k_row * KP + ((2 * c + half) ^ turn_of<KP>(k_row))];
+                if constexpr (kF32) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
-                    to[2 * ((d0 + e) * VP + placed<VP>(d0 + e, spot >> 1))] =
-                        srv_u32x2{__builtin_amdgcn_perm(vr[i][1][e / 2], vr[i][0][e / 2], sel), __builtin_amdgcn_perm(vr[i][3][e / 2], vr[i][2][e / 2], sel)};
+                    for (int e = 0; e < 4; ++e) sum[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[0][c][e]), sum[u], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) sum[u] = mma32<CT>(k, q[n][c], sum[u]);
                 }
             }
+#pragma unroll
+        for (int i = 0; i < BN / 2; ++i) s[i] = sum[i / 16][i % 16];
+        if constexpr (!kF32) {  // reads four ahead of the products
+            constexpr int kReads = kQ * (BN / 32);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 4; i < kReads; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4 * NQ, 0);
+        }
+        if constexpr (FORM) {
+            if (inv_cap != 0.0f) {
+#pragma unroll
+                for (int i = 0; i < BN / 2; ++i) {
+                    if constexpr (QT == TML_TYPE_F32) {
+                        s[i] = cap_score(s[i] * to_score, a.cap, inv_cap) * kLog2E;
+                    } else {  // cap - 2 cap / (1 + e^(2 x / cap)): 2^-23 of the cap off, next to 16-bit weights
+                        const float e = __builtin_amdgcn_exp2f(s[i] * (2.0f * to_log2 * inv_cap));
+                        s[i] = fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * kLog2E * a.cap, kLog2E * a.cap);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < BN / 2; ++i) s[i] *= to_log2;
+            }
+            if (a.slopes != nullptr) {
+                const float from = (float)((int64_t)pos - k0 - 4 * half);
+#pragma unroll
+                for (int i = 0; i < BN / 2; ++i) s[i] = fmaf(-slope, fabsf(from - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4)), s[i]);
+            }
+        }
+        const float unit = FORM ? 1.0f : to_log2;  // of the scores
+        if (!whole) {
+            const uint32_t k = (uint32_t)k0;
+            const int from = (low > k ? (int)min(low - k, (uint32_t)BN) : 0) - 4 * half, to = (high > k ? (int)min(high - k, (uint32_t)BN) : 0) - 4 * half;
+            const uint32_t there[2] = {(uint32_t)live >> 4 * half, (uint32_t)(live >> 32) >> 4 * half};
+#pragma unroll
+            for (int i = 0; i < BN / 2; ++i) {
+                const int t = 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4;  // (+ 4 half)
+                if (t < from || t >= to || (there[i / 16] >> t % 32 & 1) == 0) s[i] = -INFINITY;
+            }
+        }
+        // weights
+        float most = s[0];
+#pragma unroll
+        for (int i = 1; i < BN / 2; ++i) most = fmaxf(most, s[i]);
+        most = fmaxf(most, __shfl_xor(most, 32)) * unit;
+        if (__builtin_amdgcn_ballot_w64(most > m + kBehind) != 0) {
+            const float m_new = fmaxf(m, most);
+            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= f;
+        }
+        const float base = kUp - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+        for (int i = 0; i < BN / 2; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], unit, base));
+            l += s[i];
+        }
+        // values
+        if constexpr (kF32) {
+            const int v_lane = anew(l32);
+#pragma unroll
+            for (int j = 0; j < BN / 2; ++j) {  // tokens 8 (j / 4) + 4 half + j % 4
+                const int tok = 8 * (j / 4) + 4 * half + j % 4;
+#pragma unroll
+                for (int t = 0; t < DP / 32; ++t) {
+                    const int d = 32 * t + v_lane;
+                    const float v = ((const float *)tile_v)[4 * (tok * KP + ((d / 4) ^ turn_of<KP>(tok))) + d % 4];
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[j], o[t], 0, 0, 0);
+                }
+            }
+        } else {
+            const int v_lane = anew(lane), l16 = v_lane & 15;
+#pragma unroll
+            for (int j = 0; j < BN / 16; ++j) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = s[8 * j + e];
+                srv_u32x4 w[NP];
+                to_terms<CT, NP>(p, w);
+#pragma unroll
+                for (int t = 0; t < DP / 32; ++t) {
+                    srv_u32x4 v;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {  // four tokens a read, of 16 d a group of 16 lanes
+                        const int tok = 8 * r + 4 * (v_lane >> 5) + l16 / 4, piece = 4 * t + (v_lane >> 4 & 1) * 2 + (l16 >> 1 & 1);
+                        const shortx4 four = read_turned((const shortx4 *)(tile_v + 16 * j * KP + tok * KP + (piece ^ turn_of<KP>(tok))) + (l16 & 1));
+                        const srv_u32x2 two = __builtin_bit_cast(srv_u32x2, four);
+                        v[2 * r] = two[0];
+                        v[2 * r + 1] = two[1];
+                    }
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) o[t] = mma32<CT>(v, w[n], o[t]);
+                }
+            }
+            // the first weights, then each product beside the making of the next and the reads two ahead
+            constexpr int kProducts = BN / 16 * (DP / 32);
+            __builtin_amdgcn_sched_group_barrier(0x002, 28, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+            for (int i = 2; i < kProducts; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NP, 1);
+                __builtin_amdgcn_sched_group_barrier(0x002, 7, 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * NP, 1);
         }
     };
 
     if (begin < end) {
-        uint64_t live = rows_of(begin, block_of(begin));
-        load_tile();
+        copy_tile(lds_k0, lds_v0, lds_live, begin, block_of(begin));
         int next_block = block_of(begin + BN);
-        for (int64_t k0 = begin; k0 < end; k0 += BN) {
-            __syncthreads();  // the last tile was read
-            store_tile(live);
-            const uint64_t live_now = live;
-            __syncthreads();
+        for (int64_t k0 = begin;;) {
+            __syncthreads();  // this tile is there, the one before was read
             if (k0 + BN < end) {
-                live = rows_of(k0 + BN, next_block);
-                load_tile();
+                copy_tile(lds_k1, lds_v1, lds_live + 1, k0 + BN, next_block);
                 next_block = block_of(k0 + 2 * BN);
             }
-            // rows of this wave that see none of the tile, or all of it
-            if (k0 >= high_of(wave_last) || k0 + BN <= low_of(wave_first)) continue;
-            const bool whole = k0 + BN <= high_of(wave_first) && k0 >= low_of(wave_last) && (live_now & (~0ull >> (64 - BN))) == ~0ull >> (64 - BN);
-
-            // ---- scores
-            float s[BN / 2];
-#pragma unroll
-            for (int u = 0; u < BN / 32; ++u) {
-                floatx16 sum;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < kQ; ++c) {
-                    const int tok = 32 * u + l32;
-                    const srv_u32x4 k = lds_k[tok * KP + placed<KP>(tok, 2 * c + half)];
-                    if constexpr (kF32) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[0][c][e]), sum, 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n) sum = mma32<CT>(k, q[n][c], sum);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if constexpr (FORM) {
-                        const float x = sum[i] * to_score;
-                        const int64_t away = pos - (k0 + 32 * u + 8 * (i / 4) + 4 * half + i % 4);
-                        s[16 * u + i] = (inv_cap != 0.0f ? cap_score(x, a.cap, inv_cap) : x) * kLog2E - slope * fabsf((float)away);
-                    } else {
-                        s[16 * u + i] = sum[i] * to_log2;
-                    }
-                }
+            multiply(lds_k0, lds_v0, lds_live[0], k0);
+            if ((k0 += BN) >= end) break;
+            __syncthreads();
+            if (k0 + BN < end) {
+                copy_tile(lds_k0, lds_v0, lds_live, k0 + BN, next_block);
+                next_block = block_of(k0 + 2 * BN);
             }
-            if (!whole) {
-                const int from = (int)max(min(low - k0, (int64_t)BN), (int64_t)0), to = (int)max(min(high - k0, (int64_t)BN), (int64_t)0);
-#pragma unroll
-                for (int i = 0; i < BN / 2; ++i) {
-                    const int t = 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
-                    if (t < from || t >= to || (live_now >> t & 1) == 0) s[i] = -INFINITY;
-                }
-            }
-            // ---- weights
-            float most = s[0];
-#pragma unroll
-            for (int i = 1; i < BN / 2; ++i) most = fmaxf(most, s[i]);
-            most = fmaxf(most, __shfl_xor(most, 32));
-            if (__builtin_amdgcn_ballot_w64(most > m) != 0) {
-                const float m_new = fmaxf(m, most);
-                const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-                m = m_new;
-                l *= f;
-#pragma unroll
-                for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[t][i] *= f;
-            }
-            const float base = (m == -INFINITY ? 0.0f : m) - kUp;
-#pragma unroll
-            for (int i = 0; i < BN / 2; ++i) {
-                s[i] = __builtin_amdgcn_exp2f(s[i] - base);
-                l += s[i];
-            }
-            // ---- values
-            if constexpr (kF32) {
-#pragma unroll
-                for (int j = 0; j < BN / 8; ++j)
-#pragma unroll
-                    for (int t = 0; t < DP / 32; ++t) {
-                        const int d = 32 * t + l32;
-                        const srv_u32x4 v = lds_v[d * VP + placed<VP>(d, 2 * j + half)];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v[i]), s[4 * j + i], o[t], 0, 0, 0);
-                    }
-            } else {
-#pragma unroll
-                for (int j = 0; j < BN / 16; ++j) {
-                    float p[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = s[8 * j + e];
-                    srv_u32x4 w[NP];
-                    to_terms<CT, NP>(p, w);
-#pragma unroll
-                    for (int t = 0; t < DP / 32; ++t) {
-                        const int d = 32 * t + l32;
-                        const srv_u32x4 v = lds_v[d * VP + placed<VP>(d, 2 * j + half)];
-#pragma unroll
-                        for (int n = 0; n < NP; ++n) o[t] = mma32<CT>(v, w[n], o[t]);
-                    }
-                }
-            }
+            multiply(lds_k1, lds_v1, lds_live[1], k0);
+            if ((k0 += BN) >= end) break;
         }
     }
 
