@@ -228,7 +228,8 @@ def decode_program(lanes, cache_t, q_t, lens, heads, kv, dim, block, layout="thd
     out = rows_back(got[bo], batch, heads * dim, os_)
     for r in range(batch - 1):
         assert (got[bo][r * os_ + heads * dim:(r + 1) * os_] == 7).all()
-    weight = 2.0 ** -16 if cache_t == BF16 and q_t == BF16 else 2.0 ** -20
+    # (over a 4-bit cache the weights of 16-bit outputs are rounded to f16)
+    weight = 2.0 ** -16 if cache_t == BF16 and q_t == BF16 else 2.0 ** -11 if cache_t is None and q_t != F32 else 2.0 ** -20
     for r, length in enumerate(lens):
         pos = np.array([length - 1])
         t, k, v, km, vm = cache.of(r, length)

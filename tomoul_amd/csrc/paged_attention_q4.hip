@@ -3,40 +3,52 @@
 //
 // With rows x = n s_g + z_g of nibbles n, step s and minimum z for each group g of 32, and
 // c_g = z_g + 8 s_g,
-//   q . k_t  = sum_g s_tg (q_g . (n_tg - 8)) + c_tg sum(q_g)
+//   q . k_t  = sum_g s_tg (q_g . n_tg) + z_tg sum(q_g)
 //   out_d    = sum_t (p_t s_tg) (n_td - 8) + sum_t p_t c_tg,   g = d / 32
-// so the matrix cores multiply the nibbles as f16 integers, without a conversion: or-ed into
-// the lowest bits of 1024 a nibble is 1024 + n, four bits higher 1024 + 16 n, and a packed
-// addition takes 1032 or 1152 away; a shift, four masks and four additions for the eight of a
-// word.  The steps multiply the sums of a group (keys) or the weights (values), the middles c
-// go beside in fp32.  (The nibbles less 8 and the middles, not the nibbles and the minima:
-// the two sums would cancel each other, and the matrix cores round their sums towards zero.
-// f32 outputs were 5e-5 off that way at 448 tokens, f16 ones 5e-4 at 65536.)
+// so the matrix cores multiply nibbles as f16 numbers, without a conversion.  Keys: a nibble
+// alone is a number with no bits but the lowest, n 2^-24 in bits 0 .. 3, n 2^-20 in bits
+// 4 .. 7: a shift and four masks for the eight of a word.  Values: or-ed into the lowest bits
+// of 1024 it is 1024 + n, four bits higher 1024 + 16 n, and a packed addition takes 1032 or
+// 1152 away.  The steps multiply the sums of a group (keys) or the weights (values), minima
+// and middles go beside in fp32.  (Values less 8 and the middles, not nibbles and minima: the
+// two sums would cancel each other, and the matrix cores round their sums towards zero.  f32
+// outputs were 5e-5 off that way at 448 tokens, f16 ones 5e-4 at 65536; a key's sum is of
+// one group and loses nothing to speak of.)
 //
 // Lane layout, a tile of 32 tokens, two halves h of 16 (as paged_attention.hip):
 //   scores   MFMA h, w: rows tokens 16 h + lane % 16, k the 32 d of group w, columns heads;
 //            the lane's words w of a row follow each other
 //   weights  lane (head, c) holds those of tokens 16 h + 4 c + i, the k of the next product
-//   values   MFMA j: rows d = 16 j + lane % 16, all of group j / 2; the B operand is
-//            p_t s_tg, split into two f16 terms
-// Steps and middles of the tile's tokens pass through LDS, where every lane finds those
-// of its eight tokens.
+//   values   MFMA j: rows d = 16 j + lane % 16, all of group j / 2; the B operand is p_t s_tg
+// Steps and minima or middles of the tile's tokens pass through LDS, where every lane finds
+// those of its eight tokens.  f32 q and weights for f32 outputs are two f16 terms each, q of 16
+// bits is exact in one, and so are the weights rounded once where the output is of 16 bits:
+// that adds to an f16 output about what its own rounding does, to a bf16 one an eighth.
 #include "paged_split.hpp"
 #include "terms.hpp"
 
 namespace tml {
 namespace {
 
+// The eight nibbles of a word: register r holds those r and r + 4, times 2^-24 (r even) or 2^-20.
+__device__ __forceinline__ srv_u32x4 nibbles(uint32_t w) {
+    const uint32_t up = w >> 8;
+    return srv_u32x4{w & 0x000F000Fu, w & 0x00F000F0u, up & 0x000F000Fu, up & 0x00F000F0u};
+}
 // Nibbles at bits 0 (SHIFT 0) or 4 of both halves of a word, less 8, as two f16; SHIFT 4: times 16.
 template <int SHIFT>
-__device__ __forceinline__ uint32_t two_nibbles(uint32_t w) {
+__device__ __forceinline__ uint32_t two_nibbles(uint32_t w, uint32_t thousands) {
     const _Float16 less = SHIFT == 0 ? (_Float16)-1032.0f : (_Float16)-1152.0f;
-    const uint32_t up = (w & (0x000F000Fu << SHIFT)) | 0x64006400u;
+    const uint32_t up = (w & (0x000F000Fu << SHIFT)) | thousands;
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(srv_f16x2, up) + (srv_f16x2){less, less});
 }
-// The eight nibbles of a word: register r holds those r and r + 4, times 1 (r even) or 16.
-__device__ __forceinline__ srv_u32x4 nibbles(uint32_t w) {
-    return srv_u32x4{two_nibbles<0>(w), two_nibbles<4>(w), two_nibbles<0>(w >> 8), two_nibbles<4>(w >> 8)};
+// 1024 in both halves, in a vector register: one instruction masks and ors then.
+__device__ __forceinline__ uint32_t two_thousands() {
+    uint32_t v = 0x64006400u;
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+v"(v));
+#endif
+    return v;
 }
 
 // Two floats in two f16 terms each.
@@ -90,21 +102,27 @@ __device__ __forceinline__ Words<(N + 3) / 4> load_bytes(const char *p) {
     return r;
 }
 
-// G: groups of a head.  ONCE: the cache is read with the streaming policy.
-template <int G, bool ONCE>
-__global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAttentionArgs a, AttnShape sh) {
+// G: groups of a head.  WIDE: q and the output are f32.  FORM: the scores are capped or
+// biased.  ONCE: the cache is read with the streaming policy.
+template <int G, bool WIDE, bool FORM, bool ONCE>
+__global__ __launch_bounds__(kThreads, G > 4 ? 1 : 2) void paged_attention_q4_kernel(PagedAttentionArgs a, AttnShape sh) {
     constexpr int D = 32 * G;
     constexpr int VW = (G + 3) / 4;  // words of a lane's values
-    constexpr float kUp = 14.0f;     // base of the weights' exponent: their terms reach down to 2^-38 of the largest
+    constexpr int NT = WIDE ? 2 : 1;  // terms of q and of the weights
+    // The maximum that weights are relative to may fall behind by kBehind (in powers of two)
+    // before sums are scaled.  kUp: base of the weights' exponent, their terms reach down to
+    // 2^-38 of the largest (f32 outputs) or 2^-23 (and the maximum behind).
+    constexpr float kBehind = WIDE ? 0.0f : 8.0f, kUp = WIDE ? 14.0f : 6.0f;
 
     __shared__ __align__(16) int64_t row_off[kWaves][kTile];
-    __shared__ __align__(16) srv_f32x2 meta[kWaves][2][kTile][G];  // steps and middles, of keys, of values
+    __shared__ __align__(16) srv_f32x2 meta[kWaves][2][kTile][G];  // steps and minima of keys, steps and middles of values
     __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
     TML_DYNAMIC_LDS(floatx4, dyn);
     float *const wave_o = (float *)dyn;  // [wave][head][D]
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
     const int l16 = lane & 15, c4 = lane >> 4;
     const int64_t P = a.block_size;
+    const uint32_t thousands = two_thousands();
 
     ListWalk walk;
     if (!first_list(a.q_type, a, sh, walk)) return;
@@ -119,7 +137,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
         // ---- q as the scores' B operand: lane (head, c) has d = 32 w + 8 c + e, in the nibbles' order.
         // Scaled by a power of two to [2^14, 2^15) at most, and the odd registers by 2^-4.
         const int64_t q_at = b * a.q_stride + (head0 + min(l16, gn - 1)) * D;
-        srv_u32x4 q[2][G];
+        srv_u32x4 q[NT][G];
         float q_sum[G], to_score = a.scale;
         {
             float v[G][8];
@@ -127,7 +145,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
 #pragma unroll
             for (int w = 0; w < G; ++w) {
                 const int64_t at = q_at + 32 * w + 8 * c4;
-                if (a.q_type == TML_TYPE_F32) srv_floats<TML_TYPE_F32>(srv_load8<TML_TYPE_F32>(a.q, at), v[w]);
+                if (WIDE) srv_floats<TML_TYPE_F32>(srv_load8<TML_TYPE_F32>(a.q, at), v[w]);
                 else if (a.q_type == TML_TYPE_F16) srv_floats<TML_TYPE_F16>(srv_load8<TML_TYPE_F16>(a.q, at), v[w]);
                 else srv_floats<TML_TYPE_BF16>(srv_load8<TML_TYPE_BF16>(a.q, at), v[w]);
 #pragma unroll
@@ -138,7 +156,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
             }
             most = max(most, (uint32_t)__shfl_xor((int)most, 16));
             most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-            to_score *= __uint_as_float(most - (14u << 23));
+            to_score *= __uint_as_float(most - (14u << 23)) * 0x1p24f;
             const float up = __uint_as_float((268u << 23) - most);
 #pragma unroll
             for (int w = 0; w < G; ++w) {
@@ -150,22 +168,27 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
                 }
                 sum += __shfl_xor(sum, 16);
                 sum += __shfl_xor(sum, 32);
-                q_sum[w] = sum;
+                q_sum[w] = sum * 0x1p-24f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float f = r % 2 ? 0x1p-4f : 1.0f;
-                    uint32_t first, second;
-                    two_terms(v[w][r] * f, v[w][r + 4] * f, &first, &second);
-                    q[0][w][r] = first;
-                    q[1][w][r] = second;
+                    if constexpr (WIDE) {
+                        uint32_t first, second;
+                        two_terms(v[w][r] * f, v[w][r + 4] * f, &first, &second);
+                        q[0][w][r] = first;
+                        q[1][w][r] = second;
+                    } else {
+                        q[0][w][r] = srv_pack_f16(v[w][r] * f, v[w][r + 4] * f);
+                    }
                 }
             }
         }
         const float to_log2 = to_score * kLog2E;
         float slope = 0.0f, inv_cap = 0.0f;
-        const bool formed = a.slopes != nullptr || a.cap != 0.0f;
-        if (a.slopes != nullptr) slope = a.slopes[head0 + min(l16, gn - 1)] * kLog2E;
-        if (a.cap != 0.0f) inv_cap = 1.0f / a.cap;
+        if constexpr (FORM) {
+            if (a.slopes != nullptr) slope = a.slopes[head0 + min(l16, gn - 1)] * kLog2E;
+            if (a.cap != 0.0f) inv_cap = 1.0f / a.cap;
+        }
 
         float m = -INFINITY, l = 0.0f;  // of this lane's head; l over this lane's tokens alone
         uint32_t peak = 0;              // exponent of the largest step so far, of f32 bits; the weights are in units of it
@@ -219,7 +242,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
             for (int g = 0; g < G; ++g) {
                 const uint32_t d = mine ? marks.w[g] : 0u;
                 const float step = tml_half_bits(d & 0xFFFFu);
-                meta[wave][lane >> 5][lane & 31][g] = srv_f32x2{step, fmaf(step, 8.0f, tml_half_bits(d >> 16))};
+                meta[wave][lane >> 5][lane & 31][g] = srv_f32x2{step, fmaf(step, lane < 32 ? 0.0f : 8.0f, tml_half_bits(d >> 16))};
                 step_most = fmaxf(step_most, step);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -228,27 +251,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
             // ---- scores
             float s[8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int e = 0; e < 8; ++e) s[e] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * h + i] = 0.0f;
+            for (int w = 0; w < G; ++w) {
 #pragma unroll
-                for (int w = 0; w < G; ++w) {
+                for (int h = 0; h < 2; ++h) {
                     const srv_u32x4 n = nibbles(kr[h].w[w]);
                     floatx4 sum = mma16<TML_TYPE_F16>(n, q[0][w], floatx4{0, 0, 0, 0});
-                    sum = mma16<TML_TYPE_F16>(n, q[1][w], sum);
+                    if constexpr (WIDE) sum = mma16<TML_TYPE_F16>(n, q[1][w], sum);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const srv_f32x2 d = meta[wave][0][16 * h + 4 * c4 + i][w];
                         s[4 * h + i] = fmaf(sum[i], d[0], fmaf(q_sum[w], d[1], s[4 * h + i]));
                     }
                 }
+                if (G > 4 && w % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
-            if (formed) {
+            if constexpr (FORM) {
+                const float from = (float)(sp.len - 1 - sp.first - ((int64_t)t * kTile + 4 * c4));
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float x = s[e] * to_score;
-                    const int64_t away = sp.len - 1 - sp.first - ((int64_t)t * kTile + 16 * (e / 4) + 4 * c4 + e % 4);
-                    s[e] = (inv_cap != 0.0f ? cap_score(x, a.cap, inv_cap) : x) * kLog2E - slope * (float)away;
+                    s[e] = fmaf(-slope, from - (float)(16 * (e / 4) + e % 4), (inv_cap != 0.0f ? cap_score(x, a.cap, inv_cap) : x) * kLog2E);
                 }
             } else {
 #pragma unroll
@@ -267,7 +291,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
             for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
-            if (__builtin_amdgcn_ballot_w64(most > m) != 0) {
+            if (__builtin_amdgcn_ballot_w64(most > m + kBehind) != 0) {
                 const float m_new = fmaxf(m, most);
                 const float f = rescale(m, m_new);
                 m = m_new;
@@ -291,21 +315,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
             // (no step yet: all of them are zero)
             const float unit_step = peak == 0u ? 1.0f : __uint_as_float((253u << 23) - peak);  // 2^-1 / the largest's power of two
             const float base = (m == -INFINITY ? 0.0f : m) - kUp;
-            float p[8];
+            float p[8], in_units[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 p[e] = __builtin_amdgcn_exp2f(s[e] - base);
                 l += p[e];
+                in_units[e] = p[e] * unit_step;
             }
-            float step[8][G];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const srv_f32x2 d = meta[wave][1][16 * (e / 4) + 4 * c4 + e % 4][g];
-                    step[e][g] = d[0];
-                    middle[g] = fmaf(p[e], d[1], middle[g]);
-                }
             // ---- values
             srv_u32x4 pair[2 * VW];  // 16 bits of tokens 2 i and 2 i + 1
 #pragma unroll
@@ -314,16 +330,26 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
                 for (int i = 0; i < 4; ++i)
                     pair[x][i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[x / 2], vr[2 * i].w[x / 2], x % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] *= unit_step;
-#pragma unroll
             for (int g = 0; g < G; ++g) {
-                srv_u32x4 w0, w1;
+                float step[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const srv_f32x2 d = meta[wave][1][16 * (e / 4) + 4 * c4 + e % 4][g];
+                    step[e] = d[0];
+                    middle[g] = fmaf(p[e], d[1], middle[g]);
+                }
+                srv_u32x4 weight[NT];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    uint32_t first, second;
-                    two_terms(p[2 * i] * step[2 * i][g], p[2 * i + 1] * step[2 * i + 1][g], &first, &second);
-                    w0[i] = first;
-                    w1[i] = second;
+                    const float x = in_units[2 * i] * step[2 * i], y = in_units[2 * i + 1] * step[2 * i + 1];
+                    if constexpr (WIDE) {
+                        uint32_t first, second;
+                        two_terms(x, y, &first, &second);
+                        weight[0][i] = first;
+                        weight[1][i] = second;
+                    } else {
+                        weight[0][i] = srv_pack_f16(x, y);
+                    }
                 }
 #pragma unroll
                 for (int j = 2 * g; j < 2 * g + 2; ++j) {
@@ -331,11 +357,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q4_kernel(PagedAt
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t two = j % 4 >= 2 ? pair[j / 4][i] >> 8 : pair[j / 4][i];
-                        n[i] = j % 2 ? two_nibbles<4>(two) : two_nibbles<0>(two);
+                        n[i] = j % 2 ? two_nibbles<4>(two, thousands) : two_nibbles<0>(two, thousands);
                     }
-                    o[j] = mma16<TML_TYPE_F16>(n, w0, o[j]);
-                    o[j] = mma16<TML_TYPE_F16>(n, w1, o[j]);
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) o[j] = mma16<TML_TYPE_F16>(n, weight[x], o[j]);
                 }
+                if (G > 4 && g % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (else registers run out)
             }
             load_v();
         }
@@ -372,13 +399,19 @@ Status launch_join(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t
 constexpr int kPerCu = 2;  // workgroups
 constexpr int64_t kLastLevel = (int64_t)256 << 20;  // a cache past it is read with the streaming policy
 
-template <int G>
-void launch_groups(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
+template <int G, bool WIDE, bool FORM>
+void launch_kernel(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
     const size_t lds = (size_t)kWaves * sh.heads * 32 * G * 4;
     const dim3 grid(1u << sh.grid_log2), block(kThreads);
     const double bytes = 40.0 * G * a.n_blocks * a.block_size * a.kv_heads;
-    if (bytes > kLastLevel) paged_attention_q4_kernel<G, true><<<grid, block, lds, s>>>(a, sh);
-    else paged_attention_q4_kernel<G, false><<<grid, block, lds, s>>>(a, sh);
+    if (bytes > kLastLevel) paged_attention_q4_kernel<G, WIDE, FORM, true><<<grid, block, lds, s>>>(a, sh);
+    else paged_attention_q4_kernel<G, WIDE, FORM, false><<<grid, block, lds, s>>>(a, sh);
+}
+template <int G>
+void launch_groups(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
+    const bool form = a.cap != 0.0f || a.slopes != nullptr;
+    if (a.q_type == TML_TYPE_F32) form ? launch_kernel<G, true, true>(a, sh, s) : launch_kernel<G, true, false>(a, sh, s);
+    else form ? launch_kernel<G, false, true>(a, sh, s) : launch_kernel<G, false, false>(a, sh, s);
 }
 
 }  // namespace
