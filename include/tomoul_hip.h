@@ -490,7 +490,8 @@ int tml_hip_paged_attention_ex_dev(int q_type, int cache_type, int64_t batch, in
  * in an encoder.  The scores are
  *   s_t = cap * tanh(scale * q . k_t / cap) - slopes[h] * |pos - t|
  * with cap and slopes as in tml_hip_paged_attention_ex_dev; a token that sees nothing gets
- * zeros, and what lies in other positions, NaN among it, is not looked at.
+ * zeros, and what lies in other positions, NaN among it, is not looked at.  An infinite
+ * value makes its element infinite or NaN in the outputs of those who see it.
  *   tokens       rows of q and out; those at query_start[requests] and after are left as they
  *                were.  Starts and lengths that do not fit (negative, past tokens, past the
  *                table) count as the nearest that do

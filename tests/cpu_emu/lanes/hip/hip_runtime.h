@@ -40,6 +40,8 @@
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 tml_emu_plain_mfma_bf16_32
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16 tml_emu_plain_mfma_f16_32
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16 tml_emu_plain_read_tr
+#define __builtin_amdgcn_s_barrier tml_emu_plain_s_barrier
+#define __builtin_amdgcn_permlane32_swap tml_emu_plain_permlane32_swap
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8 tml_emu_plain_mfma_i8
 #define tml_emu_launcher tml_emu_plain_launcher
 #define tml_emu_launch tml_emu_plain_launch
@@ -62,6 +64,8 @@
 #undef __builtin_amdgcn_mfma_f32_32x32x16_bf16
 #undef __builtin_amdgcn_mfma_f32_32x32x16_f16
 #undef __builtin_amdgcn_ds_read_tr16_b64_v4i16
+#undef __builtin_amdgcn_s_barrier
+#undef __builtin_amdgcn_permlane32_swap
 #undef __builtin_amdgcn_mfma_i32_16x16x64_i8
 #undef tml_emu_launcher
 #undef tml_emu_launch
@@ -111,6 +115,7 @@ tml_lane_launcher<P...> tml_emu_launch(void (*k)(P...), dim3 g, dim3 b, size_t s
 #define TML_LANE_OP __attribute__((noinline, noduplicate))
 
 inline void __syncthreads() { tml_lane_block_barrier(); }
+inline void __builtin_amdgcn_s_barrier() { tml_lane_block_barrier(); }
 
 template <typename T>
 inline T tml_lane_from(const tml_lane_meeting &m, unsigned lane) {
@@ -242,4 +247,13 @@ TML_LANE_OP inline tml_emu_s16x4 __builtin_amdgcn_ds_read_tr16_b64_v4i16(__attri
         out[j] = four[lane % 4];
     }
     return out;
+}
+// The upper half of the first and the lower half of the second change places.
+TML_LANE_OP inline tml_emu_u32x2_swap __builtin_amdgcn_permlane32_swap(unsigned a, unsigned b, bool, bool) {
+    const unsigned mine[2] = {a, b};
+    const tml_lane_meeting &m = tml_lane_meet(__builtin_return_address(0), mine, sizeof mine);
+    const unsigned lane = tml_emu_lane();
+    unsigned other[2];
+    std::memcpy(other, m.data[lane ^ 32], sizeof other);
+    return lane < 32 ? tml_emu_u32x2_swap{a, other[0]} : tml_emu_u32x2_swap{other[1], b};
 }

@@ -198,6 +198,14 @@ class Cache:
             self.values.append(val)
             self.mags.append(mag)
 
+    def put(self, odd):
+        """(request, position, key or value (0, 1), head, d, number) into a cache of floats."""
+        for r, pos, w, h, d, x in odd:
+            page, at = self.table[r, pos // self.block], pos % self.block
+            self.values[w][page, at, h, d] = x
+            b, tk, hd = self.strides
+            self.bytes[w][page * b + at * tk + h * hd + d] = stored(np.array([x]), self.t)[0]
+
     def of(self, r, length):
         """Positions of request r that are in the cache, their keys and values, and magnitudes."""
         t = np.arange(length)
@@ -269,11 +277,12 @@ def test_attention_ex(lanes, q_t, cache_t, case):
 
 # ------------------------------------------------------------------ prompts
 def prompt_program(lanes, q_t, cache_t, both, heads, kv, dim, block, layout="thd", prefix=None, window=0, cap=0.0, slopes=False, pad=2, lost=(), seed=0,
-                   reverse=False, edit=None):
+                   reverse=False, odd=()):
     """both: (context, new tokens) of each request."""
     rng = np.random.default_rng(seed)
     lens = [c + n for c, n in both]
     cache = Cache(rng, cache_t, lens, kv, dim, block, layout, 0, lost)
+    cache.put(odd)
     starts = np.concatenate([[0], np.cumsum([n for _, n in both])]).astype(np.int32)
     tokens = int(starts[-1]) + pad
     q = stored(1.5 * rng.standard_normal((tokens, heads * dim)), q_t)
@@ -304,6 +313,7 @@ def prompt_program(lanes, q_t, cache_t, both, heads, kv, dim, block, layout="thd
         want, tol = ref.attention(values(q[starts[r]:starts[r + 1]], q_t).reshape(n, heads, dim), k, v, pos, scale=scale, cap=cap, slopes=sl,
                                   seen=ref.sees(pos, t, prefix[r] if prefix else 0, window), positions=t, weight=weight)
         mine = values(out[starts[r]:starts[r + 1]], q_t).reshape(want.shape)
+        mine = np.where(np.isinf(want) & ~np.isfinite(mine), want, mine)  # (an infinite value's element is infinite or NaN)
         close(mine, want, tol + HALF_ULP[q_t] * (np.abs(want) + tol) + TINY[q_t], f"request {r}")
 
 
@@ -329,6 +339,18 @@ def test_prompt_attention_shapes(lanes, case):
     prompt_program(lanes, F16, F16, dim=64, seed=3, **case)
     prompt_program(lanes, F32, BF16, dim=40, seed=4, reverse=True, **case)
     prompt_program(lanes, F32, F32, dim=64, seed=5, **case)
+
+
+ODD = [(0, 100, 1, 0, 3, np.inf), (0, 120, 1, 0, 3, -np.inf), (0, 130, 1, 1, 70 % 40, np.nan), (0, 90, 1, 0, 0, -np.inf), (0, 140, 0, 0, 5, np.nan),
+       (0, 64, 0, 1, 2, np.inf), (0, 149, 1, 1, 1, np.inf)]
+
+
+@pytest.mark.parametrize("q_t,cache_t", COMBOS, ids=tname)
+def test_prompt_attention_infinities_and_nan_are_for_those_who_see_them(lanes, q_t, cache_t):
+    # an infinity or a NaN of a later (or of a left) position reaches no one else
+    odd = [o for o in ODD if o[2] == 1 or np.isnan(o[5]) or q_t == cache_t]
+    prompt_program(lanes, q_t, cache_t, [(60, 90)], 4, 2, 40, 16, odd=odd, seed=7)
+    prompt_program(lanes, q_t, cache_t, [(60, 90)], 2, 2, 40, 16, odd=odd, window=30, prefix=[110], seed=8)
 
 
 @pytest.mark.parametrize("starts,lens", [([0, 100, 5], [9, 9]), ([-3, 4, 4], [9, 30000]), ([5, 2, 7], [-4, 3]), ([0, 7, 0x7FFFFFFF], [9, 0x7FFFFFFF]),

@@ -20,7 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, HERE)
 import serving_ref as ref  # noqa: E402
 from serving_ref import BF16, F16, F32, HALF_ULP, STORED, TINY, close, stored, tname, values  # noqa: E402
-from test_cpu_serving_more import COMBOS, Cache, check_logprobs, pool_index, pool_strides, rows_back, rows_of, wild  # noqa: E402
+from test_cpu_serving_more import COMBOS, ODD, Cache, check_logprobs, pool_index, pool_strides, rows_back, rows_of, wild  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -140,10 +140,11 @@ def test_attention_ex(q_t, cache_t, dim):
 
 
 # ------------------------------------------------------------------ prompts
-def prompt(q_t, cache_t, both, heads, kv, dim, block, layout="thd", prefix=None, window=0, cap=0.0, slopes=False, pad=2, lost=(), seed=0):
+def prompt(q_t, cache_t, both, heads, kv, dim, block, layout="thd", prefix=None, window=0, cap=0.0, slopes=False, pad=2, lost=(), seed=0, odd=()):
     rng = np.random.default_rng(seed)
     lens = [c + n for c, n in both]
     cache = Cache(rng, cache_t, lens, kv, dim, block, layout, 0, lost)
+    cache.put(odd)
     starts = np.concatenate([[0], np.cumsum([n for _, n in both])]).astype(np.int32)
     tokens, scale = int(starts[-1]) + pad, float(np.float32(1 / np.sqrt(dim)))
     q = stored(1.5 * rng.standard_normal((tokens, heads * dim)), q_t)
@@ -171,6 +172,7 @@ def prompt(q_t, cache_t, both, heads, kv, dim, block, layout="thd", prefix=None,
         want, tol = ref.attention(values(q[starts[r]:starts[r + 1]], q_t).reshape(n, heads, dim), k, v, pos, scale=scale, cap=cap, slopes=sl,
                                   seen=ref.sees(pos, t, prefix[r] if prefix else 0, window), positions=t, weight=weight)
         mine = values(out[starts[r]:starts[r + 1]], q_t).reshape(want.shape)
+        mine = np.where(np.isinf(want) & ~np.isfinite(mine), want, mine)  # (an infinite value's element is infinite or NaN)
         close(mine, want, tol + HALF_ULP[q_t] * (np.abs(want) + tol) + TINY[q_t], f"request {r}")
 
 
@@ -196,6 +198,14 @@ def test_prompt_attention_shapes(case):
     prompt(BF16, BF16, dim=128, seed=3, **case)
     prompt(F32, BF16, dim=40, seed=4, **case)
     prompt(F32, F32, dim=64, seed=5, **case)
+
+
+@pytest.mark.parametrize("q_t,cache_t", COMBOS, ids=tname)
+def test_prompt_attention_infinities_and_nan_are_for_those_who_see_them(q_t, cache_t):
+    odd = [o for o in ODD if o[2] == 1 or np.isnan(o[5]) or q_t == cache_t]
+    for dim in (40, 64, 128, 256):
+        prompt(q_t, cache_t, [(60, 90)], 4, 2, dim, 16, odd=odd, seed=7)
+        prompt(q_t, cache_t, [(60, 90)], 2, 2, dim, 16, odd=odd, window=30, prefix=[110], seed=8)
 
 
 # ----------------------------------------------------------------- logprobs

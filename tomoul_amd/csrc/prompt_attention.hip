@@ -39,7 +39,7 @@ namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kWaves = 4;           // of a team: 32 rows each
 constexpr int kRows = 32 * kWaves;  // of a workgroup
 
 struct PromptShape {
@@ -75,6 +75,12 @@ __device__ __forceinline__ int anew(int v) {
     asm volatile("" : "+v"(v));
 #endif
     return v;
+}
+
+// The larger of a lane's and the lane's 32 away.
+__device__ __forceinline__ float max_of_halves(float v) {
+    const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
 }
 
 // New tokens of request r: their first row of q, and how many (not past q's end).
@@ -117,11 +123,66 @@ struct Prompt {
     static constexpr int kQ = kF32 ? DP / 8 : DP / 16;       // 16 bytes of q a lane, each term
     // registers of a lane: q, output, scores and weights; two workgroups a CU where they leave room
     static constexpr int kRegs = 4 * kQ * NQ + DP / 2 + BN / 2 + BN / 4 * NP;
-    static constexpr int kPerCu = kRegs > 180 ? 1 : 2;
+    static constexpr bool kTwo = kRegs <= 160;               // two waves of a SIMD
+    static constexpr int kTile = BN * KP;                    // pieces of a tile's keys
 };
 
-template <int CT, int QT, int DP, bool FORM>
-__global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void prompt_attention_kernel(PromptAttentionArgs a, PromptShape sh) {
+// Until at most N of this wave's copies are under way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | 0x7 << 4 | 0xF << 8);
+}
+
+// One row by a wave, in fp32 from end to end: a lane a token for the scores, a lane a d for the
+// values.  For the few rows beside which values are infinite or NaN where they may not look.
+template <int CT, int QT>
+__device__ __forceinline__ void one_row(const PromptAttentionArgs &a, const PromptShape &sh, int64_t b, int64_t len, int64_t q_row, int64_t head, int64_t pos,
+                                                  int64_t prefix, int64_t kv) {
+    const int lane = threadIdx.x & 63, D = (int)a.head_dim;
+    const int64_t low = a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0, high = min(max(pos + 1, prefix), len);
+    const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
+    auto row_of = [&](int64_t t) {  // element of the caches, or -1
+        const int block = a.block_table[b * a.table_stride + (uint32_t)t / (uint32_t)a.block_size];
+        if (block < 0 || block >= a.n_blocks) return (int64_t)-1;
+        return block * a.block_stride + (int64_t)((uint32_t)t % (uint32_t)a.block_size) * a.token_stride + kv * a.head_stride;
+    };
+    auto score_of = [&](int64_t t, int64_t off) {
+        float x = 0.0f;
+        for (int d = 0; d < D; ++d) x = fmaf(srv_load1(QT, a.q, q_row * a.q_stride + head * D + d), srv_load1(CT, a.k_cache, off + d), x);
+        x *= a.scale;
+        if (a.cap != 0.0f) x = cap_score(x, a.cap, 1.0f / a.cap);
+        return (x - slope * fabsf((float)(pos - t))) * kLog2E;
+    };
+    float m = -INFINITY;
+    for (int64_t t = low + lane; t < high; t += 64) {
+        const int64_t off = row_of(t);
+        if (off >= 0) m = fmaxf(m, score_of(t, off));
+    }
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (m == -INFINITY) m = 0.0f;
+    float l = 0.0f, out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t t0 = low; t0 < high; t0 += 64) {
+        const int64_t t = t0 + lane, off = t < high ? row_of(t) : -1;
+        const float p = off >= 0 ? __builtin_amdgcn_exp2f(score_of(t, off) - m) : 0.0f;
+        l += p;
+        for (int j = 0; j < 64 && t0 + j < high; ++j) {
+            const float w = __shfl(p, j);
+            const int64_t from = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(off >> 32), j) << 32) | (uint32_t)__shfl((int)(uint32_t)off, j));
+            if (from < 0 || w == 0.0f) continue;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (lane + 64 * x < D) out[x] = fmaf(w, srv_load1(CT, a.v_cache, from + lane + 64 * x), out[x]);
+        }
+    }
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+        if (lane + 64 * x < D) srv_store1(QT, a.out, q_row * a.out_stride + head * D + lane + 64 * x, l == 0.0f ? 0.0f : out[x] / l);
+}
+
+// TEAMS: of four waves with the same rows each, which share the tiles.
+template <int CT, int QT, int DP, bool FORM, int TEAMS>
+__global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTwo && TEAMS == 1 ? 2 : 1)) void prompt_attention_kernel(PromptAttentionArgs a, PromptShape sh) {
     using C = Prompt<CT, QT, DP, FORM>;
     constexpr bool kF32 = C::kF32;
     constexpr int kBytes = C::kBytes, NQ = C::NQ, NP = C::NP, BN = C::BN, KP = C::KP, kQ = C::kQ, kOwn = C::kOwn;
@@ -133,10 +194,11 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
     constexpr float kUp = CT != TML_TYPE_F16 ? 0.0f : QT == TML_TYPE_F32 ? 14.0f : 7.0f;
 
     // (arrays of their own: the compiler waits for copies to the array that it reads)
-    __shared__ srv_u32x4 lds_k0[BN * KP], lds_k1[BN * KP], lds_v0[BN * KP], lds_v1[BN * KP];
-    __shared__ RowAt row_at[kWaves][kOwn];
-    __shared__ uint64_t lds_live[2];  // of a tile's tokens
-    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    __shared__ srv_u32x4 lds_k0[TEAMS * C::kTile], lds_k1[TEAMS * C::kTile], lds_v0[TEAMS * C::kTile], lds_v1[TEAMS * C::kTile];
+    __shared__ RowAt row_at[2][TEAMS * kWaves][kOwn];
+    __shared__ uint64_t lds_live[2][TEAMS];  // of a tile's tokens
+    __shared__ int lds_odd;                  // infinities or NaNs were found where not all rows see them
+    const int lane = threadIdx.x & 63, any_wave = uniform((int)(threadIdx.x >> 6)), wave = any_wave % kWaves, team = any_wave / kWaves;
     const int l32 = lane & 31, half = lane >> 5;
     const int D = (int)a.head_dim;
     const int64_t P = a.block_size;
@@ -259,44 +321,66 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
 
-    // ---- copies: a wave's tokens are its share of the tile, lane % kOwn looks one up
-    auto block_of = [&](int64_t k0) {
-        const int64_t tok = k0 + wave * kOwn + lane % kOwn;
+    const char *const zeros_at = (const char *)zero_row;
+    // ---- the team's tile `it` is tokens tile_at(it) and on
+    const int steps = (int)((max(end - begin, (int64_t)0) + BN * TEAMS - 1) / (BN * TEAMS));
+    auto tile_at = [&](int it) { return begin + (int64_t)(TEAMS * it + team) * BN; };
+    // copies: a wave's tokens are its share of the tile, lane % kOwn looks one up
+    auto block_of = [&](int it) {
+        const int64_t tok = tile_at(it) + wave * kOwn + lane % kOwn;
         return a.block_table[b * a.table_stride + (uint32_t)min(tok, len - 1) / (uint32_t)P];
     };
-    auto copy_tile = [&](srv_u32x4 *to_k, srv_u32x4 *to_v, uint64_t *to_live, int64_t k0, int in_block) {
-        const int64_t tok = k0 + wave * kOwn + lane % kOwn;
+    auto find_rows = [&](int it, int in_block) __attribute__((always_inline)) {
+        const int64_t tok = tile_at(it) + wave * kOwn + lane % kOwn;
         const bool live = tok < end && in_block >= 0 && in_block < a.n_blocks;
         const int64_t off = (in_block * a.block_stride + (int64_t)((uint32_t)tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes;
-        row_at[wave][lane % kOwn] = live ? RowAt{(const char *)a.k_cache + off, (const char *)a.v_cache + off} : RowAt{(const char *)zero_row, (const char *)zero_row};
+        row_at[it & 1][any_wave][lane % kOwn] =
+            live ? RowAt{(const char *)a.k_cache + off, (const char *)a.v_cache + off} : RowAt{zeros_at, zeros_at};
         const uint64_t all = __builtin_amdgcn_ballot_w64(live);
         if (lane == 0) {
-            if constexpr (kOwn == 16) ((uint16_t *)to_live)[wave] = (uint16_t)all;
-            else ((uint8_t *)to_live)[wave] = (uint8_t)all;
+            if constexpr (kOwn == 16) ((uint16_t *)&lds_live[it & 1][team])[wave] = (uint16_t)all;
+            else ((uint8_t *)&lds_live[it & 1][team])[wave] = (uint8_t)all;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const int copier = anew(lane);
+    };
+    // Copy i is of 64 / KP tokens, a lane a piece: the turn of a token's number is that of its bits
+    // one by one, so the pieces of copy i are those of copy 0 turned on.
+    constexpr int kAtOnce = 64 / KP;
+    const uint32_t first_piece = ((uint32_t)lane % KP ^ turn_of<KP>((uint32_t)lane / KP)) * 16;
+    struct Sources {
+        const char *at[C::kCopies];
+    };
+    auto sources_of = [&](const RowAt (&rows_here)[kOwn], bool values) __attribute__((always_inline)) {
+        Sources from;
 #pragma unroll
         for (int i = 0; i < C::kCopies; ++i) {
-            const int at = i * 64 + copier, t = at / KP, piece = (at % KP) ^ turn_of<KP>(wave * kOwn + t);
-            const RowAt row_here = row_at[wave][t];
-            const char *from_k = row_here.k + 16 * piece, *from_v = row_here.v + 16 * piece;
-            if (D < DP && piece * (16 / kBytes) >= D) from_k = from_v = (const char *)(zero_row + piece);
-            __builtin_amdgcn_global_load_lds(TML_GPTR(from_k), TML_LPTR(to_k + wave * kOwn * KP + i * 64), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(TML_GPTR(from_v), TML_LPTR(to_v + wave * kOwn * KP + i * 64), 16, 0, 0);
+            const RowAt &row_here = rows_here[i * kAtOnce + (uint32_t)lane / KP];
+            from.at[i] = values ? row_here.v : row_here.k;
+        }
+        return from;
+    };
+    auto copy_rows = [&](srv_u32x4 *to, const Sources &from) __attribute__((always_inline)) {
+        const uint32_t here = (uint32_t)anew((int)first_piece);
+#pragma unroll
+        for (int i = 0; i < C::kCopies; ++i) {
+            const uint32_t turned = (uint32_t)turn_of<KP>(wave * kOwn + i * kAtOnce) * 16;
+            const char *const piece = D == DP || (int)(first_piece ^ turned) < D * kBytes ? from.at[i] + (here ^ turned) : zeros_at;
+            __builtin_amdgcn_global_load_lds(TML_GPTR(piece), TML_LPTR(to + any_wave * kOwn * KP + i * 64), 16, 0, 0);
         }
     };
 
-    // ---- a tile
-    auto multiply = [&](const srv_u32x4 *tile_k, const srv_u32x4 *tile_v, uint64_t live, int64_t k0) {
-        // rows of this wave that see none of the tile, or all of it
-        if (k0 >= high_of(wave_last) || k0 + BN <= low_of(wave_first)) return;
-        const bool whole = k0 + BN <= high_of(wave_first) && k0 >= low_of(wave_last) && (live & (~0ull >> (64 - BN))) == ~0ull >> (64 - BN);
+    float s[BN / 2];  // scores, then weights
+    srv_u32x4 weights[kF32 ? 1 : BN / 16][NP];
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i) s[i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < (kF32 ? 1 : BN / 16); ++j)
+#pragma unroll
+        for (int n = 0; n < NP; ++n) weights[j][n] = srv_u32x4{0, 0, 0, 0};
 
-        // scores, before the scale (FORM: as powers of two)
-        float s[BN / 2];
-        floatx16 sum[BN / 32];
+    // ---- scores of a tile, before the scale
+    auto multiply_keys = [&](const srv_u32x4 *tile_k, floatx16 (&sum)[BN / 32]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u)
 #pragma unroll
@@ -306,7 +390,7 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
         for (int c = 0; c < kQ; ++c)
 #pragma unroll
             for (int u = 0; u < BN / 32; ++u) {
-                const srv_u32x4 k = tile_k[32 * u * KP + k_row * KP + ((2 * c + half) ^ turn_of<KP>(k_row))];
+                const srv_u32x4 k = tile_k[team * C::kTile + (32 * u + k_row) * KP + ((2 * c + half) ^ turn_of<KP>(k_row))];
                 if constexpr (kF32) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[0][c][e]), sum[u], 0, 0, 0);
@@ -315,18 +399,74 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
                     for (int n = 0; n < NQ; ++n) sum[u] = mma32<CT>(k, q[n][c], sum[u]);
                 }
             }
+    };
+    auto take_scores = [&](const floatx16 (&sum)[BN / 32]) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < BN / 2; ++i) s[i] = sum[i / 16][i % 16];
-        if constexpr (!kF32) {  // reads four ahead of the products
-            constexpr int kReads = kQ * (BN / 32);
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    };
+    // Values: eight tokens of 16 j and on of this lane's d of 32 t and on (f32: the one of token j).
+    // (few steps from the array on: through a longer way the compiler loses which array is read,
+    // and waits for the copies to all)
+    struct Places {
+        int lane;
+        uint32_t at[DP / 32][2];  // bytes, of the first 16 tokens' two fours
+    };
+    auto places = [&]() __attribute__((always_inline)) {
+        Places p;
+        const int v_lane = p.lane = anew(lane);
 #pragma unroll
-            for (int i = 4; i < kReads; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                // four tokens a read, of 16 d a group of 16 lanes
+                const int tok = 8 * r + 4 * (v_lane >> 5) + (v_lane & 15) / 4, piece = 4 * t + (v_lane >> 4 & 1) * 2 + (v_lane >> 1 & 1);
+                p.at[t][r] = (uint32_t)((team * C::kTile + tok * KP + (piece ^ turn_of<KP>(tok))) * 16 + 8 * (v_lane & 1));
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, 4 * NQ, 0);
+        return p;
+    };
+    auto value_at = [&](const srv_u32x4 *tile_v, const Places &p, int j, int t) __attribute__((always_inline)) {
+        if constexpr (kF32) {
+            const int tok = 8 * (j / 4) + 4 * (p.lane >> 5) + j % 4, d = 32 * t + (p.lane & 31);
+            return ((const float *)tile_v)[4 * (team * C::kTile + tok * KP + ((d / 4) ^ turn_of<KP>(tok))) + d % 4];
+        } else {
+            srv_u32x4 v;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const shortx4 four = read_turned((const shortx4 *)((const char *)tile_v + p.at[t][r]) + 32 * j * KP);
+                const srv_u32x2 two = __builtin_bit_cast(srv_u32x2, four);
+                v[2 * r] = two[0];
+                v[2 * r + 1] = two[1];
+            }
+            return v;
         }
+    };
+    constexpr int kJ = kF32 ? BN / 2 : BN / 16;
+    auto multiply_value = [&](auto v, int j, floatx16 sum) __attribute__((always_inline)) {
+        if constexpr (kF32) {
+            return __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[j], sum, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) sum = mma32<CT>(v, weights[j][n], sum);
+            return sum;
+        }
+    };
+    auto multiply_values = [&](const srv_u32x4 *tile_v) __attribute__((always_inline)) {
+        const Places p = places();
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) o[t] = multiply_value(value_at(tile_v, p, j, t), j, o[t]);
+    };
+    struct Moved {
+        bool any;
+        float by, unit;  // what the output is multiplied with; of the scores
+    };
+    // ---- weights of tile `it`
+    // (the maximum moves, and the output waits for that until the products under way are in it)
+    auto new_maximum = [&](int it) __attribute__((always_inline)) {
+        const int64_t k0 = tile_at(it);
+        const uint64_t live = lds_live[it & 1][team];
+        const bool whole = k0 + BN <= high_of(wave_first) && k0 >= low_of(wave_last) && (live & (~0ull >> (64 - BN))) == ~0ull >> (64 - BN);
         if constexpr (FORM) {
             if (inv_cap != 0.0f) {
 #pragma unroll
@@ -359,100 +499,164 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
                 if (t < from || t >= to || (there[i / 16] >> t % 32 & 1) == 0) s[i] = -INFINITY;
             }
         }
-        // weights
         float most = s[0];
 #pragma unroll
         for (int i = 1; i < BN / 2; ++i) most = fmaxf(most, s[i]);
-        most = fmaxf(most, __shfl_xor(most, 32)) * unit;
-        if (__builtin_amdgcn_ballot_w64(most > m + kBehind) != 0) {
-            const float m_new = fmaxf(m, most);
-            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            m = m_new;
-            l *= f;
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] *= f;
-        }
+        most = max_of_halves(most) * unit;
+        const bool moves = __builtin_amdgcn_ballot_w64(most > m + kBehind) != 0;
+        const float m_new = moves ? fmaxf(m, most) : m, f = m == m_new || m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        l *= f;
+        return Moved{moves, f, unit};
+    };
+    auto new_weights = [&](float unit, srv_u32x4 (&to)[kF32 ? 1 : BN / 16][NP]) __attribute__((always_inline)) {
         const float base = kUp - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
         for (int i = 0; i < BN / 2; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], unit, base));
             l += s[i];
         }
-        // values
-        if constexpr (kF32) {
-            const int v_lane = anew(l32);
-#pragma unroll
-            for (int j = 0; j < BN / 2; ++j) {  // tokens 8 (j / 4) + 4 half + j % 4
-                const int tok = 8 * (j / 4) + 4 * half + j % 4;
-#pragma unroll
-                for (int t = 0; t < DP / 32; ++t) {
-                    const int d = 32 * t + v_lane;
-                    const float v = ((const float *)tile_v)[4 * (tok * KP + ((d / 4) ^ turn_of<KP>(tok))) + d % 4];
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[j], o[t], 0, 0, 0);
-                }
-            }
-        } else {
-            const int v_lane = anew(lane), l16 = v_lane & 15;
+        if constexpr (!kF32) {
 #pragma unroll
             for (int j = 0; j < BN / 16; ++j) {
                 float p[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) p[e] = s[8 * j + e];
-                srv_u32x4 w[NP];
-                to_terms<CT, NP>(p, w);
-#pragma unroll
-                for (int t = 0; t < DP / 32; ++t) {
-                    srv_u32x4 v;
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {  // four tokens a read, of 16 d a group of 16 lanes
-                        const int tok = 8 * r + 4 * (v_lane >> 5) + l16 / 4, piece = 4 * t + (v_lane >> 4 & 1) * 2 + (l16 >> 1 & 1);
-                        const shortx4 four = read_turned((const shortx4 *)(tile_v + 16 * j * KP + tok * KP + (piece ^ turn_of<KP>(tok))) + (l16 & 1));
-                        const srv_u32x2 two = __builtin_bit_cast(srv_u32x2, four);
-                        v[2 * r] = two[0];
-                        v[2 * r + 1] = two[1];
-                    }
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) o[t] = mma32<CT>(v, w[n], o[t]);
-                }
+                to_terms<CT, NP>(p, to[j]);
             }
-            // the first weights, then each product beside the making of the next and the reads two ahead
-            constexpr int kProducts = BN / 16 * (DP / 32);
-            __builtin_amdgcn_sched_group_barrier(0x002, 28, 1);
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
-#pragma unroll
-            for (int i = 2; i < kProducts; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, NP, 1);
-                __builtin_amdgcn_sched_group_barrier(0x002, 7, 1);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, 2 * NP, 1);
         }
     };
 
-    if (begin < end) {
-        copy_tile(lds_k0, lds_v0, lds_live, begin, block_of(begin));
-        int next_block = block_of(begin + BN);
-        for (int64_t k0 = begin;;) {
-            __syncthreads();  // this tile is there, the one before was read
-            if (k0 + BN < end) {
-                copy_tile(lds_k1, lds_v1, lds_live + 1, k0 + BN, next_block);
-                next_block = block_of(k0 + 2 * BN);
-            }
-            multiply(lds_k0, lds_v0, lds_live[0], k0);
-            if ((k0 += BN) >= end) break;
-            __syncthreads();
-            if (k0 + BN < end) {
-                copy_tile(lds_k0, lds_v0, lds_live, k0 + BN, next_block);
-                next_block = block_of(k0 + 2 * BN);
-            }
-            multiply(lds_k1, lds_v1, lds_live[1], k0);
-            if ((k0 += BN) >= end) break;
+    // What some rows of the workgroup do not see of a tile weighs nothing for them, but zero times
+    // an infinity or a NaN is a NaN: where such a tile's values hold one, the rows are done again
+    // in the end, one by one.  A wave looks through the tokens that it copied.
+    auto look_for_odd = [&](const srv_u32x4 *tile_v, int it) __attribute__((always_inline)) {
+        const int64_t k0 = tile_at(it);
+        if (min(k0 + BN, end) <= high_of(block_first) && k0 >= low_of(block_last)) return;
+        constexpr uint32_t kExponent = kF32 ? 0x7F800000u : CT == TML_TYPE_F16 ? 0x7C00u : 0x7F80u;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < C::kCopies; ++i) {
+            const srv_u32x4 v = tile_v[any_wave * kOwn * KP + i * 64 + lane];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) odd |= (v[x] & kExponent) == kExponent || (!kF32 && (v[x] >> 16 & kExponent) == kExponent);
         }
+        if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) lds_odd = 1;
+    };
+
+    // ---- A turn a tile: the scores' product, then the weights beside the product of the tile
+    // before.  Keys are copied one tile ahead, values with their weights' turn.
+    if (steps > 0) {
+        // (the first turn multiplies the values of lds_v1 by no weights)
+#pragma unroll 1
+        for (int i = threadIdx.x; i < TEAMS * C::kTile; i += 64 * kWaves * TEAMS) lds_v1[i] = srv_u32x4{0, 0, 0, 0};
+        if (threadIdx.x == 0) lds_odd = 0;
+        find_rows(0, block_of(0));
+        copy_rows(lds_k0, sources_of(row_at[0][any_wave], false));
+        int next_block = block_of(1);
+        auto turn = [&](int it, srv_u32x4 *k_now, srv_u32x4 *k_next, srv_u32x4 *v_now, srv_u32x4 *v_before) __attribute__((always_inline)) {
+            // (no branch around the copies, or a wait for one would be a wait for all: past the last tile
+            // they copy zeros)
+            const Sources values = sources_of(row_at[it & 1][any_wave], true);
+            wait_copies<0>();
+            __syncthreads();  // this tile's keys and the values before are there, the tile before was read
+            look_for_odd(v_before, it - 1);
+            find_rows(it + 1, next_block);
+            const Sources keys = sources_of(row_at[(it + 1) & 1][any_wave], false);
+            copy_rows(k_next, keys);
+            copy_rows(v_now, values);
+            next_block = block_of(it + 2);
+            floatx16 sum[BN / 32];
+            if constexpr (kF32) {  // (the weights are the scores' registers)
+                multiply_values(v_before);
+                multiply_keys(k_now, sum);
+                take_scores(sum);
+                const Moved moved = new_maximum(it);
+                new_weights(moved.unit, weights);
+                if (moved.any)
+#pragma unroll
+                    for (int t = 0; t < DP / 32; ++t) o[t] *= moved.by;
+            } else {
+                multiply_keys(k_now, sum);
+                constexpr int kReads = kQ * (BN / 32);  // four ahead of the products
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                for (int i = 4; i < kReads; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4 * NQ, 0);
+                take_scores(sum);
+                const Moved moved = new_maximum(it);
+                srv_u32x4 next[BN / 16][NP];
+                multiply_values(v_before);
+                new_weights(moved.unit, next);
+                constexpr int kProducts = BN / 16 * (DP / 32);
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+                for (int i = 2; i < kProducts; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, NP, 1);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * NP, 1);
+                if (moved.any)
+#pragma unroll
+                    for (int t = 0; t < DP / 32; ++t) o[t] *= moved.by;
+#pragma unroll
+                for (int j = 0; j < BN / 16; ++j)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) weights[j][n] = next[j][n];
+            }
+        };
+        for (int it = 0; it < steps; it += 2) {
+            turn(it, lds_k0, lds_k1, lds_v0, lds_v1);
+            turn(it + 1, lds_k1, lds_k0, lds_v1, lds_v0);
+        }
+        wait_copies<0>();
+        __syncthreads();
+        look_for_odd(lds_v1, (steps - 1) | 1);
+        multiply_values(lds_v1);
     }
 
+    if (steps > 0) {
+        __syncthreads();
+        if (lds_odd != 0) {
+            for (int i = any_wave; i < kRows && row0 + i < rows; i += TEAMS * kWaves) {
+                const int64_t here = row0 + i, at_token = token_of(here);
+                one_row<CT, QT>(a, sh, b, len, first + at_token, (int64_t)kv * sh.group + (here - at_token * sh.group), ctx + at_token, prefix, kv);
+            }
+            return;
+        }
+    }
     l += __shfl_xor(l, 32);
+    if constexpr (TEAMS == 2) {  // the second team's part joins the first's
+        // (in the tiles' LDS: 16 bytes of each lane follow each other, DP / 8 times, half of them in
+        // the keys' array)
+        __syncthreads();
+        constexpr int kHalf = DP / 16;
+        static_assert(TEAMS == 1 || kHalf * 256 <= TEAMS * C::kTile, "the output fits the tiles");
+        const int at = wave * 64 + lane;
+        if (team == 1) {
+#pragma unroll
+            for (int x = 0; x < DP / 8; ++x)
+                (x < kHalf ? lds_k0 : lds_v0)[x % kHalf * 256 + at] =
+                    srv_u32x4{__float_as_uint(o[x / 4][4 * (x % 4)]), __float_as_uint(o[x / 4][4 * (x % 4) + 1]), __float_as_uint(o[x / 4][4 * (x % 4) + 2]),
+                              __float_as_uint(o[x / 4][4 * (x % 4) + 3])};
+            ((srv_f32x2 *)lds_k1)[at] = srv_f32x2{m, l};
+        }
+        __syncthreads();
+        if (team == 1) return;
+        const srv_f32x2 other = ((const srv_f32x2 *)lds_k1)[at];
+        const float top = fmaxf(m, other[0]);
+        const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top), g = other[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(other[0] - top);
+        l = l * f + other[1] * g;
+#pragma unroll
+        for (int x = 0; x < DP / 8; ++x) {
+            const srv_u32x4 four = (x < kHalf ? lds_k0 : lds_v0)[x % kHalf * 256 + at];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[x / 4][4 * (x % 4) + i] = fmaf(o[x / 4][4 * (x % 4) + i], f, __uint_as_float(four[i]) * g);
+        }
+    }
     if (row0 + 32 * wave + l32 >= rows) return;
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t at = (first + token) * a.out_stride + head * D;
@@ -472,12 +676,27 @@ __global__ __launch_bounds__(kThreads, (Prompt<CT, QT, DP, FORM>::kPerCu)) void 
         }
 }
 
+// Two teams halve a workgroup's way through its tiles and fill the SIMDs where there are few
+// workgroups, for the joining of their parts; where two workgroups of one team share a CU they go their ways
+// apart, which eight waves behind one barrier do not.  Measured, one / two teams: 1500 frames, 20 heads
+// of 64 (240 workgroups) 37.8 / 32.7 us; sixteen chunks over contexts to 4096 (512) 171 / 205; two
+// prompts of 6000 to 8192 tokens (3500) 978 / 1129.
+template <int CT, int QT, int DP, bool FORM>
+void launch_teams(const PromptAttentionArgs &a, const PromptShape &sh, hipStream_t s) {
+    const dim3 grid(sh.tiles * (unsigned)a.kv_heads);
+    if constexpr (Prompt<CT, QT, DP, FORM>::kTwo && CT == QT && CT != TML_TYPE_F32 && !FORM) {
+        if (grid.x <= (unsigned)device_cus()) {
+            prompt_attention_kernel<CT, QT, DP, FORM, 2><<<grid, dim3(128 * kWaves), 0, s>>>(a, sh);
+            return;
+        }
+    }
+    prompt_attention_kernel<CT, QT, DP, FORM, 1><<<grid, dim3(64 * kWaves), 0, s>>>(a, sh);
+}
 template <int CT, int QT, bool FORM>
 void launch_dim(const PromptAttentionArgs &a, const PromptShape &sh, hipStream_t s) {
-    const dim3 grid((unsigned)(sh.tiles * (unsigned)a.kv_heads)), block(kThreads);
-    if (a.head_dim <= 64) prompt_attention_kernel<CT, QT, 64, FORM><<<grid, block, 0, s>>>(a, sh);
-    else if (a.head_dim <= 128) prompt_attention_kernel<CT, QT, 128, FORM><<<grid, block, 0, s>>>(a, sh);
-    else prompt_attention_kernel<CT, QT, 256, FORM><<<grid, block, 0, s>>>(a, sh);
+    if (a.head_dim <= 64) launch_teams<CT, QT, 64, FORM>(a, sh, s);
+    else if (a.head_dim <= 128) launch_teams<CT, QT, 128, FORM>(a, sh, s);
+    else launch_teams<CT, QT, 256, FORM>(a, sh, s);
 }
 template <int CT, int QT>
 void launch_form(const PromptAttentionArgs &a, const PromptShape &sh, hipStream_t s) {
