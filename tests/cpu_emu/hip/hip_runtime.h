@@ -334,6 +334,7 @@ inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(tml_emu_bf16x8, tm
 inline tml_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(tml_emu_f16x8, tml_emu_f16x8, tml_emu_f32x16 c, int, int, int) { return c; }
 typedef unsigned tml_emu_u32x2_swap __attribute__((ext_vector_type(2)));
 inline tml_emu_u32x2_swap __builtin_amdgcn_permlane32_swap(unsigned a, unsigned b, bool, bool) { return {a, b}; }
+inline tml_emu_u32x2_swap __builtin_amdgcn_permlane16_swap(unsigned a, unsigned b, bool, bool) { return {a, b}; }
 typedef short tml_emu_read_tr __attribute__((ext_vector_type(4)));
 inline tml_emu_read_tr __builtin_amdgcn_ds_read_tr16_b64_v4i16(__attribute__((address_space(3))) tml_emu_read_tr *p) { return *(const tml_emu_read_tr *)p; }
 typedef int tml_emu_i32x4 __attribute__((ext_vector_type(4)));

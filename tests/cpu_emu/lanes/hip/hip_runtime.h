@@ -42,6 +42,7 @@
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16 tml_emu_plain_read_tr
 #define __builtin_amdgcn_s_barrier tml_emu_plain_s_barrier
 #define __builtin_amdgcn_permlane32_swap tml_emu_plain_permlane32_swap
+#define __builtin_amdgcn_permlane16_swap tml_emu_plain_permlane16_swap
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8 tml_emu_plain_mfma_i8
 #define tml_emu_launcher tml_emu_plain_launcher
 #define tml_emu_launch tml_emu_plain_launch
@@ -66,6 +67,7 @@
 #undef __builtin_amdgcn_ds_read_tr16_b64_v4i16
 #undef __builtin_amdgcn_s_barrier
 #undef __builtin_amdgcn_permlane32_swap
+#undef __builtin_amdgcn_permlane16_swap
 #undef __builtin_amdgcn_mfma_i32_16x16x64_i8
 #undef tml_emu_launcher
 #undef tml_emu_launch
@@ -256,4 +258,13 @@ TML_LANE_OP inline tml_emu_u32x2_swap __builtin_amdgcn_permlane32_swap(unsigned 
     unsigned other[2];
     std::memcpy(other, m.data[lane ^ 32], sizeof other);
     return lane < 32 ? tml_emu_u32x2_swap{a, other[0]} : tml_emu_u32x2_swap{other[1], b};
+}
+// The same for the odd 16s of the first and the even 16s of the second.
+TML_LANE_OP inline tml_emu_u32x2_swap __builtin_amdgcn_permlane16_swap(unsigned a, unsigned b, bool, bool) {
+    const unsigned mine[2] = {a, b};
+    const tml_lane_meeting &m = tml_lane_meet(__builtin_return_address(0), mine, sizeof mine);
+    const unsigned lane = tml_emu_lane();
+    unsigned other[2];
+    std::memcpy(other, m.data[lane ^ 16], sizeof other);
+    return (lane & 16) == 0 ? tml_emu_u32x2_swap{a, other[0]} : tml_emu_u32x2_swap{other[1], b};
 }

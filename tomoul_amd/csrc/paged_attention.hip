@@ -373,6 +373,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void paged_attention_k
 }
 
 constexpr int kPerCu = 2;  // workgroups
+constexpr int kAtOnce = 16;  // query heads: a matrix instruction's columns
 
 // A cache past the GPU's last-level cache is read with the streaming policy, a
 // smaller one so that the next step may find it there.  Measured, plain / streaming:
@@ -445,14 +446,14 @@ Status check_paged_attention(const PagedAttentionArgs &a) {
 }
 
 size_t paged_attention_workspace_floats(const PagedAttentionArgs &a) {
-    return attn_empty(a) ? 0 : split_floats(a, shape_of(a, kPerCu));
+    return attn_empty(a) ? 0 : split_floats(a, shape_of(a, kPerCu, kAtOnce));
 }
 
 Status launch_paged_attention(const PagedAttentionArgs &in, const Workspace &ws, hipStream_t s) {
     PagedAttentionArgs a = in;
     if (attn_empty(a)) return Status::Ok();
     if (a.n_blocks == 0) a.table_width = 0;  // no cache: nothing to look at
-    AttnShape sh = shape_of(a, kPerCu);
+    AttnShape sh = shape_of(a, kPerCu, kAtOnce);
     TML_TRY(split_in(a, ws, &sh));
     if (a.cache_type == TML_TYPE_F32) return launch_form<TML_TYPE_F32, TML_TYPE_F32>(a, sh, s);
     if (a.cache_type == TML_TYPE_F16)

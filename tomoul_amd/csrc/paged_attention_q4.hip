@@ -15,15 +15,21 @@
 // outputs were 5e-5 off that way at 448 tokens, f16 ones 5e-4 at 65536; a key's sum is of
 // one group and loses nothing to speak of.)
 //
-// Lane layout, a tile of 32 tokens, two halves h of 16 (as paged_attention.hip):
-//   scores   MFMA h, w: rows tokens 16 h + lane % 16, k the 32 d of group w, columns heads;
-//            the lane's words w of a row follow each other
-//   weights  lane (head, c) holds those of tokens 16 h + 4 c + i, the k of the next product
-//   values   MFMA j: rows d = 16 j + lane % 16, all of group j / 2; the B operand is p_t s_tg
-// Steps and minima or middles of the tile's tokens pass through LDS, where every lane finds
-// those of its eight tokens.  f32 q and weights for f32 outputs are two f16 terms each, q of 16
-// bits is exact in one, and so are the weights rounded once where the output is of 16 bits:
-// that adds to an f16 output about what its own rounding does, to a bf16 one an eighth.
+// Four heads and four groups share the 16 rows or columns that a matrix instruction has, so
+// that with grouped heads of four none of them, and none of the work on what comes out,
+// is idle.  A tile is 32 tokens:
+//   scores   S = q K^T for 16 tokens (columns): row 4 (w % 4) + i is head i, with the elements of
+//            group w alone, zeros elsewhere.  The products of four groups go into one
+//            accumulator, of which lane (token, c) holds group c's sums of four heads; it
+//            multiplies them with the step, and two swaps of halves and rows add the groups
+//            up and leave lane (token, c) the score of head c
+//   weights  pass through LDS, to where lane (4 g + head, c) makes the next product's B operand:
+//            p of its head times the steps of group g, for the eight tokens of its c
+//   values   rows d = 16 j + lane % 16 of group j / 2, of whose output the columns of that group are
+//            kept
+// f32 q, and weights for f32 outputs, are two f16 terms each; q of 16 bits is exact in one, and
+// so are the weights rounded once where the output is of 16 bits: that adds to an f16 output
+// about what its own rounding does, to a bf16 one an eighth.
 #include "paged_split.hpp"
 #include "terms.hpp"
 
@@ -55,6 +61,18 @@ __device__ __forceinline__ uint32_t two_thousands() {
 __device__ __forceinline__ void two_terms(float x, float y, uint32_t *first, uint32_t *second) {
     *first = srv_pack_f16(x, y);
     *second = srv_pack_f16(x - tml_half_bits(*first & 0xFFFFu), y - tml_half_bits(*first >> 16));
+}
+
+// Lane (l, c) of four rows of 16 lanes brings c's part of four sums; it gets sum c of the four rows'.
+__device__ __forceinline__ float sum_and_share(const float (&v)[4]) {
+    float two[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 2]), false, false);
+        two[i] = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    }
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(two[0]), __float_as_uint(two[1]), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
 }
 
 // N consecutive words at p, which may lie on any 4-byte boundary.
@@ -102,25 +120,29 @@ __device__ __forceinline__ Words<(N + 3) / 4> load_bytes(const char *p) {
     return r;
 }
 
-// G: groups of a head.  WIDE: q and the output are f32.  FORM: the scores are capped or
-// biased.  ONCE: the cache is read with the streaming policy.
-template <int G, bool WIDE, bool FORM, bool ONCE>
-__global__ __launch_bounds__(kThreads, G > 4 ? 1 : 2) void paged_attention_q4_kernel(PagedAttentionArgs a, AttnShape sh) {
+// G: groups of a head.  HQ: heads taken at once, in fours.  WIDE: q and the output are f32.  FORM:
+// the scores are capped or biased.  ONCE: the cache is read with the streaming policy.
+template <int G, int HQ, bool WIDE, bool FORM, bool ONCE>
+__global__ __launch_bounds__(kThreads, G * HQ > 8 || (WIDE && G * HQ > 4) ? 1 : 2) void paged_attention_q4_kernel(PagedAttentionArgs a, AttnShape sh) {
     constexpr int D = 32 * G;
-    constexpr int VW = (G + 3) / 4;  // words of a lane's values
+    constexpr int VW = (G + 3) / 4;   // words of a lane's values
+    constexpr int GQ = (G + 3) / 4;   // groups, in fours
+    constexpr int MW = (G + 1) / 2;   // steps and minima that a lane brings of a token's value
     constexpr int NT = WIDE ? 2 : 1;  // terms of q and of the weights
     // The maximum that weights are relative to may fall behind by kBehind (in powers of two)
     // before sums are scaled.  kUp: base of the weights' exponent, their terms reach down to
-    // 2^-38 of the largest (f32 outputs) or 2^-23 (and the maximum behind).
-    constexpr float kBehind = WIDE ? 0.0f : 8.0f, kUp = WIDE ? 14.0f : 6.0f;
+    // 2^-34 of the largest (f32 outputs) or 2^-23 (and the maximum behind).
+    constexpr float kBehind = WIDE ? 4.0f : 8.0f, kUp = WIDE ? 10.0f : 6.0f;
 
     __shared__ __align__(16) int64_t row_off[kWaves][kTile];
-    __shared__ __align__(16) srv_f32x2 meta[kWaves][2][kTile][G];  // steps and minima of keys, steps and middles of values
+    __shared__ __align__(16) srv_f32x2 marks[kWaves][4 * GQ][kTile];  // steps and middles of values
+    __shared__ __align__(16) float weights[kWaves][4 * HQ][kTile];
     __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
     TML_DYNAMIC_LDS(floatx4, dyn);
     float *const wave_o = (float *)dyn;  // [wave][head][D]
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
     const int l16 = lane & 15, c4 = lane >> 4;
+    const int hi = l16 & 3, gi = l16 >> 2;  // this lane's column: of the heads, of the groups
     const int64_t P = a.block_size;
     const uint32_t thousands = two_thousands();
 
@@ -131,100 +153,123 @@ __global__ __launch_bounds__(kThreads, G > 4 ? 1 : 2) void paged_attention_q4_ke
         const int64_t b = walk.b, unit = walk.unit;
         const Span sp = walk.sp;
         const int64_t kv = sh.parts == 1 ? unit : div_short(unit, sh.parts);
-        const int g0 = (int)(unit - kv * sh.parts) * 16, gn = min(16, sh.group - g0);
+        const int g0 = (int)(unit - kv * sh.parts) * 4 * HQ, gn = min(4 * HQ, sh.group - g0);
         const int64_t head0 = kv * sh.group + g0;
 
-        // ---- q as the scores' B operand: lane (head, c) has d = 32 w + 8 c + e, in the nibbles' order.
-        // Scaled by a power of two to [2^14, 2^15) at most, and the odd registers by 2^-4.
-        const int64_t q_at = b * a.q_stride + (head0 + min(l16, gn - 1)) * D;
-        srv_u32x4 q[NT][G];
-        float q_sum[G], to_score = a.scale;
-        {
-            float v[G][8];
+        // ---- q as the scores' A operand: lane (4 (w % 4) + head, c) has d = 32 w + 8 c + e, in the
+        // nibbles' order, others zeros.  Scaled by a power of two to [2^14, 2^15) at most, and the
+        // odd registers by 2^-4.
+        srv_u32x4 q[HQ][NT][G];
+        float q_sum[HQ][4][GQ], to_score[HQ];  // sums of head 4 x + i over group 4 y + c; of head 4 x + c
+#pragma unroll
+        for (int x = 0; x < HQ; ++x) {
+            const int64_t q_at = b * a.q_stride + (head0 + min(4 * x + hi, gn - 1)) * D;
+            float v[GQ][8];  // of this lane's groups 4 y + gi
             uint32_t most = 27u << 23;
 #pragma unroll
-            for (int w = 0; w < G; ++w) {
-                const int64_t at = q_at + 32 * w + 8 * c4;
-                if (WIDE) srv_floats<TML_TYPE_F32>(srv_load8<TML_TYPE_F32>(a.q, at), v[w]);
-                else if (a.q_type == TML_TYPE_F16) srv_floats<TML_TYPE_F16>(srv_load8<TML_TYPE_F16>(a.q, at), v[w]);
-                else srv_floats<TML_TYPE_BF16>(srv_load8<TML_TYPE_BF16>(a.q, at), v[w]);
+            for (int y = 0; y < GQ; ++y) {
+                const int w = 4 * y + gi;
+                const int64_t at = q_at + 32 * min(w, G - 1) + 8 * c4;
+                if (WIDE) srv_floats<TML_TYPE_F32>(srv_load8<TML_TYPE_F32>(a.q, at), v[y]);
+                else if (a.q_type == TML_TYPE_F16) srv_floats<TML_TYPE_F16>(srv_load8<TML_TYPE_F16>(a.q, at), v[y]);
+                else srv_floats<TML_TYPE_BF16>(srv_load8<TML_TYPE_BF16>(a.q, at), v[y]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const uint32_t x = __float_as_uint(v[w][e]) & 0x7F800000u;
-                    most = max(most, x < 0x7F800000u ? x : 0u);
+                    if (w >= G) v[y][e] = 0.0f;
+                    const uint32_t bits = __float_as_uint(v[y][e]) & 0x7F800000u;
+                    most = max(most, bits < 0x7F800000u ? bits : 0u);
                 }
             }
-            most = max(most, (uint32_t)__shfl_xor((int)most, 16));
-            most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-            to_score *= __uint_as_float(most - (14u << 23)) * 0x1p24f;
-            const float up = __uint_as_float((268u << 23) - most);
 #pragma unroll
-            for (int w = 0; w < G; ++w) {
+            for (int o = 4; o < 64; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));  // over groups and c
+            const float up = __uint_as_float((268u << 23) - most);
+            to_score[x] = a.scale * __uint_as_float((uint32_t)__shfl((int)most, c4) - (14u << 23)) * 0x1p24f;
+#pragma unroll
+            for (int y = 0; y < GQ; ++y) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[w][e] *= up;
-                    sum += v[w][e];
+                    v[y][e] *= up;
+                    sum += v[y][e];
                 }
                 sum += __shfl_xor(sum, 16);
                 sum += __shfl_xor(sum, 32);
-                q_sum[w] = sum * 0x1p-24f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q_sum[x][i][y] = __shfl(sum, 4 * c4 + i) * 0x1p-24f;  // (of column 4 c + i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float f = r % 2 ? 0x1p-4f : 1.0f;
-                    if constexpr (WIDE) {
-                        uint32_t first, second;
-                        two_terms(v[w][r] * f, v[w][r + 4] * f, &first, &second);
-                        q[0][w][r] = first;
-                        q[1][w][r] = second;
-                    } else {
-                        q[0][w][r] = srv_pack_f16(v[w][r] * f, v[w][r + 4] * f);
-                    }
+                    uint32_t term[2];
+                    if constexpr (WIDE) two_terms(v[y][r] * f, v[y][r + 4] * f, &term[0], &term[1]);
+                    else term[0] = srv_pack_f16(v[y][r] * f, v[y][r + 4] * f);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int w = 4 * y; w < min(4 * y + 4, G); ++w) q[x][n][w][r] = gi == w % 4 ? term[n] : 0u;
                 }
             }
         }
-        const float to_log2 = to_score * kLog2E;
-        float slope = 0.0f, inv_cap = 0.0f;
+        float slope[HQ], inv_cap = 0.0f;
         if constexpr (FORM) {
-            if (a.slopes != nullptr) slope = a.slopes[head0 + min(l16, gn - 1)] * kLog2E;
+#pragma unroll
+            for (int x = 0; x < HQ; ++x) slope[x] = a.slopes != nullptr ? a.slopes[head0 + min(4 * x + c4, gn - 1)] * kLog2E : 0.0f;
             if (a.cap != 0.0f) inv_cap = 1.0f / a.cap;
         }
 
-        float m = -INFINITY, l = 0.0f;  // of this lane's head; l over this lane's tokens alone
-        uint32_t peak = 0;              // exponent of the largest step so far, of f32 bits; the weights are in units of it
-        floatx4 o[2 * G];
-        float middle[G];                // sums of p c over this lane's tokens
+        float m[HQ], l[HQ];  // of head 4 x + c4; l over the tokens of this lane alone
+        uint32_t peak = 0;   // exponent of the largest step so far, of f32 bits; the weights are in units of it
+        floatx4 o[HQ][2 * G];
+        float middle[HQ][GQ];  // sums of p c of head 4 x + hi over the tokens of c4, group 4 y + gi
 #pragma unroll
-        for (int j = 0; j < 2 * G; ++j) o[j] = floatx4{0, 0, 0, 0};
+        for (int x = 0; x < HQ; ++x) {
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
 #pragma unroll
-        for (int g = 0; g < G; ++g) middle[g] = 0.0f;
+            for (int j = 0; j < 2 * G; ++j) o[x][j] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int y = 0; y < GQ; ++y) middle[x][y] = 0.0f;
+        }
 
         // ---- the tiles: lane % 32 looks up a token's row
         auto block_of = [&](int tile) {
             const int64_t tok = sp.first + (int64_t)tile * kTile + (lane & 31);
             return a.block_table[b * a.table_stride + (uint32_t)min(tok, sp.len - 1) / (uint32_t)P];
         };
-        Words<G> marks;  // steps and minima of the token of lane % 32, of its key or its value
+        Words<G> kr[2];             // keys of tokens 16 h + l16, the lane's words of groups 0 ..
+        uint32_t km[2][GQ];         // and the steps and minima of group 4 y + c4
+        Words<VW> vr[8];            // values of tokens 8 c4 + e
+        uint32_t vm[MW];            // steps and minima of the value of token lane % 32: groups MW (lane / 32) ..
         auto rows_of = [&](int tile, int in_block) {
             const int64_t tok = sp.first + (int64_t)tile * kTile + (lane & 31);
             const bool live = tile < t1 && tok < sp.len && in_block >= 0 && in_block < a.n_blocks;
-            // (a token no one may look at reads the cache's first row, its steps and middles are zero)
+            // (a token no one may look at reads the cache's first row)
             const int64_t off = live ? in_block * a.block_stride + (int64_t)((uint32_t)tok % (uint32_t)P) * a.token_stride + kv * a.head_stride : 0;
             row_off[wave][lane & 31] = off;
-            marks = load_words<G, ONCE>((const char *)(lane < 32 ? a.k_cache : a.v_cache) + off + 16 * G);
+            const char *const from = (const char *)a.v_cache + off + 16 * G;
+            if constexpr (G % 2 == 0) {
+                const Words<MW> w = load_words<MW, ONCE>(from + (lane >> 5) * 4 * MW);
+#pragma unroll
+                for (int i = 0; i < MW; ++i) vm[i] = w.w[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < MW; ++i) vm[i] = *(const uint32_t *)(from + 4 * min((lane >> 5) * MW + i, G - 1));
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             return (uint32_t)__builtin_amdgcn_ballot_w64(live);
         };
-        Words<G> kr[2];
-        Words<VW> vr[8];
         auto load_k = [&]() {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) kr[h] = load_words<G, ONCE>((const char *)a.k_cache + row_off[wave][16 * h + l16] + 4 * G * c4);
+            for (int h = 0; h < 2; ++h) {
+                const char *const row = (const char *)a.k_cache + row_off[wave][16 * h + l16];
+                kr[h] = load_words<G, ONCE>(row + 4 * G * c4);
+#pragma unroll
+                for (int y = 0; y < GQ; ++y) km[h][y] = *(const uint32_t *)(row + 16 * G + 4 * min(4 * y + c4, G - 1));
+            }
         };
         auto load_v = [&]() {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vr[e] = load_bytes<G, ONCE>((const char *)a.v_cache + row_off[wave][16 * (e / 4) + 4 * c4 + e % 4] + G * l16);
+            for (int e = 0; e < 8; ++e) vr[e] = load_bytes<G, ONCE>((const char *)a.v_cache + row_off[wave][8 * c4 + e] + G * l16);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
@@ -236,92 +281,116 @@ __global__ __launch_bounds__(kThreads, G > 4 ? 1 : 2) void paged_attention_q4_ke
         __builtin_amdgcn_sched_barrier(0);
         load_v();
         while (t < t1) {
-            const bool mine = seen >> (lane & 31) & 1;
-            float step_most = 0.0f;
+            // ---- steps and middles of the values to LDS, the steps in units of the largest so far (a
+            // step that is no number, or infinite, counts as none: its weights are what they are)
+            {
+                const bool mine = seen >> (lane & 31) & 1;
+                float step[MW], least[MW];
+                uint32_t most = 0;
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const uint32_t d = mine ? marks.w[g] : 0u;
-                const float step = tml_half_bits(d & 0xFFFFu);
-                meta[wave][lane >> 5][lane & 31][g] = srv_f32x2{step, fmaf(step, lane < 32 ? 0.0f : 8.0f, tml_half_bits(d >> 16))};
-                step_most = fmaxf(step_most, step);
+                for (int i = 0; i < MW; ++i) {
+                    const uint32_t d = mine ? vm[i] : 0u;
+                    step[i] = tml_half_bits(d & 0xFFFFu);
+                    least[i] = tml_half_bits(d >> 16);
+                    const uint32_t bits = __float_as_uint(step[i]) & 0x7F800000u;
+                    most = max(most, bits < 0x7F800000u ? bits : 0u);
+                }
+                if (__builtin_amdgcn_ballot_w64(most > peak) != 0) {
+#pragma unroll
+                    for (int x = 1; x < 64; x <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, x));
+                    const float f = peak == 0u ? 1.0f : __uint_as_float(peak) / __uint_as_float(most);
+                    peak = most;
+#pragma unroll
+                    for (int x = 0; x < HQ; ++x)
+#pragma unroll
+                        for (int j = 0; j < 2 * G; ++j) o[x][j] *= f;
+                }
+                // (no step yet: all of them are zero)
+                const float in_units = peak == 0u ? 1.0f : __uint_as_float((253u << 23) - peak);  // 2^-1 / the largest's power of two
+#pragma unroll
+                for (int i = 0; i < MW; ++i) {
+                    const int g = (lane >> 5) * MW + i;
+                    if (G % 2 == 0 || g < G) marks[wave][g][lane & 31] = srv_f32x2{step[i] * in_units, fmaf(step[i], 8.0f, least[i])};
+                }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-
-            // ---- scores
-            float s[8];
+            // ---- scores: of head 4 x + c4 and tokens 16 h + l16
+            float s[HQ][2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+            for (int h = 0; h < 2; ++h) {
+                floatx4 sum[HQ][GQ];
 #pragma unroll
-            for (int w = 0; w < G; ++w) {
+                for (int x = 0; x < HQ; ++x)
+#pragma unroll
+                    for (int y = 0; y < GQ; ++y) sum[x][y] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < G; ++w) {
+                    const srv_u32x4 n = nibbles(kr[h].w[w]);
+#pragma unroll
+                    for (int x = 0; x < HQ; ++x)
+#pragma unroll
+                        for (int term = 0; term < NT; ++term) sum[x][w / 4] = mma16<TML_TYPE_F16>(q[x][term][w], n, sum[x][w / 4]);
+                }
+#pragma unroll
+                for (int x = 0; x < HQ; ++x) {
+                    float by[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int y = 0; y < GQ; ++y) {
+                        const uint32_t d = G % 4 == 0 || 4 * y + c4 < G ? km[h][y] : 0u;
+                        const float step = tml_half_bits(d & 0xFFFFu), least = tml_half_bits(d >> 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) by[i] = fmaf(sum[x][y][i], step, fmaf(q_sum[x][i][y], least, by[i]));
+                    }
+                    s[x][h] = sum_and_share(by);
+                }
+            }
+            bool behind = false;
+#pragma unroll
+            for (int x = 0; x < HQ; ++x)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const srv_u32x4 n = nibbles(kr[h].w[w]);
-                    floatx4 sum = mma16<TML_TYPE_F16>(n, q[0][w], floatx4{0, 0, 0, 0});
-                    if constexpr (WIDE) sum = mma16<TML_TYPE_F16>(n, q[1][w], sum);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const srv_f32x2 d = meta[wave][0][16 * h + 4 * c4 + i][w];
-                        s[4 * h + i] = fmaf(sum[i], d[0], fmaf(q_sum[w], d[1], s[4 * h + i]));
+                    if constexpr (FORM) {
+                        const float y = s[x][h] * to_score[x], from = (float)(sp.len - 1 - sp.first - ((int64_t)t * kTile + 16 * h + l16));
+                        s[x][h] = fmaf(-slope[x], from, (inv_cap != 0.0f ? cap_score(y, a.cap, inv_cap) : y) * kLog2E);
+                    } else {
+                        s[x][h] *= to_score[x] * kLog2E;
                     }
+                    s[x][h] = (seen >> (16 * h + l16) & 1) ? s[x][h] : -INFINITY;
+                    behind |= s[x][h] > m[x] + kBehind;
                 }
-                if (G > 4 && w % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (FORM) {
-                const float from = (float)(sp.len - 1 - sp.first - ((int64_t)t * kTile + 4 * c4));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = s[e] * to_score;
-                    s[e] = fmaf(-slope, from - (float)(16 * (e / 4) + e % 4), (inv_cap != 0.0f ? cap_score(x, a.cap, inv_cap) : x) * kLog2E);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] *= to_log2;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = (seen >> (16 * (e / 4) + 4 * c4 + e % 4) & 1) ? s[e] : -INFINITY;
             t += kWaves;
             seen = rows_of(t, block);
             load_k();
             block = block_of(t + kWaves);
 
             // ---- weights
-            float most = s[0];
+            if (__builtin_amdgcn_ballot_w64(behind) != 0) {
 #pragma unroll
-            for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            if (__builtin_amdgcn_ballot_w64(most > m + kBehind) != 0) {
-                const float m_new = fmaxf(m, most);
-                const float f = rescale(m, m_new);
-                m = m_new;
-                l *= f;
+                for (int x = 0; x < HQ; ++x) {
+                    float most = fmaxf(s[x][0], s[x][1]);
 #pragma unroll
-                for (int j = 0; j < 2 * G; ++j) o[j] *= f;
+                    for (int i = 1; i < 16; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
+                    const float m_new = fmaxf(m[x], most), f = rescale(m[x], m_new);
+                    m[x] = m_new;
+                    l[x] *= f;
+                    const float column = __shfl(f, 16 * hi);
 #pragma unroll
-                for (int g = 0; g < G; ++g) middle[g] *= f;
+                    for (int j = 0; j < 2 * G; ++j) o[x][j] *= column;
+#pragma unroll
+                    for (int y = 0; y < GQ; ++y) middle[x][y] *= column;
+                }
             }
-            // (a step that is no number, or infinite, counts as none: its weights are what they are)
-            uint32_t step_bits = lane < 32 ? 0u : __float_as_uint(step_most) & 0x7F800000u;
-            if (step_bits == 0x7F800000u) step_bits = 0u;
-            if (__builtin_amdgcn_ballot_w64(step_bits > peak) != 0) {
 #pragma unroll
-                for (int x = 1; x < 64; x <<= 1) step_bits = max(step_bits, (uint32_t)__shfl_xor((int)step_bits, x));
-                const float f = peak == 0u ? 1.0f : __uint_as_float(peak) / __uint_as_float(step_bits);
-                peak = step_bits;
+            for (int x = 0; x < HQ; ++x) {
+                const float base = (m[x] == -INFINITY ? 0.0f : m[x]) - kUp;
 #pragma unroll
-                for (int j = 0; j < 2 * G; ++j) o[j] *= f;
+                for (int h = 0; h < 2; ++h) {
+                    const float p = __builtin_amdgcn_exp2f(s[x][h] - base);
+                    l[x] += p;
+                    weights[wave][4 * x + c4][16 * h + l16] = p;
+                }
             }
-            // (no step yet: all of them are zero)
-            const float unit_step = peak == 0u ? 1.0f : __uint_as_float((253u << 23) - peak);  // 2^-1 / the largest's power of two
-            const float base = (m == -INFINITY ? 0.0f : m) - kUp;
-            float p[8], in_units[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(s[e] - base);
-                l += p[e];
-                in_units[e] = p[e] * unit_step;
-            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
             // ---- values
             srv_u32x4 pair[2 * VW];  // 16 bits of tokens 2 i and 2 i + 1
 #pragma unroll
@@ -330,29 +399,31 @@ __global__ __launch_bounds__(kThreads, G > 4 ? 1 : 2) void paged_attention_q4_ke
                 for (int i = 0; i < 4; ++i)
                     pair[x][i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[x / 2], vr[2 * i].w[x / 2], x % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                float step[8];
+            for (int y = 0; y < GQ; ++y) {
+                srv_u32x4 weight[HQ][NT];
+                srv_f32x2 mark[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const srv_f32x2 d = meta[wave][1][16 * (e / 4) + 4 * c4 + e % 4][g];
-                    step[e] = d[0];
-                    middle[g] = fmaf(p[e], d[1], middle[g]);
-                }
-                srv_u32x4 weight[NT];
+                for (int e = 0; e < 8; ++e) mark[e] = marks[wave][4 * y + gi][8 * c4 + e];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = in_units[2 * i] * step[2 * i], y = in_units[2 * i + 1] * step[2 * i + 1];
-                    if constexpr (WIDE) {
-                        uint32_t first, second;
-                        two_terms(x, y, &first, &second);
-                        weight[0][i] = first;
-                        weight[1][i] = second;
-                    } else {
-                        weight[0][i] = srv_pack_f16(x, y);
+                for (int x = 0; x < HQ; ++x) {
+                    float p[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        p[e] = weights[wave][4 * x + hi][8 * c4 + e];
+                        middle[x][y] = fmaf(p[e], mark[e][1], middle[x][y]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float u = p[2 * i] * mark[2 * i][0], v = p[2 * i + 1] * mark[2 * i + 1][0];
+                        uint32_t term[2];
+                        if constexpr (WIDE) two_terms(u, v, &term[0], &term[1]);
+                        else term[0] = srv_pack_f16(u, v);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) weight[x][n][i] = term[n];
                     }
                 }
 #pragma unroll
-                for (int j = 2 * g; j < 2 * g + 2; ++j) {
+                for (int j = 8 * y; j < min(8 * y + 8, 2 * G); ++j) {
                     srv_u32x4 n;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -360,27 +431,46 @@ __global__ __launch_bounds__(kThreads, G > 4 ? 1 : 2) void paged_attention_q4_ke
                         n[i] = j % 2 ? two_nibbles<4>(two, thousands) : two_nibbles<0>(two, thousands);
                     }
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) o[j] = mma16<TML_TYPE_F16>(n, weight[x], o[j]);
+                    for (int x = 0; x < HQ; ++x)
+#pragma unroll
+                        for (int term = 0; term < NT; ++term) o[x][j] = mma16<TML_TYPE_F16>(n, weight[x][term], o[x][j]);
                 }
-                if (G > 4 && g % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (else registers run out)
             }
             load_v();
         }
 
         // ---- the waves' parts
-        const float f = join_scale(wave_m, wave_l, wave, m, l);
-        const float up = (peak == 0u ? 0.0f : __uint_as_float(peak) * 2.0f) * f;  // out of the weights' units
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            middle[g] += __shfl_xor(middle[g], 16);
-            middle[g] += __shfl_xor(middle[g], 32);
+        for (int x = 0; x < HQ; ++x) {
+#pragma unroll
+            for (int i = 1; i < 16; i <<= 1) l[x] += __shfl_xor(l[x], i);
+            if (l16 == 0) {
+                wave_m[wave][4 * x + c4] = m[x];
+                wave_l[wave][4 * x + c4] = l[x];
+            }
         }
-        if (l16 < gn) {
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 2 * G; ++j) {
-                const float r = j % 2 ? up * 0x1p-4f : up, z = middle[j / 2] * f;
-                *(floatx4 *)(wave_o + (wave * sh.heads + l16) * D + 16 * j + 4 * c4) =
-                    floatx4{fmaf(o[j][0], r, z), fmaf(o[j][1], r, z), fmaf(o[j][2], r, z), fmaf(o[j][3], r, z)};
+        for (int x = 0; x < HQ; ++x) {
+            const int head = 4 * x + hi;
+            float top = wave_m[0][head];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wave_m[w][head]);
+            const float f = rescale(wave_m[wave][head], top);
+            const float up = (peak == 0u ? 0.0f : __uint_as_float(peak) * 2.0f) * f;  // out of the weights' units
+#pragma unroll
+            for (int y = 0; y < GQ; ++y) {
+                float z = middle[x][y];
+                z += __shfl_xor(z, 16);
+                z += __shfl_xor(z, 32);
+                z *= f;
+#pragma unroll
+                for (int j = 8 * y; j < min(8 * y + 8, 2 * G); ++j) {
+                    const float r = j % 2 ? up * 0x1p-4f : up;
+                    if (head < gn && gi == j / 2 % 4)
+                        *(floatx4 *)(wave_o + (wave * sh.heads + head) * D + 16 * j + 4 * c4) =
+                            floatx4{fmaf(o[x][j][0], r, z), fmaf(o[x][j][1], r, z), fmaf(o[x][j][2], r, z), fmaf(o[x][j][3], r, z)};
+                }
             }
         }
         store_list(a.q_type, a, sh, walk, t1, head0, gn, D, wave_m, wave_l, wave_o);
@@ -399,19 +489,29 @@ Status launch_join(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t
 constexpr int kPerCu = 2;  // workgroups
 constexpr int64_t kLastLevel = (int64_t)256 << 20;  // a cache past it is read with the streaming policy
 
-template <int G, bool WIDE, bool FORM>
+// Query heads taken at once: eight, or four where the registers end (and where there are no more).
+int heads_at_once(const PagedAttentionArgs &a) { return a.head_dim > 128 || a.q_heads / a.kv_heads <= 4 ? 4 : 8; }
+
+template <int G, int HQ, bool WIDE, bool FORM>
 void launch_kernel(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
     const size_t lds = (size_t)kWaves * sh.heads * 32 * G * 4;
     const dim3 grid(1u << sh.grid_log2), block(kThreads);
     const double bytes = 40.0 * G * a.n_blocks * a.block_size * a.kv_heads;
-    if (bytes > kLastLevel) paged_attention_q4_kernel<G, WIDE, FORM, true><<<grid, block, lds, s>>>(a, sh);
-    else paged_attention_q4_kernel<G, WIDE, FORM, false><<<grid, block, lds, s>>>(a, sh);
+    if (bytes > kLastLevel) paged_attention_q4_kernel<G, HQ, WIDE, FORM, true><<<grid, block, lds, s>>>(a, sh);
+    else paged_attention_q4_kernel<G, HQ, WIDE, FORM, false><<<grid, block, lds, s>>>(a, sh);
+}
+template <int G, int HQ>
+void launch_form(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
+    const bool form = a.cap != 0.0f || a.slopes != nullptr;
+    if (a.q_type == TML_TYPE_F32) form ? launch_kernel<G, HQ, true, true>(a, sh, s) : launch_kernel<G, HQ, true, false>(a, sh, s);
+    else form ? launch_kernel<G, HQ, false, true>(a, sh, s) : launch_kernel<G, HQ, false, false>(a, sh, s);
 }
 template <int G>
 void launch_groups(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
-    const bool form = a.cap != 0.0f || a.slopes != nullptr;
-    if (a.q_type == TML_TYPE_F32) form ? launch_kernel<G, true, true>(a, sh, s) : launch_kernel<G, true, false>(a, sh, s);
-    else form ? launch_kernel<G, false, true>(a, sh, s) : launch_kernel<G, false, false>(a, sh, s);
+    if constexpr (G <= 4) {
+        if (sh.at_once == 8) return launch_form<G, 2>(a, sh, s);
+    }
+    launch_form<G, 1>(a, sh, s);
 }
 
 }  // namespace
@@ -432,13 +532,13 @@ Status check_paged_attention_q4(const PagedAttentionArgs &a) {
     return Status::Ok();
 }
 
-size_t paged_attention_q4_workspace_floats(const PagedAttentionArgs &a) { return attn_empty(a) ? 0 : split_floats(a, shape_of(a, kPerCu)); }
+size_t paged_attention_q4_workspace_floats(const PagedAttentionArgs &a) { return attn_empty(a) ? 0 : split_floats(a, shape_of(a, kPerCu, heads_at_once(a))); }
 
 Status launch_paged_attention_q4(const PagedAttentionArgs &in, const Workspace &ws, hipStream_t s) {
     PagedAttentionArgs a = in;
     if (attn_empty(a)) return Status::Ok();
     if (a.n_blocks == 0) a.table_width = 0;  // no cache: nothing to look at
-    AttnShape sh = shape_of(a, kPerCu);
+    AttnShape sh = shape_of(a, kPerCu, heads_at_once(a));
     TML_TRY(split_in(a, ws, &sh));
     switch (a.head_dim / 32) {
         case 1: launch_groups<1>(a, sh, s); break;

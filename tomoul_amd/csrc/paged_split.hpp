@@ -2,8 +2,8 @@
 // (paged_attention.hip, paged_attention_q4.hip): the split of the batch's tiles over
 // the workgroups, the waves' and the parts' joining, the scores' caps and biases.
 //
-// Split.  A request's tiles of 32 tokens, for each key-value head (and 16 query
-// heads of its group), follow each other in one long list over the batch, which the
+// Split.  A request's tiles of 32 tokens, for each key-value head (and the query heads
+// of its group that a workgroup takes at once), follow each other in one long list over the batch, which the
 // workgroups share evenly: each sums the requests' lengths itself, so the split goes
 // by the lengths as they are on the GPU, ragged or not, without the host.  A
 // workgroup's share is some whole heads and at most two parts of one; its waves take
@@ -29,8 +29,9 @@ struct ListParts {
 
 struct AttnShape {
     int group;      // query heads of a key-value head
-    int parts;      // 16-head parts of a group
-    int heads;      // query heads of a part, at most 16
+    int at_once;    // query heads that a workgroup takes at a time
+    int parts;      // of a group
+    int heads;      // query heads of a part
     int64_t units;  // key-value heads * parts: a request's lists of tiles
     int64_t positions;  // of a table row
     int grid_log2;  // workgroups
@@ -229,8 +230,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_attention_join_kernel(P
     const int head = (int)blockIdx.x * kJoinWaves + uniform((int)(threadIdx.x >> 6));
     const int64_t b = blockIdx.y;
     if (head >= (int)a.q_heads) return;
-    const int kv = (int)((uint32_t)head / (uint32_t)sh.group), in_group = head - kv * sh.group, g = in_group & 15;
-    const ListParts list = sh.lists[b * sh.units + kv * sh.parts + (in_group >> 4)];
+    const int kv = (int)((uint32_t)head / (uint32_t)sh.group), in_group = head - kv * sh.group, part = in_group / sh.at_once, g = in_group - part * sh.at_once;
+    const ListParts list = sh.lists[b * sh.units + kv * sh.parts + part];
     const int count = uniform(list.count), D = (int)a.head_dim;
     if (count == 0) return;
     const float *const first = sh.partials + (2 * (int64_t)uniform(list.first) + 1) * sh.part_floats;
@@ -273,11 +274,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_attention_join_kernel(P
 // Workgroups: a power of two, the largest of which `per_cu` fit each CU.
 inline int workgroups_log2(int per_cu) { return 31 - __builtin_clz((unsigned)(per_cu * std::max(1, device_cus()))); }
 
-inline AttnShape shape_of(const PagedAttentionArgs &a, int per_cu) {
+inline AttnShape shape_of(const PagedAttentionArgs &a, int per_cu, int at_once) {
     AttnShape sh{};
     sh.group = (int)(a.q_heads / a.kv_heads);
-    sh.parts = (sh.group + 15) / 16;
-    sh.heads = std::min(sh.group, 16);
+    sh.at_once = at_once;
+    sh.parts = (sh.group + at_once - 1) / at_once;
+    sh.heads = std::min(sh.group, at_once);
     sh.units = a.kv_heads * sh.parts;
     sh.positions = a.table_width * a.block_size;
     sh.grid_log2 = workgroups_log2(per_cu);
