@@ -386,7 +386,7 @@ constexpr int64_t kLastLevel = (int64_t)256 << 20;
 template <int CT, int QT, int DP, bool FORM>
 void launch_kernel(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
     const size_t lds = (size_t)kWaves * sh.heads * DP * 4;
-    const dim3 grid(1u << sh.grid_log2), block(kThreads);
+    const dim3 grid(sh.grid), block(kThreads);
     const double bytes = 2.0 * type_bytes(CT) * a.n_blocks * a.block_size * a.kv_heads * a.head_dim;
     if (bytes > kLastLevel) paged_attention_kernel<CT, QT, DP, true, FORM><<<grid, block, lds, s>>>(a, sh);
     else paged_attention_kernel<CT, QT, DP, false, FORM><<<grid, block, lds, s>>>(a, sh);

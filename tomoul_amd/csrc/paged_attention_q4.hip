@@ -80,7 +80,7 @@ template <int N>
 struct Words {
     uint32_t w[N];
 };
-template <int N, bool ONCE>
+template <int N>
 __device__ __forceinline__ Words<N> load_words(const char *p) {
     Words<N> r;
     typedef srv_u32x4 x4 __attribute__((aligned(4)));
@@ -88,42 +88,47 @@ __device__ __forceinline__ Words<N> load_words(const char *p) {
     int i = 0;
 #pragma unroll
     for (; i + 4 <= N; i += 4) {
-        const x4 v = ONCE ? __builtin_nontemporal_load((const x4 *)(p + 4 * i)) : *(const x4 *)(p + 4 * i);
+        const x4 v = *(const x4 *)(p + 4 * i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) r.w[i + j] = v[j];
     }
     if (N % 4 >= 2) {
-        const x2 v = ONCE ? __builtin_nontemporal_load((const x2 *)(p + 4 * (N / 4 * 4))) : *(const x2 *)(p + 4 * (N / 4 * 4));
+        const x2 v = *(const x2 *)(p + 4 * (N / 4 * 4));
         r.w[N / 4 * 4] = v[0];
         r.w[N / 4 * 4 + 1] = v[1];
     }
-    if (N % 2 == 1) r.w[N - 1] = ONCE ? __builtin_nontemporal_load((const uint32_t *)(p + 4 * (N - 1))) : *(const uint32_t *)(p + 4 * (N - 1));
+    if (N % 2 == 1) r.w[N - 1] = *(const uint32_t *)(p + 4 * (N - 1));
     return r;
 }
 // N consecutive bytes at p in (N + 3) / 4 words.  Past the last of a row's 16 lanes lie its
 // steps and minima, 4 N bytes, so 3 bytes may be taken as 4 and 5 to 7 as 8.
-template <int N, bool ONCE>
+template <int N>
 __device__ __forceinline__ Words<(N + 3) / 4> load_bytes(const char *p) {
     Words<(N + 3) / 4> r;
     if constexpr (N == 1) {
-        r.w[0] = ONCE ? __builtin_nontemporal_load((const uint8_t *)p) : *(const uint8_t *)p;
+        r.w[0] = *(const uint8_t *)p;
     } else if constexpr (N == 2) {
-        r.w[0] = ONCE ? __builtin_nontemporal_load((const uint16_t *)p) : *(const uint16_t *)p;
+        r.w[0] = *(const uint16_t *)p;
     } else if constexpr (N <= 4) {
         typedef uint32_t any __attribute__((aligned(1)));
-        r.w[0] = ONCE ? __builtin_nontemporal_load((const any *)p) : *(const any *)p;
+        r.w[0] = *(const any *)p;
     } else {
-        const srv_u32x2_any v = ONCE ? __builtin_nontemporal_load((const srv_u32x2_any *)p) : *(const srv_u32x2_any *)p;
+        const srv_u32x2_any v = *(const srv_u32x2_any *)p;
         r.w[0] = v[0];
         r.w[1] = v[1];
     }
     return r;
 }
 
+// Workgroups on a CU, as the registers allow.  (16-bit q, dim 128, groups of four heads: three against
+// two 64 against 70 us for 64 requests of up to 4096 tokens, 40.6 against 39 for two of up to 65536;
+// four spill: 102 and 66.)
+constexpr int per_cu(int groups, int fours, bool wide) { return wide ? (groups * fours > 4 ? 1 : 2) : (groups * fours > 4 || fours > 1 ? 2 : 3); }
+
 // G: groups of a head.  HQ: heads taken at once, in fours.  WIDE: q and the output are f32.  FORM:
-// the scores are capped or biased.  ONCE: the cache is read with the streaming policy.
-template <int G, int HQ, bool WIDE, bool FORM, bool ONCE>
-__global__ __launch_bounds__(kThreads, G * HQ > 8 || (WIDE && G * HQ > 4) ? 1 : 2) void paged_attention_q4_kernel(PagedAttentionArgs a, AttnShape sh) {
+// the scores are capped or biased.
+template <int G, int HQ, bool WIDE, bool FORM>
+__global__ __launch_bounds__(kThreads, per_cu(G, HQ, WIDE)) void paged_attention_q4_kernel(PagedAttentionArgs a, AttnShape sh) {
     constexpr int D = 32 * G;
     constexpr int VW = (G + 3) / 4;   // words of a lane's values
     constexpr int GQ = (G + 3) / 4;   // groups, in fours
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(kThreads, G * HQ > 8 || (WIDE && G * HQ > 4) ? 1 : 
             row_off[wave][lane & 31] = off;
             const char *const from = (const char *)a.v_cache + off + 16 * G;
             if constexpr (G % 2 == 0) {
-                const Words<MW> w = load_words<MW, ONCE>(from + (lane >> 5) * 4 * MW);
+                const Words<MW> w = load_words<MW>(from + (lane >> 5) * 4 * MW);
 #pragma unroll
                 for (int i = 0; i < MW; ++i) vm[i] = w.w[i];
             } else {
@@ -262,14 +267,14 @@ __global__ __launch_bounds__(kThreads, G * HQ > 8 || (WIDE && G * HQ > 4) ? 1 : 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const char *const row = (const char *)a.k_cache + row_off[wave][16 * h + l16];
-                kr[h] = load_words<G, ONCE>(row + 4 * G * c4);
+                kr[h] = load_words<G>(row + 4 * G * c4);
 #pragma unroll
                 for (int y = 0; y < GQ; ++y) km[h][y] = *(const uint32_t *)(row + 16 * G + 4 * min(4 * y + c4, G - 1));
             }
         };
         auto load_v = [&]() {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vr[e] = load_bytes<G, ONCE>((const char *)a.v_cache + row_off[wave][8 * c4 + e] + G * l16);
+            for (int e = 0; e < 8; ++e) vr[e] = load_bytes<G>((const char *)a.v_cache + row_off[wave][8 * c4 + e] + G * l16);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
@@ -486,19 +491,18 @@ Status launch_join(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t
     return Status::Ok();
 }
 
-constexpr int kPerCu = 2;  // workgroups
-constexpr int64_t kLastLevel = (int64_t)256 << 20;  // a cache past it is read with the streaming policy
-
 // Query heads taken at once: eight, or four where the registers end (and where there are no more).
 int heads_at_once(const PagedAttentionArgs &a) { return a.head_dim > 128 || a.q_heads / a.kv_heads <= 4 ? 4 : 8; }
+AttnShape shape_of(const PagedAttentionArgs &a) {
+    const int heads = heads_at_once(a);
+    return shape_of(a, per_cu((int)a.head_dim / 32, heads / 4, a.q_type == TML_TYPE_F32), heads);
+}
 
 template <int G, int HQ, bool WIDE, bool FORM>
 void launch_kernel(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
     const size_t lds = (size_t)kWaves * sh.heads * 32 * G * 4;
-    const dim3 grid(1u << sh.grid_log2), block(kThreads);
-    const double bytes = 40.0 * G * a.n_blocks * a.block_size * a.kv_heads;
-    if (bytes > kLastLevel) paged_attention_q4_kernel<G, HQ, WIDE, FORM, true><<<grid, block, lds, s>>>(a, sh);
-    else paged_attention_q4_kernel<G, HQ, WIDE, FORM, false><<<grid, block, lds, s>>>(a, sh);
+    const dim3 grid(sh.grid), block(kThreads);
+    paged_attention_q4_kernel<G, HQ, WIDE, FORM><<<grid, block, lds, s>>>(a, sh);
 }
 template <int G, int HQ>
 void launch_form(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
@@ -532,13 +536,13 @@ Status check_paged_attention_q4(const PagedAttentionArgs &a) {
     return Status::Ok();
 }
 
-size_t paged_attention_q4_workspace_floats(const PagedAttentionArgs &a) { return attn_empty(a) ? 0 : split_floats(a, shape_of(a, kPerCu, heads_at_once(a))); }
+size_t paged_attention_q4_workspace_floats(const PagedAttentionArgs &a) { return attn_empty(a) ? 0 : split_floats(a, shape_of(a)); }
 
 Status launch_paged_attention_q4(const PagedAttentionArgs &in, const Workspace &ws, hipStream_t s) {
     PagedAttentionArgs a = in;
     if (attn_empty(a)) return Status::Ok();
     if (a.n_blocks == 0) a.table_width = 0;  // no cache: nothing to look at
-    AttnShape sh = shape_of(a, kPerCu, heads_at_once(a));
+    AttnShape sh = shape_of(a);
     TML_TRY(split_in(a, ws, &sh));
     switch (a.head_dim / 32) {
         case 1: launch_groups<1>(a, sh, s); break;

@@ -34,7 +34,7 @@ struct AttnShape {
     int heads;      // query heads of a part
     int64_t units;  // key-value heads * parts: a request's lists of tiles
     int64_t positions;  // of a table row
-    int grid_log2;  // workgroups
+    int grid;  // workgroups
     int part_floats;  // of a part: 16-head part's values, maxima and sums
     float *partials;  // two parts a workgroup
     ListParts *lists;  // [batch][units], or nullptr: no list can be long enough to be split
@@ -127,8 +127,7 @@ __device__ __forceinline__ bool first_list(int qt, const PagedAttentionArgs &a, 
     // Lists of so few tiles that a part costs more to join than to read stay whole:
     // the workgroups share the lists then, not their tiles.
     w.lists = __builtin_amdgcn_ballot_w64(longest > kWhole) == 0;
-    w.share = max(w.lists ? (a.batch * sh.units + gridDim.x - 1) >> sh.grid_log2 : (total + gridDim.x - 1) >> sh.grid_log2,
-                  (int64_t)(w.lists ? 1 : kWhole / 2));
+    w.share = max(div_short((w.lists ? a.batch * sh.units : total) + gridDim.x - 1, gridDim.x), (int64_t)(w.lists ? 1 : kWhole / 2));
     w.u = (int64_t)blockIdx.x * w.share;
     w.u_end = min(w.u + w.share, w.lists ? a.batch * sh.units : total);
     if (w.u >= w.u_end) return false;
@@ -271,9 +270,6 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_attention_join_kernel(P
     if (2 * lane + 128 < D) store_result(QT, a, b, head, 2 * lane + 128, sum[1], sum_l);
 }
 
-// Workgroups: a power of two, the largest of which `per_cu` fit each CU.
-inline int workgroups_log2(int per_cu) { return 31 - __builtin_clz((unsigned)(per_cu * std::max(1, device_cus()))); }
-
 inline AttnShape shape_of(const PagedAttentionArgs &a, int per_cu, int at_once) {
     AttnShape sh{};
     sh.group = (int)(a.q_heads / a.kv_heads);
@@ -282,7 +278,7 @@ inline AttnShape shape_of(const PagedAttentionArgs &a, int per_cu, int at_once) 
     sh.heads = std::min(sh.group, at_once);
     sh.units = a.kv_heads * sh.parts;
     sh.positions = a.table_width * a.block_size;
-    sh.grid_log2 = workgroups_log2(per_cu);
+    sh.grid = per_cu * std::max(1, device_cus());
     sh.part_floats = sh.heads * (int)(a.head_dim + 2);
     return sh;
 }
@@ -299,13 +295,13 @@ inline bool may_split(const PagedAttentionArgs &a) {
 
 // Floats of the workspace: the parts, then where each list's parts are.
 inline size_t split_floats(const PagedAttentionArgs &a, const AttnShape &sh) {
-    return may_split(a) ? (size_t)((((int64_t)2 << sh.grid_log2) * sh.part_floats) + 2 * a.batch * sh.units) : 0;
+    return may_split(a) ? (size_t)((int64_t)2 * sh.grid * sh.part_floats + 2 * a.batch * sh.units) : 0;
 }
 inline Status split_in(const PagedAttentionArgs &a, const Workspace &ws, AttnShape *sh) {
     if (!may_split(a)) return Status::Ok();
     if (ws.partial_floats < split_floats(a, *sh)) return Status::Err(TML_ERR_INVALID_ARG, "paged attention: workspace too small");
     sh->partials = ws.partials;
-    sh->lists = (ListParts *)(ws.partials + ((int64_t)2 << sh->grid_log2) * sh->part_floats);
+    sh->lists = (ListParts *)(ws.partials + (int64_t)2 * sh->grid * sh->part_floats);
     return Status::Ok();
 }
 
