@@ -8,11 +8,11 @@
 // maximum: it rises a few times a row) and joins them at the end; bound by memory, or for
 // few rows by what one CU can read.
 //
-// The `top` best, by value and then by the lower index, from the lanes' own best: the
-// n-th of a wave's 64 is a value that n elements reach, the largest of the waves' such
-// values is T, and a second pass over the row (out of the caches) collects the few that
-// reach T.  Each of them then counts those before it, which is its place.  Where they
-// are more than LDS holds, the n-th of those held is the next T.
+// The `top` best, by value and then by the lower index, from the lanes' own best: in each
+// of w waves at least n / w elements reach the (n / w)-th largest of them, so n of the row
+// reach the least of the waves' such values, T, and a second pass over the row (out of the caches) collects
+// the few that do.  Each of them then counts those before it, which is its place.  Where
+// they are more than LDS holds, the n-th of those held is the next T.
 #include "serving.hpp"
 
 #include <algorithm>
@@ -57,9 +57,8 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsArgs a) {
     const unsigned cols = (unsigned)a.cols, chunks = cols / 8, rest = cols % 8;
 
     Sums sum{kLowest, 0.0f, 0.0f};
-    int best = -1;  // index of this lane's first maximum
-    float best_x = -INFINITY;
-    auto take = [&](const auto &v, unsigned first) {
+    float best = -INFINITY;  // of this lane, NaN aside
+    auto take = [&](const auto &v) {
         constexpr int N = sizeof v / sizeof(float);
         float most = v[0];
 #pragma unroll
@@ -68,14 +67,7 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsArgs a) {
             const float d = sum.m - most, f = __builtin_amdgcn_exp2f(d * kLog2E);
             sum = {most, sum.s * f, (sum.t + sum.s * fmaxf(d, kFar)) * f};
         }
-        if (TOP && (most > best_x || best < 0)) {
-#pragma unroll
-            for (int e = N - 1; e >= 0; --e)
-                if (v[e] == most) {
-                    best = (int)(first + e);
-                    best_x = most;
-                }
-        }
+        if (TOP) best = fmaxf(best, most);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const float y = v[e] - sum.m, p = __builtin_amdgcn_exp2f(y * kLog2E);
@@ -92,36 +84,31 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsArgs a) {
             if (c + u * kThreads < chunks) {
                 float v[8];
                 srv_floats<T>(raw[u], v);
-                take(v, 8 * (c + u * kThreads));
+                take(v);
             }
     }
     if (threadIdx.x < rest) {  // the odd end, an element a lane
         const float v[1] = {srv_load1(T, a.logits, at + 8 * (int64_t)chunks + threadIdx.x)};
-        take(v, 8 * chunks + threadIdx.x);
+        take(v);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum = join(sum, {__shfl_xor(sum.m, o), __shfl_xor(sum.s, o), __shfl_xor(sum.t, o)});
     if (lane == 0) wave_sums[wave] = sum;
     if constexpr (TOP) {
-        // the n-th of the lanes' best, 0 where there are fewer
-        const uint64_t key = best < 0 ? 0 : key_of(best_x, (uint32_t)best);
-        const uint32_t key_hi = (uint32_t)(key >> 32), key_lo = (uint32_t)key;
-        int before = 0;
-#pragma unroll 4
-        for (int j = 0; j < 64; ++j) {
-            const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)key_hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)key_lo, j);
-            before += other > key;
-        }
-        if (lane == 0) wave_key[wave] = 0;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (before == (int)a.top - 1 && key != 0) wave_key[wave] = key;
+        // the k-th largest of the lanes' best, bit by bit (that of a lane without elements is -inf)
+        const uint32_t key = (uint32_t)(key_of(best, 0) >> 32);
+        const int k = ((int)a.top + WAVES - 1) / WAVES;
+        uint32_t kth = 0;
+#pragma unroll
+        for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1)
+            if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= (kth | bit))) >= k) kth |= bit;
+        if (lane == 0) wave_key[wave] = (uint64_t)kth << 32;
         if (threadIdx.x == 0) count = 0;
     }
     __syncthreads();
-    sum = wave_sums[0];
+    sum = wave_sums[lane % WAVES];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) sum = join(sum, wave_sums[w]);
+    for (int o = 1; o < WAVES; o <<= 1) sum = join(sum, {__shfl_xor(sum.m, o), __shfl_xor(sum.s, o), __shfl_xor(sum.t, o)});
     const float log_s = logf(sum.s);
     const bool none = sum.s == 0.0f;  // no logit but -inf
     if (threadIdx.x == 0) {
@@ -136,11 +123,11 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsArgs a) {
     if constexpr (TOP) {
         uint64_t least = wave_key[0];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) least = max(least, wave_key[w]);
+        for (int w = 1; w < WAVES; ++w) least = min(least, wave_key[w]);
         const int n = (int)a.top;
         int found;
         for (;;) {
-            const float least_x = least == 0 ? -INFINITY : value_of(least);
+            const float least_x = value_of(least);
             auto offer = [&](float x, unsigned index) {
                 if (x >= least_x) {
                     const uint64_t key = key_of(x, index);
