@@ -5,15 +5,16 @@
 // c_g = z_g + 8 s_g,
 //   q . k_t  = sum_g s_tg (q_g . n_tg) + z_tg sum(q_g)
 //   out_d    = sum_t (p_t s_tg) (n_td - 8) + sum_t p_t c_tg,   g = d / 32
-// so the matrix cores multiply nibbles as f16 numbers, without a conversion.  Keys: a nibble
-// alone is a number with no bits but the lowest, n 2^-24 in bits 0 .. 3, n 2^-20 in bits
-// 4 .. 7: a shift and four masks for the eight of a word.  Values: or-ed into the lowest bits
-// of 1024 it is 1024 + n, four bits higher 1024 + 16 n, and a packed addition takes 1032 or
-// 1152 away.  The steps multiply the sums of a group (keys) or the weights (values), minima
-// and middles go beside in fp32.  (Values less 8 and the middles, not nibbles and minima: the
-// two sums would cancel each other, and the matrix cores round their sums towards zero.  f32
-// outputs were 5e-5 off that way at 448 tokens, f16 ones 5e-4 at 65536; a key's sum is of
-// one group and loses nothing to speak of.)
+// so the matrix cores multiply nibbles as f16 numbers, without a conversion: or-ed into the
+// lowest bits of 1024 a nibble is 1024 + n, four bits higher 1024 + 16 n, and a packed addition
+// takes 1032 or 1152 away.  For keys and 16-bit outputs it is left out: a nibble alone is a
+// number with no bits but the lowest, n 2^-24 in bits 0 .. 3, n 2^-20 in bits 4 .. 7, so a shift
+// and four masks do for the eight of a word.  The matrix cores align such products as if they were
+// 2^6 to 2^10 larger and lose bits below: f32 outputs were 2e-6 off at 448 tokens, 3e-7 with n - 8.
+// The steps multiply the sums of a group (keys) or the weights (values), minima and middles
+// go beside in fp32.  (Values less 8 and the middles, not nibbles and minima: the two sums
+// would cancel each other, and the matrix cores round their sums towards zero.  f32 outputs
+// were 5e-5 off that way at 448 tokens, f16 ones 5e-4 at 65536.)
 //
 // Four heads and four groups share the 16 rows or columns that a matrix instruction has, so
 // that with grouped heads of four none of them, and none of the work on what comes out,
@@ -137,6 +138,8 @@ __global__ __launch_bounds__(kThreads, per_cu(G, HQ, WIDE)) void paged_attention
     // The maximum that weights are relative to may fall behind by kBehind (in powers of two)
     // before sums are scaled.  kUp: base of the weights' exponent, their terms reach down to
     // 2^-34 of the largest (f32 outputs) or 2^-23 (and the maximum behind).
+    // kKeys: what a key's number is multiplied with for its nibble (less 8 where WIDE).
+    constexpr float kKeys = WIDE ? 1.0f : 0x1p24f;
     constexpr float kBehind = WIDE ? 4.0f : 8.0f, kUp = WIDE ? 10.0f : 6.0f;
 
     __shared__ __align__(16) int64_t row_off[kWaves][kTile];
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(kThreads, per_cu(G, HQ, WIDE)) void paged_attention
 #pragma unroll
             for (int o = 4; o < 64; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));  // over groups and c
             const float up = __uint_as_float((268u << 23) - most);
-            to_score[x] = a.scale * __uint_as_float((uint32_t)__shfl((int)most, c4) - (14u << 23)) * 0x1p24f;
+            to_score[x] = a.scale * __uint_as_float((uint32_t)__shfl((int)most, c4) - (14u << 23)) * kKeys;
 #pragma unroll
             for (int y = 0; y < GQ; ++y) {
                 float sum = 0.0f;
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(kThreads, per_cu(G, HQ, WIDE)) void paged_attention
                 sum += __shfl_xor(sum, 16);
                 sum += __shfl_xor(sum, 32);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q_sum[x][i][y] = __shfl(sum, 4 * c4 + i) * 0x1p-24f;  // (of column 4 c + i)
+                for (int i = 0; i < 4; ++i) q_sum[x][i][y] = __shfl(sum, 4 * c4 + i) / kKeys;  // (of column 4 c + i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float f = r % 2 ? 0x1p-4f : 1.0f;
@@ -329,7 +332,10 @@ __global__ __launch_bounds__(kThreads, per_cu(G, HQ, WIDE)) void paged_attention
                     for (int y = 0; y < GQ; ++y) sum[x][y] = floatx4{0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < G; ++w) {
-                    const srv_u32x4 n = nibbles(kr[h].w[w]);
+                    const uint32_t word = kr[h].w[w];
+                    const srv_u32x4 n = WIDE ? srv_u32x4{two_nibbles<0>(word, thousands), two_nibbles<4>(word, thousands), two_nibbles<0>(word >> 8, thousands),
+                                                         two_nibbles<4>(word >> 8, thousands)}
+                                             : nibbles(word);
 #pragma unroll
                     for (int x = 0; x < HQ; ++x)
 #pragma unroll
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(kThreads, per_cu(G, HQ, WIDE)) void paged_attention
 #pragma unroll
                     for (int y = 0; y < GQ; ++y) {
                         const uint32_t d = G % 4 == 0 || 4 * y + c4 < G ? km[h][y] : 0u;
-                        const float step = tml_half_bits(d & 0xFFFFu), least = tml_half_bits(d >> 16);
+                        const float step = tml_half_bits(d & 0xFFFFu), least = fmaf(step, WIDE ? 8.0f : 0.0f, tml_half_bits(d >> 16));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) by[i] = fmaf(sum[x][y][i], step, fmaf(q_sum[x][i][y], least, by[i]));
                     }
