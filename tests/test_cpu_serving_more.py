@@ -497,3 +497,9 @@ def test_refusals_logprobs(lanes):
     refusals(lanes, "token_logprobs", good, [
         (0, 3, INVALID_FORMAT), (1, -1, INVALID_SHAPE), (2, -1, INVALID_SHAPE), (8, -1, INVALID_SHAPE), (8, 65, INVALID_SHAPE), (2, 1 << 31, INVALID_SHAPE),
         (3, None, INVALID_ARG), (4, 7, INVALID_SHAPE), (5, None, INVALID_ARG), (6, None, INVALID_ARG), ((9, 10), (None, None), INVALID_ARG)])
+
+
+@pytest.mark.parametrize("q_t", [F32, F16, BF16], ids=tname)
+@pytest.mark.parametrize("dim,heads,kv", [(32, 5, 1), (64, 12, 2), (96, 17, 1), (128, 6, 1), (128, 16, 2), (160, 7, 1), (256, 9, 1)])
+def test_attention_q4_wide_groups(lanes, q_t, dim, heads, kv):
+    decode_program(lanes, None, q_t, [70, 0, 600], heads, kv, dim, 16, cus=2, cap=20.0 if dim == 128 else 0.0, slopes=dim == 64, seed=dim + heads)

@@ -266,3 +266,9 @@ def test_logprobs_more_candidates_than_are_held():
 def test_logprobs_many_rows():
     x = np.random.default_rng(5).standard_normal((1100, 9001))
     logprobs(BF16, x, 0, list(range(1100)))
+
+
+@pytest.mark.parametrize("q_t", [F32, F16, BF16], ids=tname)
+@pytest.mark.parametrize("dim,heads,kv", [(32, 5, 1), (64, 12, 2), (96, 17, 1), (128, 6, 1), (128, 16, 2), (160, 7, 1), (256, 9, 1)])
+def test_attention_q4_wide_groups(q_t, dim, heads, kv):
+    decode(None, q_t, [70, 0, 1600, 33], heads, kv, dim, 16, cap=20.0 if dim == 128 else 0.0, slopes=dim == 64, seed=dim + heads)

@@ -14,7 +14,9 @@
 //
 // A thread takes eight elements of a key and the same eight of its value, four threads
 // a group; rows pass through LDS so that memory is read and written in whole words
-// whatever the order in a row.  Bound by memory.
+// whatever the order in a row.  16384 tokens, 8 heads of 128, bf16, 88 MB: the store takes 29 us
+// (3.0 TB/s, bound by its instructions: some twenty an element, the group's extremes and the
+// rounding), the load 19 us (4.6 TB/s, memory).  Kernels by G: 61 us for both became 55.
 #include "serving.hpp"
 
 #include <algorithm>

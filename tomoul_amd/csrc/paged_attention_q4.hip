@@ -31,6 +31,13 @@
 // f32 q, and weights for f32 outputs, are two f16 terms each; q of 16 bits is exact in one, and
 // so are the weights rounded once where the output is of 16 bits: that adds to an f16 output
 // about what its own rounding does, to a bf16 one an eighth.
+//
+// Measured on MI355X (launches in a graph): bf16, 64 requests of up to 4096 tokens, 32 heads on 8
+// of 128 65 us (2.3 TB/s of the cache's 5 bits; in 16 bits 112 us), two of 40k to 65k tokens,
+// f16, 41 us (3.2 TB/s); one of 448 tokens, f32, 20 heads of 64, 9.5 us.  Memory does not bound it:
+// a tile of 4 KB is some 300 vector instructions of a wave, of which the nibbles of values are
+// 100 and the weights 60, and they take 0.5 us of a SIMD; loads two tiles ahead gained nothing
+// (41.3 for 39 us).  Short lists are bound by the chain of dependent loads and by the joining.
 #include "paged_split.hpp"
 #include "terms.hpp"
 
@@ -497,8 +504,14 @@ Status launch_join(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t
     return Status::Ok();
 }
 
-// Query heads taken at once: eight, or four where the registers end (and where there are no more).
-int heads_at_once(const PagedAttentionArgs &a) { return a.head_dim > 128 || a.q_heads / a.kv_heads <= 4 ? 4 : 8; }
+// Query heads taken at once: four, or eight where a group has more and the registers hold two
+// workgroups a CU.  32 requests of 2048 tokens, 64 heads on 8, eight / four at once: bf16, dim 128
+// 34.5 / 44.4 us, dim 64 27 / 34 us; f32 q, dim 64 30 / 31 us, dim 128 (one workgroup a CU) 44.8 /
+// 41.2 us.
+constexpr bool eights_fit(int groups, bool wide) { return groups <= (wide ? 2 : 4); }
+int heads_at_once(const PagedAttentionArgs &a) {
+    return a.q_heads / a.kv_heads > 4 && eights_fit((int)a.head_dim / 32, a.q_type == TML_TYPE_F32) ? 8 : 4;
+}
 AttnShape shape_of(const PagedAttentionArgs &a) {
     const int heads = heads_at_once(a);
     return shape_of(a, per_cu((int)a.head_dim / 32, heads / 4, a.q_type == TML_TYPE_F32), heads);
@@ -513,12 +526,13 @@ void launch_kernel(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t
 template <int G, int HQ>
 void launch_form(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
     const bool form = a.cap != 0.0f || a.slopes != nullptr;
-    if (a.q_type == TML_TYPE_F32) form ? launch_kernel<G, HQ, true, true>(a, sh, s) : launch_kernel<G, HQ, true, false>(a, sh, s);
-    else form ? launch_kernel<G, HQ, false, true>(a, sh, s) : launch_kernel<G, HQ, false, false>(a, sh, s);
+    if (a.q_type == TML_TYPE_F32) {
+        if constexpr (HQ == 1 || eights_fit(G, true)) form ? launch_kernel<G, HQ, true, true>(a, sh, s) : launch_kernel<G, HQ, true, false>(a, sh, s);
+    } else form ? launch_kernel<G, HQ, false, true>(a, sh, s) : launch_kernel<G, HQ, false, false>(a, sh, s);
 }
 template <int G>
 void launch_groups(const PagedAttentionArgs &a, const AttnShape &sh, hipStream_t s) {
-    if constexpr (G <= 4) {
+    if constexpr (eights_fit(G, false)) {
         if (sh.at_once == 8) return launch_form<G, 2>(a, sh, s);
     }
     launch_form<G, 1>(a, sh, s);

@@ -30,6 +30,14 @@
 // once, which adds to an output about what its own rounding does (2^-8 of bf16, 2^-11 of f16,
 // at most).
 // An f32 cache runs on the fp32 matrix cores.
+//
+// Measured on MI355X (launches in a graph): bf16, two causal prompts of 6000 to 8192 tokens, 32
+// heads on 8 of 128, 0.98 ms, 830 TFLOP/s of the pairs seen (a library product reaches 1130);
+// 1500 frames, 20 heads of 64, f16, 32 us; sixteen chunks of 1 to 256 tokens over contexts to 4096,
+// capped, 170 us.  The first is bound by issue: without the exponentials it took 918, without the
+// second product 722, without the copies 713 of 970 us, so a SIMD's two waves hardly overlap
+// their products with each other's exponentials.  The others are bound by their longest workgroups (66 tiles of
+// 2.5 us): a request's tokens are not split.
 #include "terms.hpp"
 
 #include <algorithm>
