@@ -547,7 +547,7 @@ int tml_hip_kv_load_q4_dev(int type, int64_t tokens, int64_t kv_heads, int64_t h
  *   q, out   F32, F16 or BF16
  * Arithmetic: products and sums are fp32, of the nibbles as they are, of q (f32: two f16
  * terms, 2^-22 of each element; 16 bits: exact; both but for 2^-35 of its head's largest or of
- * 2^-100) and of the weights times the values' steps (f32: two f16 terms, 2^-22 of each, 2^-38
+ * 2^-100) and of the weights times the values' steps (f32: two f16 terms, 2^-22 of each, 2^-34
  * of the largest step's; 16 bits: one, 2^-11 of each, 2^-23 of the largest step's).
  * An infinite or NaN element of q makes its head's outputs NaN. */
 int tml_hip_paged_attention_q4_dev(int q_type, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,

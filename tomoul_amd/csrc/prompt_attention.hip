@@ -176,7 +176,7 @@ __device__ __forceinline__ void one_row(const PromptAttentionArgs &a, const Prom
         for (int j = 0; j < 64 && t0 + j < high; ++j) {
             const float w = __shfl(p, j);
             const int64_t from = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(off >> 32), j) << 32) | (uint32_t)__shfl((int)(uint32_t)off, j));
-            if (from < 0 || w == 0.0f) continue;
+            if (from < 0) continue;  // (a weight of 0 keeps an infinity: NaN)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
                 if (lane + 64 * x < D) out[x] = fmaf(w, srv_load1(CT, a.v_cache, from + lane + 64 * x), out[x]);
