@@ -129,9 +129,11 @@ struct Prompt {
     static constexpr int kOwn = BN / kWaves;                 // tokens that a wave copies
     static constexpr int kCopies = kOwn * KP / 64;
     static constexpr int kQ = kF32 ? DP / 8 : DP / 16;       // 16 bytes of q a lane, each term
-    // registers of a lane: q, output, scores and weights; two workgroups a CU where they leave room
-    static constexpr int kRegs = 4 * kQ * NQ + DP / 2 + BN / 2 + BN / 4 * NP;
-    static constexpr bool kTwo = kRegs <= 160;               // two waves of a SIMD
+    // Two workgroups a CU, two waves of a SIMD, or one with all of the registers.  Two / one, two causal
+    // prompts of 4096 tokens: bf16, 32 heads on 8 of 128 399 / 539 us; f32 q on f16 597 / 834, on
+    // bf16 840 / 971; 16 heads on 8 of 256, bf16 653 / 504; f32 cache, 2048 tokens, 16 on 8 of 128
+    // 657 / 448, 20 of 64 335 / 322.
+    static constexpr bool kTwo = !kF32 && DP <= 128;
     static constexpr int kTile = BN * KP;                    // pieces of a tile's keys
 };
 
