@@ -128,10 +128,12 @@ __device__ __forceinline__ Words<(N + 3) / 4> load_bytes(const char *p) {
     return r;
 }
 
-// Workgroups on a CU, as the registers allow.  (16-bit q, dim 128, groups of four heads: three against
-// two 64 against 70 us for 64 requests of up to 4096 tokens, 40.6 against 39 for two of up to 65536;
-// four spill: 102 and 66.)
-constexpr int per_cu(int groups, int fours, bool wide) { return wide ? (groups * fours > 4 ? 1 : 2) : (groups * fours > 4 || fours > 1 ? 2 : 3); }
+// Workgroups on a CU: three where the registers hold them, else two.  Three / two, bf16, 32 heads on 8
+// of 128: 64 ragged requests of up to 4096 tokens 64 / 70 us, of up to 2048 42 / 47 us, one of 60000
+// 35 / 31 us, 32 of 2048 alike 30 / 25 us (a list is half a workgroup's share there); over
+// eighteen batches two took 1.02 times as long.  Four spill: 102 us for the first.  Where two spill:
+// two / one, f32, 64 of 1000 tokens, 32 heads on 8 of 192, 34 / 45 us.
+constexpr int per_cu(int groups, int fours, bool wide) { return wide || groups * fours > 4 || fours > 1 ? 2 : 3; }
 
 // G: groups of a head.  HQ: heads taken at once, in fours.  WIDE: q and the output are f32.  FORM:
 // the scores are capped or biased.
