@@ -338,3 +338,55 @@ def test_store_of_many_rows():
         want = np.full((n_blocks * block, kv, row), 0xEE, np.uint8)
         want[slots.cpu().numpy()] = ref.pack_rows(values(x.cpu().numpy().reshape(tokens, kv, dim), F32))[w]
         assert np.array_equal(caches[0][w].cpu().numpy().reshape(want.shape), want)
+
+
+def test_offsets_past_32_bits():
+    """Caches of over 4 GiB, the requests' blocks at both ends: bit for bit what small caches with the same rows give."""
+    import torch
+    kv, dim, heads, block, lens = 2, 128, 8, 16, [700, 33, 64]
+    row = ref.row_bytes(dim)
+    tokens, need = sum(lens), sum(-(-n // block) for n in lens)
+    width = 64
+    g = torch.Generator().manual_seed(9)
+    k, v = (torch.randn(tokens, kv * dim, generator=g).bfloat16().cuda() for _ in range(2))
+    q = torch.randn(tokens, heads * dim, generator=g).bfloat16().cuda()
+    start = torch.tensor([0, 700, 733, 797], dtype=torch.int32, device="cuda")
+    seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    results = []
+    for large in (False, True):
+        out = []
+        for four in (False, True):
+            size = block * kv * (row if four else 2 * dim)
+            n_blocks = (5 << 30) // size if large else need
+            caches = [torch.empty(n_blocks * size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+            blocks = [i if i % 3 == 0 else n_blocks - need + i for i in range(need)] if large else list(range(need))
+            table = torch.full((3, width), -1, dtype=torch.int32)
+            slots, at = [], 0
+            for r, n in enumerate(lens):
+                for i in range(-(-n // block)):
+                    table[r, i] = blocks[at]
+                    slots += [blocks[at] * block + t for t in range(min(block, n - i * block))]
+                    at += 1
+            table, slots = table.cuda(), torch.tensor(slots, dtype=torch.int64).cuda()
+            strides = (size, kv * row, row) if four else (block * kv * dim, kv * dim, dim)
+            pointers = [c.data_ptr() for c in caches]
+            rest = (table.data_ptr(), width, width, seq.data_ptr(), SCALE)
+            o = torch.zeros(3, heads * dim, dtype=torch.bfloat16, device="cuda")
+            if four:
+                _abi.kv_store_q4_dev(BF16, tokens, kv, dim, k.data_ptr(), v.data_ptr(), kv * dim, kv * dim, slots.data_ptr(), *pointers, n_blocks, block, *strides)
+                _abi.paged_attention_q4_dev(BF16, 3, heads, kv, dim, q.data_ptr(), heads * dim, *pointers, n_blocks, block, *strides, *rest, o.data_ptr(), heads * dim)
+                back = [torch.zeros_like(k) for _ in range(2)]
+                _abi.kv_load_q4_dev(BF16, tokens, kv, dim, *pointers, n_blocks, block, *strides, slots.data_ptr(), *(x.data_ptr() for x in back), kv * dim, kv * dim)
+                out += [o, *back]
+            else:
+                _abi.kv_store_dev(BF16, BF16, tokens, kv, dim, k.data_ptr(), v.data_ptr(), kv * dim, kv * dim, slots.data_ptr(), *pointers, n_blocks, block, *strides)
+                _abi.paged_attention_ex_dev(BF16, BF16, 3, heads, kv, dim, q.data_ptr(), heads * dim, *pointers, n_blocks, block, *strides, *rest, o.data_ptr(), heads * dim, cap=CAP)
+                p = torch.zeros_like(q)
+                _abi.prompt_attention_dev(BF16, BF16, tokens, 3, heads, kv, dim, q.data_ptr(), heads * dim, *pointers, n_blocks, block, *strides, table.data_ptr(), width, width,
+                                          start.data_ptr(), seq.data_ptr(), SCALE, p.data_ptr(), heads * dim)
+                out += [o, p]
+            torch.cuda.synchronize()
+            del caches
+        results.append(out)
+    for a, b in zip(*results):
+        assert torch.isfinite(a.float()).all() and torch.equal(a, b)
