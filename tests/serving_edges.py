@@ -1,0 +1,146 @@
+"""Calls at the edges of the operators around prompts and 4-bit caches, written once for the CPU build
+(tests/cpu_emu/lanes.py) and for the GPU (`GpuProgram`): `program` is a class of either.
+
+Tolerances are those of serving_ref.attention, derived there, but for caps: cap * tanh(x / cap) is
+off by 6 u of the smaller of the cap and 3 |x| (a series below |x / cap| = 0.35), not of the cap.
+Outputs of 16 bits of prompts may use a form that is 12 u of the cap off where that is an eighth of
+their weights' own rounding at most.
+"""
+import numpy as np
+
+import serving_ref as ref
+from serving_ref import BF16, F16, F32, HALF_ULP, STORED, TINY, close, stored, values
+from test_cpu_serving_more import Cache, rows_back, rows_of
+
+COMBOS = [(F32, F32), (F32, F16), (F16, F16), (F32, BF16), (BF16, BF16)]
+
+
+class GpuProgram:
+    """lanes.Program's interface on the GPU: calls run as they are made."""
+
+    def __init__(self, cus=None, reverse=False):
+        self.buffers, self.shapes, self.codes, self.messages = [], [], [], []
+
+    def buf(self, array):
+        import torch
+        a = np.ascontiguousarray(array)
+        self.buffers.append(torch.from_numpy(a.reshape(-1).view(np.uint8).copy()).cuda())
+        self.shapes.append((a.dtype, a.shape))
+        return len(self.buffers) - 1
+
+    def call(self, name, *args):
+        from tomoul_amd import _abi
+        given = [self.buffers[a[1]].data_ptr() + (a[2] if len(a) > 2 else 0) if isinstance(a, tuple) else a for a in args]
+        self.codes.append(getattr(_abi.lib(), f"tml_hip_{name}_dev")(*given))
+        self.messages.append("")
+
+    def run(self):
+        import torch
+        torch.cuda.synchronize()
+        return [b.cpu().numpy().view(t).reshape(shape) for b, (t, shape) in zip(self.buffers, self.shapes)]
+
+
+def expected(q, keys, vals, pos, cap, weight, **kw):
+    """serving_ref.attention with the cap's tolerance as above."""
+    if not cap:
+        return ref.attention(q, keys, vals, pos, weight=weight, **kw)
+    want, wide = ref.attention(q, keys, vals, pos, cap=cap, weight=weight, **kw)
+    with np.errstate(invalid="ignore"):  # the largest score without the cap
+        x = max([np.abs(keys[:, h // (q.shape[1] // keys.shape[1])] @ q[:, h].T).max(initial=0) for h in range(q.shape[1])]) * abs(kw["scale"])
+    if not cap > 3 * x:
+        return want, wide
+    # (6 u of 3 |x| is 18 u |x|; the tolerance without a cap has 2 u |s| of it)
+    _, tol = ref.attention(q, keys, vals, pos, weight=weight + 36 * ref.U * x, **kw)
+    return want, tol
+
+
+def prompt(program, q_t, cache_t, both, heads, kv, dim, block, layout="thd", prefix=None, window=0, cap=0.0, slopes=False, scale=None, pad=2, lost=(), odd=(),
+           odd_q=(), seed=0, cus=256, reverse=False, loud=1.5, lens=None):
+    """both: (context, new tokens) of each request; odd_q: (row, element, number) of q; lens: of the caches, where not their sums."""
+    rng = np.random.default_rng(seed)
+    lens = [c + n for c, n in both] if lens is None else lens
+    cache = Cache(rng, cache_t, lens, kv, dim, block, layout, 0, lost)
+    cache.put(odd)
+    starts = np.concatenate([[0], np.cumsum([n for _, n in both])]).astype(np.int32)
+    tokens = int(starts[-1]) + pad
+    q = stored(loud * rng.standard_normal((tokens, heads * dim)), q_t)
+    for row, d, x in odd_q:
+        q[row, d] = stored(np.array([x]), q_t)[0]
+    sl = (2.0 ** -rng.uniform(0, 8, heads)).astype(np.float32) if slopes else None
+    qs, os_ = heads * dim + 3, heads * dim + 1
+    scale = float(np.float32(1 / np.sqrt(dim) if scale is None else scale))
+    p = program(cus, reverse)
+    bq, bo = p.buf(rows_of(q, qs, STORED[q_t](1))), p.buf(np.full((tokens - 1) * os_ + heads * dim, 7, STORED[q_t]))
+    bk, bv, bt = p.buf(cache.bytes[0]), p.buf(cache.bytes[1]), p.buf(cache.table)
+    bl, bs = p.buf(np.array(lens, np.int32)), p.buf(starts)
+    bp = p.buf(np.array(prefix, np.int32)) if prefix is not None else None
+    bsl = p.buf(sl) if slopes else None
+    p.call("prompt_attention", q_t, cache_t, tokens, len(both), heads, kv, dim, ("b", bq), qs, ("b", bk), ("b", bv), cache.n_blocks, block, *cache.strides,
+           ("b", bt), cache.width, cache.width, ("b", bs), ("b", bl), None if bp is None else ("b", bp), window, scale, cap, ("b", bsl) if slopes else None,
+           ("b", bo), os_, None)
+    got = p.run()
+    assert p.codes == [0], p.messages
+    out = rows_back(got[bo], tokens, heads * dim, os_)
+    for r in range(tokens - 1):
+        assert (got[bo][r * os_ + heads * dim:(r + 1) * os_] == 7).all()
+    assert (out[starts[-1]:] == 7).all()
+    weight = 2.0 ** -20 if q_t == F32 else HALF_ULP[q_t] * (1.125 if cap else 1.0)
+    for r, (_, n) in enumerate(both):
+        if n == 0:
+            continue
+        pos = np.arange(lens[r] - n, lens[r])
+        t, k, v, _, _ = cache.of(r, lens[r])
+        want, tol = expected(values(q[starts[r]:starts[r + 1]], q_t).reshape(n, heads, dim), k, v, pos, cap, weight, scale=scale, slopes=sl,
+                             seen=ref.sees(pos, t, prefix[r] if prefix else 0, window), positions=t)
+        mine = values(out[starts[r]:starts[r + 1]], q_t).reshape(want.shape)
+        mine = np.where(np.isinf(want) & ~np.isfinite(mine), want, mine)  # (an infinite value's element is infinite or NaN)
+        close(mine, want, tol + HALF_ULP[q_t] * (np.abs(want) + tol) + TINY[q_t], f"request {r}")
+
+
+def decode(program, q_t, cache_t, lens, heads, kv, dim, block, cap=0.0, slopes=False, scale=None, odd=(), odd_q=(), seed=0, cus=256, loud=1.5, window=0, spoil=()):
+    """One new token a request; cache_t None: in 4 bits.  spoil: (request, position, key or value, head, group) whose group is NaN."""
+    rng = np.random.default_rng(seed)
+    cache = Cache(rng, cache_t, lens, kv, dim, block, "thd", window)
+    cache.put(odd)
+    for r, pos, w, h, g in spoil:
+        page, at = cache.table[r, pos // block], pos % block
+        cache.values[w][page, at, h, 32 * g:32 * g + 32] = np.nan
+        b, tk, hd = cache.strides
+        word = page * b + at * tk + h * hd + dim // 2 + 4 * g
+        cache.bytes[w][word:word + 4] = np.frombuffer(np.uint32(0x7E000000).tobytes(), np.uint8)
+    batch = len(lens)
+    q = stored(loud * rng.standard_normal((batch, heads * dim)), q_t)
+    for row, d, x in odd_q:
+        q[row, d] = stored(np.array([x]), q_t)[0]
+    sl = (2.0 ** -rng.uniform(0, 8, heads)).astype(np.float32) if slopes else None
+    scale = float(np.float32(1 / np.sqrt(dim) if scale is None else scale))
+    p = program(cus)
+    bq, bo = p.buf(q), p.buf(np.full((batch, heads * dim), 7, STORED[q_t]))
+    bk, bv, bt, bl = p.buf(cache.bytes[0]), p.buf(cache.bytes[1]), p.buf(cache.table), p.buf(np.array(lens, np.int32))
+    bs = p.buf(sl) if slopes else None
+    p.call("paged_attention_q4" if cache_t is None else "paged_attention_ex", *((q_t,) if cache_t is None else (q_t, cache_t)), batch, heads, kv, dim, ("b", bq),
+           heads * dim, ("b", bk), ("b", bv), cache.n_blocks, block, *cache.strides, ("b", bt), cache.width, cache.width, ("b", bl), window, scale, cap,
+           ("b", bs) if slopes else None, ("b", bo), heads * dim, None)
+    got = p.run()
+    assert p.codes == [0], p.messages
+    weight = 2.0 ** -16 if cache_t == BF16 and q_t == BF16 else 2.0 ** -11 if cache_t is None and q_t != F32 else 2.0 ** -20
+    for r, length in enumerate(lens):
+        pos = np.array([length - 1])
+        t, k, v, km, vm = cache.of(r, length)
+        want, tol = expected(values(q[r], q_t).reshape(1, heads, dim), k, v, pos, cap, weight, scale=scale, slopes=sl, seen=ref.sees(pos, t, 0, window),
+                             positions=t, key_mag=km, val_mag=vm)
+        close(values(got[bo][r], q_t).reshape(want[0].shape), want[0], tol[0] + HALF_ULP[q_t] * (np.abs(want[0]) + tol[0]) + TINY[q_t], f"request {r}")
+
+
+# ------------------------------------------------------------------------ caps
+CAPS = [2.0 ** -100, 0.5, 60.0, 65.0, 400.0, 600.0, 1e4, 1e6, 1e9, 2.0 ** 100]
+
+
+def prompt_caps(program, q_t, cache_t, cap):
+    prompt(program, q_t, cache_t, [(20, 50), (0, 3)], 4, 2, 64, 16, cap=cap, seed=11)
+    # (loud scores: some reach the caps of the middle)
+    prompt(program, q_t, cache_t, [(5, 30)], 2, 1, 40, 8, cap=cap, slopes=True, loud=30.0, seed=12)
+
+
+def decode_caps(program, q_t, cache_t, cap):
+    decode(program, q_t, cache_t, [70, 3, 0], 4, 2, 64, 16, cap=cap, seed=14)

@@ -1,0 +1,40 @@
+"""The edges of the operators around prompts and 4-bit caches on the CPU, lane by lane
+(tests/cpu_emu/lanes.py): the calls and tolerances of tests/serving_edges.py.
+CPU only; needs /opt/rocm/llvm/bin/clang++ and an x86-64 (skipped without them)."""
+import os
+import platform
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+sys.path.insert(0, HERE)
+import serving_edges as edges  # noqa: E402
+from serving_ref import BF16, F16, F32, tname  # noqa: E402
+
+CLANG = "/opt/rocm/llvm/bin/clang++"
+pytestmark = pytest.mark.skipif(not os.path.exists(CLANG) or platform.machine() != "x86_64", reason="no clang++ for the CPU build, or not x86-64")
+
+
+@pytest.fixture(scope="module")
+def program():
+    sys.path.insert(0, os.path.join(HERE, "cpu_emu"))
+    import lanes  # tests/cpu_emu/lanes.py
+    lanes.build()
+    return lanes.Program
+
+
+combos = pytest.mark.parametrize("q_t,cache_t", edges.COMBOS, ids=tname)
+decodes = pytest.mark.parametrize("q_t,cache_t", [*edges.COMBOS, (F32, None), (F16, None), (BF16, None)], ids=tname)
+
+
+@combos
+@pytest.mark.parametrize("cap", edges.CAPS)
+def test_prompt_caps(program, q_t, cache_t, cap):
+    edges.prompt_caps(program, q_t, cache_t, cap)
+
+
+@decodes
+@pytest.mark.parametrize("cap", edges.CAPS)
+def test_decode_caps(program, q_t, cache_t, cap):
+    edges.decode_caps(program, q_t, cache_t, cap)

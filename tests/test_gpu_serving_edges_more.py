@@ -1,0 +1,34 @@
+"""The edges of the operators around prompts and 4-bit caches on the GPU: the calls and
+tolerances of tests/serving_edges.py."""
+import os
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+sys.path.insert(0, HERE)
+import serving_edges as edges  # noqa: E402
+from serving_ref import BF16, F16, F32, tname  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+combos = pytest.mark.parametrize("q_t,cache_t", edges.COMBOS, ids=tname)
+decodes = pytest.mark.parametrize("q_t,cache_t", [*edges.COMBOS, (F32, None), (F16, None), (BF16, None)], ids=tname)
+
+
+@pytest.fixture(scope="module")
+def program():
+    from tomoul_amd import _abi
+    _abi.init()
+    return edges.GpuProgram
+
+
+@combos
+@pytest.mark.parametrize("cap", edges.CAPS)
+def test_prompt_caps(program, q_t, cache_t, cap):
+    edges.prompt_caps(program, q_t, cache_t, cap)
+
+
+@decodes
+@pytest.mark.parametrize("cap", edges.CAPS)
+def test_decode_caps(program, q_t, cache_t, cap):
+    edges.decode_caps(program, q_t, cache_t, cap)

@@ -202,6 +202,11 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
     // (f32 outputs) or 2^-24 (one term, and the maximum behind) of the largest.
     constexpr float kBehind = QT == TML_TYPE_F32 ? 0.0f : 8.0f;
     constexpr float kUp = CT != TML_TYPE_F16 ? 0.0f : QT == TML_TYPE_F32 ? 14.0f : 7.0f;
+    // A cap as cap - 2 cap / (1 + e^(2 x / cap)) is up to 12 2^-24 of the CAP off, whatever x is, and
+    // as much of a weight.  It is for 16-bit weights and caps up to this, where that is a tenth of what
+    // the weights' rounding is off; past it the cap is cap_score's (two f16 prompts of 4096 tokens, 32 heads
+    // on 8 of 128: 439 us up to this, 530 past it).
+    constexpr float kShortCap = QT == TML_TYPE_F32 ? 0.0f : QT == TML_TYPE_F16 ? 64.0f : 512.0f;
 
     // (arrays of their own: the compiler waits for copies to the array that it reads)
     __shared__ srv_u32x4 lds_k0[TEAMS * C::kTile], lds_k1[TEAMS * C::kTile], lds_v0[TEAMS * C::kTile], lds_v1[TEAMS * C::kTile];
@@ -318,10 +323,11 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
             if (a.scale == 0.0f) q[n][c] = srv_u32x4{0, 0, 0, 0};
         }
     const float to_log2 = to_score * kLog2E;
-    float slope = 0.0f, inv_cap = 0.0f;
+    float slope = 0.0f, inv_cap = 0.0f, short_cap = 0.0f;
     if constexpr (FORM) {
         if (a.slopes != nullptr) slope = a.slopes[head] * kLog2E;
         if (a.cap != 0.0f) inv_cap = 1.0f / a.cap;
+        if (a.cap <= kShortCap) short_cap = 2.0f * to_log2 * inv_cap;  // (16 bits: of the scale and the cap alone)
     }
 
     float m = -INFINITY, l = 0.0f;  // of this lane's row; l over this lane's tokens alone
@@ -478,16 +484,15 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
         const uint64_t live = lds_live[it & 1][team];
         const bool whole = k0 + BN <= high_of(wave_first) && k0 >= low_of(wave_last) && (live & (~0ull >> (64 - BN))) == ~0ull >> (64 - BN);
         if constexpr (FORM) {
-            if (inv_cap != 0.0f) {
+            if (QT != TML_TYPE_F32 && short_cap > 0.0f) {
 #pragma unroll
                 for (int i = 0; i < BN / 2; ++i) {
-                    if constexpr (QT == TML_TYPE_F32) {
-                        s[i] = cap_score(s[i] * to_score, a.cap, inv_cap) * kLog2E;
-                    } else {  // cap - 2 cap / (1 + e^(2 x / cap)): 2^-23 of the cap off, next to 16-bit weights
-                        const float e = __builtin_amdgcn_exp2f(s[i] * (2.0f * to_log2 * inv_cap));
-                        s[i] = fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * kLog2E * a.cap, kLog2E * a.cap);
-                    }
+                    const float e = __builtin_amdgcn_exp2f(s[i] * short_cap);
+                    s[i] = fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * kLog2E * a.cap, kLog2E * a.cap);
                 }
+            } else if (inv_cap != 0.0f) {
+#pragma unroll
+                for (int i = 0; i < BN / 2; ++i) s[i] = cap_score(s[i] * to_score, a.cap, inv_cap) * kLog2E;
             } else {
 #pragma unroll
                 for (int i = 0; i < BN / 2; ++i) s[i] *= to_log2;
