@@ -142,5 +142,10 @@ def prompt_caps(program, q_t, cache_t, cap):
     prompt(program, q_t, cache_t, [(5, 30)], 2, 1, 40, 8, cap=cap, slopes=True, loud=30.0, seed=12)
 
 
+def prompt_cap_of_large_scale(program, q_t, cache_t):
+    """scale / cap is no number here; a product of 0 is a score of 0 all the same."""
+    prompt(program, q_t, cache_t, [(5, 30)], 2, 1, 64, 8, cap=2.0 ** -100, scale=2.0 ** 40, odd_q=[(3, d, 0.0) for d in range(64)], seed=13)
+
+
 def decode_caps(program, q_t, cache_t, cap):
     decode(program, q_t, cache_t, [70, 3, 0], 4, 2, 64, 16, cap=cap, seed=14)

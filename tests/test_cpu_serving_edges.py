@@ -34,6 +34,11 @@ def test_prompt_caps(program, q_t, cache_t, cap):
     edges.prompt_caps(program, q_t, cache_t, cap)
 
 
+@combos
+def test_prompt_cap_of_large_scale(program, q_t, cache_t):
+    edges.prompt_cap_of_large_scale(program, q_t, cache_t)
+
+
 @decodes
 @pytest.mark.parametrize("cap", edges.CAPS)
 def test_decode_caps(program, q_t, cache_t, cap):

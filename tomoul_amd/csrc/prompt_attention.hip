@@ -484,7 +484,7 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
         const uint64_t live = lds_live[it & 1][team];
         const bool whole = k0 + BN <= high_of(wave_first) && k0 >= low_of(wave_last) && (live & (~0ull >> (64 - BN))) == ~0ull >> (64 - BN);
         if constexpr (FORM) {
-            if (QT != TML_TYPE_F32 && short_cap > 0.0f) {
+            if (QT != TML_TYPE_F32 && short_cap > 0.0f && short_cap < INFINITY) {
 #pragma unroll
                 for (int i = 0; i < BN / 2; ++i) {
                     const float e = __builtin_amdgcn_exp2f(s[i] * short_cap);
