@@ -91,7 +91,7 @@ def prompt(program, q_t, cache_t, both, heads, kv, dim, block, layout="thd", pre
         pos = np.arange(lens[r] - n, lens[r])
         t, k, v, _, _ = cache.of(r, lens[r])
         want, tol = expected(values(q[starts[r]:starts[r + 1]], q_t).reshape(n, heads, dim), k, v, pos, cap, weight, scale=scale, slopes=sl,
-                             seen=ref.sees(pos, t, prefix[r] if prefix else 0, window), positions=t)
+                             seen=ref.sees(pos, t, prefix[r] if prefix else 0, window if window < 1 << 62 else 0), positions=t)
         mine = values(out[starts[r]:starts[r + 1]], q_t).reshape(want.shape)
         mine = np.where(np.isinf(want) & ~np.isfinite(mine), want, mine)  # (an infinite value's element is infinite or NaN)
         close(mine, want, tol + HALF_ULP[q_t] * (np.abs(want) + tol) + TINY[q_t], f"request {r}")
@@ -149,3 +149,13 @@ def prompt_cap_of_large_scale(program, q_t, cache_t):
 
 def decode_caps(program, q_t, cache_t, cap):
     decode(program, q_t, cache_t, [70, 3, 0], 4, 2, 64, 16, cap=cap, seed=14)
+
+
+# ------------------------------------------------- more new tokens than the cache has
+def prompt_before_the_cache(program, q_t, cache_t, window):
+    """Tokens that stand before position 0 see the prefix all the same, as one sequence attends to another's cache."""
+    prompt(program, q_t, cache_t, [(0, 30), (0, 12)], 4, 2, 64, 16, lens=[9, 40], prefix=[9, 20], window=window, seed=21)
+    prompt(program, q_t, cache_t, [(0, 150)], 2, 1, 40, 8, lens=[70], prefix=[50], window=window, slopes=True, seed=22)
+
+
+WINDOWS = [0, 5, 60, 70, 1 << 31, 1 << 40, (1 << 63) - 1]

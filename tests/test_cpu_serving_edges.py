@@ -43,3 +43,9 @@ def test_prompt_cap_of_large_scale(program, q_t, cache_t):
 @pytest.mark.parametrize("cap", edges.CAPS)
 def test_decode_caps(program, q_t, cache_t, cap):
     edges.decode_caps(program, q_t, cache_t, cap)
+
+
+@combos
+@pytest.mark.parametrize("window", edges.WINDOWS)
+def test_prompt_before_the_cache(program, q_t, cache_t, window):
+    edges.prompt_before_the_cache(program, q_t, cache_t, window)

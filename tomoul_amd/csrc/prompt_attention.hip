@@ -755,6 +755,7 @@ Status launch_prompt_attention(const PromptAttentionArgs &in, hipStream_t s) {
     PromptShape sh;
     sh.group = (int)(a.q_heads / a.kv_heads);
     sh.positions = a.table_width * a.block_size;
+    if (a.window >= sh.positions) a.window = 0;  // (all of the cache; and pos - window stays a number)
     const int64_t tiles = a.tokens * sh.group / kRows + std::min(a.requests, a.tokens);
     if (tiles * a.kv_heads > (1 << 23))
         return Status::Err(TML_ERR_INVALID_SHAPE, "prompt attention: tokens * heads / 128 + requests * key-value heads must be at most 2^23");
