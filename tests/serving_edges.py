@@ -159,3 +159,32 @@ def prompt_before_the_cache(program, q_t, cache_t, window):
 
 
 WINDOWS = [0, 5, 60, 70, 1 << 31, 1 << 40, (1 << 63) - 1]
+
+
+# --------------------------------------------------------- infinities and NaN
+def sprinkled(rng, lens, kv, dim, what, share, kinds):
+    """Odd numbers at a share of the elements of keys (0) or values (1)."""
+    odd = []
+    for r, n in enumerate(lens):
+        for _ in range(max(1, int(share * n))):
+            odd.append((r, int(rng.integers(n)), what, int(rng.integers(kv)), int(rng.integers(dim)), float(rng.choice(kinds))))
+    return odd
+
+
+ODD_MASKS = [dict(), dict(window=30), dict(prefix=[110, 0, 64]), dict(window=45, prefix=[130, 70, 0], cap=20.0), dict(slopes=True, lost=[(0, 2, -1), (0, 6, 1 << 30)])]
+
+
+def prompt_odd_values(program, q_t, cache_t, dim, mask, cus=256):
+    """Infinite and NaN values reach those who see them and no one else, few and many of them, at the tiles' ends too."""
+    both, inf, nan = [(60, 90), (0, 70), (130, 3)], np.inf, np.nan
+    lens = [c + n for c, n in both]
+    rng = np.random.default_rng(dim)
+    for share in (0.02, 0.5):
+        odd = sprinkled(rng, lens, 2, dim, 1, share, [inf, -inf, nan])
+        odd += [(0, p, 1, 0, dim - 1, inf) for p in (63, 64, 127, 128, 149)] + [(1, 69, 1, 1, 0, nan)]
+        # (a page that is no block of the cache holds no values)
+        odd = [o for o in odd if (o[0], o[1] // 16) not in [(r, i) for r, i, _ in mask.get("lost", ())]]
+        prompt(program, q_t, cache_t, both, 4, 2, dim, 16, odd=odd, seed=31, cus=cus, **mask)
+    # (one head's rows: a workgroup of 128 tokens, whose first and last see tiles far apart)
+    prompt(program, q_t, cache_t, [(300, 140)], 1, 1, dim, 32, odd=sprinkled(rng, [440], 1, dim, 1, 0.05, [inf, -inf, nan]), window=mask.get("window", 0), seed=32, cus=cus)
+

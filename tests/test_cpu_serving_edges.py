@@ -49,3 +49,10 @@ def test_decode_caps(program, q_t, cache_t, cap):
 @pytest.mark.parametrize("window", edges.WINDOWS)
 def test_prompt_before_the_cache(program, q_t, cache_t, window):
     edges.prompt_before_the_cache(program, q_t, cache_t, window)
+
+
+@combos
+@pytest.mark.parametrize("dim", [40])
+@pytest.mark.parametrize("mask", edges.ODD_MASKS, ids=lambda m: "-".join(m) or "causal")
+def test_prompt_odd_values(program, q_t, cache_t, dim, mask):
+    edges.prompt_odd_values(program, q_t, cache_t, dim, mask, cus=1 if "window" in mask else 256)

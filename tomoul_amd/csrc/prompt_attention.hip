@@ -143,53 +143,6 @@ __device__ __forceinline__ void wait_copies() {
     __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | 0x7 << 4 | 0xF << 8);
 }
 
-// One row by a wave, in fp32 from end to end: a lane a token for the scores, a lane a d for the
-// values.  For the few rows beside which values are infinite or NaN where they may not look.
-template <int CT, int QT>
-__device__ __forceinline__ void one_row(const PromptAttentionArgs &a, const PromptShape &sh, int64_t b, int64_t len, int64_t q_row, int64_t head, int64_t pos,
-                                                  int64_t prefix, int64_t kv) {
-    const int lane = threadIdx.x & 63, D = (int)a.head_dim;
-    const int64_t low = a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0, high = min(max(pos + 1, prefix), len);
-    const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
-    auto row_of = [&](int64_t t) {  // element of the caches, or -1
-        const int block = a.block_table[b * a.table_stride + (uint32_t)t / (uint32_t)a.block_size];
-        if (block < 0 || block >= a.n_blocks) return (int64_t)-1;
-        return block * a.block_stride + (int64_t)((uint32_t)t % (uint32_t)a.block_size) * a.token_stride + kv * a.head_stride;
-    };
-    auto score_of = [&](int64_t t, int64_t off) {
-        float x = 0.0f;
-        for (int d = 0; d < D; ++d) x = fmaf(srv_load1(QT, a.q, q_row * a.q_stride + head * D + d), srv_load1(CT, a.k_cache, off + d), x);
-        x *= a.scale;
-        if (a.cap != 0.0f) x = cap_score(x, a.cap, 1.0f / a.cap);
-        return (x - slope * fabsf((float)(pos - t))) * kLog2E;
-    };
-    float m = -INFINITY;
-    for (int64_t t = low + lane; t < high; t += 64) {
-        const int64_t off = row_of(t);
-        if (off >= 0) m = fmaxf(m, score_of(t, off));
-    }
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if (m == -INFINITY) m = 0.0f;
-    float l = 0.0f, out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t t0 = low; t0 < high; t0 += 64) {
-        const int64_t t = t0 + lane, off = t < high ? row_of(t) : -1;
-        const float p = off >= 0 ? __builtin_amdgcn_exp2f(score_of(t, off) - m) : 0.0f;
-        l += p;
-        for (int j = 0; j < 64 && t0 + j < high; ++j) {
-            const float w = __shfl(p, j);
-            const int64_t from = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(off >> 32), j) << 32) | (uint32_t)__shfl((int)(uint32_t)off, j));
-            if (from < 0) continue;  // (a weight of 0 keeps an infinity: NaN)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (lane + 64 * x < D) out[x] = fmaf(w, srv_load1(CT, a.v_cache, from + lane + 64 * x), out[x]);
-        }
-    }
-    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-        if (lane + 64 * x < D) srv_store1(QT, a.out, q_row * a.out_stride + head * D + lane + 64 * x, l == 0.0f ? 0.0f : out[x] / l);
-}
-
 // TEAMS: of four waves with the same rows each, which share the tiles.
 template <int CT, int QT, int DP, bool FORM, int TEAMS>
 __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTwo && TEAMS == 1 ? 2 : 1)) void prompt_attention_kernel(PromptAttentionArgs a, PromptShape sh) {
@@ -212,7 +165,7 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
     __shared__ srv_u32x4 lds_k0[TEAMS * C::kTile], lds_k1[TEAMS * C::kTile], lds_v0[TEAMS * C::kTile], lds_v1[TEAMS * C::kTile];
     __shared__ RowAt row_at[2][TEAMS * kWaves][kOwn];
     __shared__ uint64_t lds_live[2][TEAMS];  // of a tile's tokens
-    __shared__ int lds_odd;                  // infinities or NaNs were found where not all rows see them
+    __shared__ int lds_odd;                  // infinities or NaNs were cleared
     const int lane = threadIdx.x & 63, any_wave = uniform((int)(threadIdx.x >> 6)), wave = any_wave % kWaves, team = any_wave / kWaves;
     const int l32 = lane & 31, half = lane >> 5;
     const int D = (int)a.head_dim;
@@ -543,20 +496,35 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
     };
 
     // What some rows of the workgroup do not see of a tile weighs nothing for them, but zero times
-    // an infinity or a NaN is a NaN: where such a tile's values hold one, the rows are done again
-    // in the end, one by one.  A wave looks through the tokens that it copied.
-    auto look_for_odd = [&](const srv_u32x4 *tile_v, int it) __attribute__((always_inline)) {
+    // an infinity or a NaN is a NaN.  Such a tile's infinities and NaNs are cleared before anyone
+    // multiplies it, by the wave that copied them, and go to those who see them in the end.  One of
+    // them near the ends of two bf16 prompts of 4096 tokens, 32 heads on 8 of 128: 380 -> 423 us (taking
+    // the workgroup's rows again one by one: 101 ms).
+    constexpr uint32_t kExponent = kF32 ? 0x7F800000u : CT == TML_TYPE_F16 ? 0x7C00u : 0x7F80u;
+    // (bits of a word that hold its infinities and NaNs)
+    auto odd_bits = [](uint32_t w) __attribute__((always_inline)) {
+        if constexpr (kF32) return (w & kExponent) == kExponent ? ~0u : 0u;
+        return ((w & kExponent) == kExponent ? 0xFFFFu : 0u) | ((w >> 16 & kExponent) == kExponent ? 0xFFFF0000u : 0u);
+    };
+    auto seen_by_all = [&](int64_t k0) { return min(k0 + BN, end) <= high_of(block_first) && k0 >= low_of(block_last); };
+    auto clear_odd = [&](srv_u32x4 *tile_v, int it) __attribute__((always_inline)) {
         const int64_t k0 = tile_at(it);
-        if (min(k0 + BN, end) <= high_of(block_first) && k0 >= low_of(block_last)) return;
-        constexpr uint32_t kExponent = kF32 ? 0x7F800000u : CT == TML_TYPE_F16 ? 0x7C00u : 0x7F80u;
-        bool odd = false;
-#pragma unroll
+        if (__builtin_expect(k0 < begin || seen_by_all(k0), 1)) return;  // (before the first tile: zeros that other waves write)
+        srv_u32x4 *const mine = tile_v + any_wave * kOwn * KP + lane;
+#pragma unroll 1
         for (int i = 0; i < C::kCopies; ++i) {
-            const srv_u32x4 v = tile_v[any_wave * kOwn * KP + i * 64 + lane];
+            srv_u32x4 v = mine[64 * i];
+            uint32_t odd = 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) odd |= (v[x] & kExponent) == kExponent || (!kF32 && (v[x] >> 16 & kExponent) == kExponent);
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t bits = odd_bits(v[x]);
+                odd |= bits;
+                v[x] &= ~bits;
+            }
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) == 0, 1)) continue;
+            mine[64 * i] = v;
+            lds_odd = 1;
         }
-        if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) lds_odd = 1;
     };
 
     // ---- A turn a tile: the scores' product, then the weights beside the product of the tile
@@ -574,8 +542,8 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
             // they copy zeros)
             const Sources values = sources_of(row_at[it & 1][any_wave], true);
             wait_copies<0>();
+            clear_odd(v_before, it - 1);
             __syncthreads();  // this tile's keys and the values before are there, the tile before was read
-            look_for_odd(v_before, it - 1);
             find_rows(it + 1, next_block);
             const Sources keys = sources_of(row_at[(it + 1) & 1][any_wave], false);
             copy_rows(k_next, keys);
@@ -585,6 +553,21 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
             if constexpr (kF32) {  // (the weights are the scores' registers)
                 multiply_values(v_before);
                 multiply_keys(k_now, sum);
+                constexpr int kAhead = 8, kReads = kJ * (DP / 32);  // reads ahead of the products
+                __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+                for (int i = kAhead; i < kReads; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+#pragma unroll
+                for (int i = 2; i < kQ; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
                 take_scores(sum);
                 const Moved moved = new_maximum(it);
                 new_weights(moved.unit, weights);
@@ -628,21 +611,11 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
             turn(it + 1, lds_k1, lds_k0, lds_v1, lds_v0);
         }
         wait_copies<0>();
+        clear_odd(lds_v1, (steps - 1) | 1);
         __syncthreads();
-        look_for_odd(lds_v1, (steps - 1) | 1);
         multiply_values(lds_v1);
     }
 
-    if (steps > 0) {
-        __syncthreads();
-        if (lds_odd != 0) {
-            for (int i = any_wave; i < kRows && row0 + i < rows; i += TEAMS * kWaves) {
-                const int64_t here = row0 + i, at_token = token_of(here);
-                one_row<CT, QT>(a, sh, b, len, first + at_token, (int64_t)kv * sh.group + (here - at_token * sh.group), ctx + at_token, prefix, kv);
-            }
-            return;
-        }
-    }
     l += __shfl_xor(l, 32);
     if constexpr (TEAMS == 2) {  // the second team's part joins the first's
         // (in the tiles' LDS: 16 bytes of each lane follow each other, DP / 8 times, half of them in
@@ -672,23 +645,59 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
             for (int i = 0; i < 4; ++i) o[x / 4][4 * (x % 4) + i] = fmaf(o[x / 4][4 * (x % 4) + i], f, __uint_as_float(four[i]) * g);
         }
     }
-    if (row0 + 32 * wave + l32 >= rows) return;
+    const bool mine = row0 + 32 * wave + l32 < rows;
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t at = (first + token) * a.out_stride + head * D;
+    const int64_t to = (first + token) * a.out_stride + head * D;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int d = 32 * t + 8 * j + 4 * half;
-            if (d >= D) continue;
+            if (!mine || d >= D) continue;
             const float x0 = o[t][4 * j] * r, x1 = o[t][4 * j + 1] * r, x2 = o[t][4 * j + 2] * r, x3 = o[t][4 * j + 3] * r;
             if constexpr (QT == TML_TYPE_F32) {
-                *(srv_u32x4_any *)((float *)a.out + at + d) = srv_u32x4{__float_as_uint(x0), __float_as_uint(x1), __float_as_uint(x2), __float_as_uint(x3)};
+                *(srv_u32x4_any *)((float *)a.out + to + d) = srv_u32x4{__float_as_uint(x0), __float_as_uint(x1), __float_as_uint(x2), __float_as_uint(x3)};
             } else {
-                *(srv_u32x2_any *)((uint16_t *)a.out + at + d) =
+                *(srv_u32x2_any *)((uint16_t *)a.out + to + d) =
                     QT == TML_TYPE_F16 ? srv_u32x2{srv_pack_f16(x0, x1), srv_pack_f16(x2, x3)} : srv_u32x2{srv_pack_bf16(x0, x1), srv_pack_bf16(x2, x3)};
             }
         }
+    if (__builtin_expect(steps > 0 && lds_odd != 0, 0)) {  // (set before the last barrier)
+        // A lane a token finds the ones that were cleared; their rows' lanes then take them one by one.
+        // The tiles that all see, in the middle, are left out.
+        const int64_t all_see = high_of(block_first);
+        for (int64_t k0 = begin; k0 < end; k0 += BN) {
+            if (seen_by_all(k0)) {
+                if (end <= all_see) break;
+                k0 = begin + ((all_see - begin) / BN - 1) * BN;
+                continue;
+            }
+            const int64_t tok = k0 + lane % BN;
+            int64_t off = -1;
+            if (tok < end) {
+                const int block = a.block_table[b * a.table_stride + (uint32_t)tok / (uint32_t)P];
+                if (block >= 0 && block < a.n_blocks) off = (block * a.block_stride + (int64_t)((uint32_t)tok % (uint32_t)P) * a.token_stride + kv * a.head_stride) * kBytes;
+            }
+            uint32_t odd = 0;
+            if (off >= 0)
+                for (int x = 0; x < D * kBytes / 16; ++x) {
+                    const srv_u32x4 v = *(const srv_u32x4 *)((const char *)a.v_cache + off + 16 * x);
+                    odd |= odd_bits(v[0]) | odd_bits(v[1]) | odd_bits(v[2]) | odd_bits(v[3]);
+                }
+            uint64_t todo = __builtin_amdgcn_ballot_w64(odd != 0) & (~0ull >> (64 - BN));
+            while (todo != 0) {
+                const int from = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                const int64_t at = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(off >> 32), from) << 32) | (uint32_t)__shfl((int)(uint32_t)off, from));
+                const bool sees = mine && k0 + from >= low && k0 + from < high && l != 0.0f;
+                for (int i = 0; i < D / 2; ++i) {
+                    const int d = 8 * (i / 4) + 4 * half + i % 4;
+                    const float x = srv_load1(CT, (const char *)a.v_cache + at, d);
+                    if (sees && !(fabsf(x) < INFINITY)) srv_store1(QT, a.out, to + d, srv_load1(QT, a.out, to + d) + x);
+                }
+            }
+        }
+    }
 }
 
 // Two teams halve a workgroup's way through its tiles and fill the SIMDs where there are few
