@@ -498,10 +498,10 @@ int tml_hip_paged_attention_ex_dev(int q_type, int cache_type, int64_t batch, in
  *   other arguments, types, heads and alignment as in tml_hip_paged_attention_dev; tokens
  *   below 2^24, tokens * q_heads / 128 + requests * kv_heads at most 2^23
  * Arithmetic: products and sums are fp32, of q and of the weights e^(s - max) as terms of the
- * cache's type: q as there (an infinite element of f32 q on a 16-bit cache makes its
- * head's outputs NaN); weights one term where out has 16 bits (2^-8 of each for bf16, 2^-11
- * for f16), two of f16 (2^-22) or three of bf16 (2^-24) where it is f32.  An f32 cache is
- * all fp32.  Needs no workspace.
+ * cache's type: q as there (f32 q on an f16 cache to 2^-36 of its head's largest; infinite
+ * elements of q and of keys give what their scores give); weights one term where out has 16
+ * bits (2^-8 of each for bf16, 2^-11 for f16), two of f16 (2^-22) or three of bf16 (2^-24)
+ * where it is f32.  An f32 cache is all fp32.  Needs no workspace.
  * One new token a request is taken too (a mixed batch), but a request's 128 (token, head)
  * rows go through its cache one after another: tml_hip_paged_attention_ex_dev shares long
  * caches among the GPU's workgroups. */

@@ -93,7 +93,10 @@ def prompt(program, q_t, cache_t, both, heads, kv, dim, block, layout="thd", pre
         want, tol = expected(values(q[starts[r]:starts[r + 1]], q_t).reshape(n, heads, dim), k, v, pos, cap, weight, scale=scale, slopes=sl,
                              seen=ref.sees(pos, t, prefix[r] if prefix else 0, window if window < 1 << 62 else 0), positions=t)
         mine = values(out[starts[r]:starts[r + 1]], q_t).reshape(want.shape)
-        mine = np.where(np.isinf(want) & ~np.isfinite(mine), want, mine)  # (an infinite value's element is infinite or NaN)
+        # (an infinite value's element is infinite or NaN in those who see it; a weight may underflow here or there)
+        infinite = np.repeat(np.isinf(v), heads // kv, 1).astype(float)
+        sees_one = np.einsum("nt,thd->nhd", ref.sees(pos, t, prefix[r] if prefix else 0, window if window < 1 << 62 else 0).astype(float), infinite) > 0
+        mine = np.where(sees_one & ~np.isfinite(want) & ~np.isfinite(mine), want, mine)
         close(mine, want, tol + HALF_ULP[q_t] * (np.abs(want) + tol) + TINY[q_t], f"request {r}")
 
 
@@ -188,3 +191,27 @@ def prompt_odd_values(program, q_t, cache_t, dim, mask, cus=256):
     # (one head's rows: a workgroup of 128 tokens, whose first and last see tiles far apart)
     prompt(program, q_t, cache_t, [(300, 140)], 1, 1, dim, 32, odd=sprinkled(rng, [440], 1, dim, 1, 0.05, [inf, -inf, nan]), window=mask.get("window", 0), seed=32, cus=cus)
 
+
+KEY_MASKS = [dict(), dict(cap=20.0), dict(cap=1e4, slopes=True), dict(window=40), dict(prefix=[100, 0, 133], cap=5.0), dict(scale=-0.2), dict(scale=-0.3, cap=3.0)]
+
+
+def prompt_odd_keys(program, q_t, cache_t, dim, mask, cus=256):
+    """A score of -inf weighs nothing, one of +inf makes its row NaN, a capped one is the cap: whatever the terms of q are."""
+    both, inf, nan = [(60, 90), (0, 70), (130, 3)], np.inf, np.nan
+    lens = [c + n for c, n in both]
+    # few infinite keys (rows with scores of -inf alone stay numbers), elements of q that are 0, tiny next to the others, or both signs
+    rng = np.random.default_rng(dim)
+    tiny = 1e-6 if q_t == F16 else 1e-20 if q_t == F32 and cache_t != BF16 else 1e-35
+    odd_q = [(int(rng.integers(160)), int(rng.integers(4)) * dim + 3, x) for x in (0.0, -0.0, tiny, -tiny, 1.0, -2.0, 0.3) * 6]
+    for odd in ([(0, 30, 0, 0, 3, inf)], [(0, 5, 0, 0, 3, -inf), (0, 100, 0, 1, 3, -inf), (1, 3, 0, 1, 3, inf), (2, 131, 0, 0, 3, inf)],
+                [(0, 64, 0, 0, 3, inf), (0, 64, 0, 0, 4, inf), (0, 70, 0, 0, 3, -inf)], [(0, 20, 0, 0, 3, inf), (0, 120, 0, 0, 5, nan), (1, 0, 0, 0, 3, inf)],
+                [(0, 20, 0, 0, 3, inf), (0, 130, 1, 0, 7, -inf)]):
+        prompt(program, q_t, cache_t, both, 4, 2, dim, 16, odd=odd, odd_q=odd_q, seed=41, cus=cus, **mask)
+
+
+def prompt_odd_q(program, q_t, cache_t, dim):
+    """Infinite and NaN elements of q give what their scores give: NaN, or under a cap the cap."""
+    odd_q = [(3, 5, np.nan), (40, dim + 1, np.nan), (70, 3 * dim, np.nan), (7, 2 * dim + 1, np.inf), (90, 9, -np.inf), (91, 9, np.inf), (91, 10, np.inf), (92, dim, -np.inf)]
+    for cap in (0.0, 20.0):
+        prompt(program, q_t, cache_t, [(60, 90), (0, 70)], 4, 2, dim, 16, odd_q=odd_q, cap=cap, seed=42)
+        prompt(program, q_t, cache_t, [(60, 90), (0, 70)], 4, 2, dim, 16, odd_q=odd_q, odd=[(0, 30, 0, 0, 3, np.inf)], cap=cap, slopes=True, seed=43)

@@ -50,3 +50,16 @@ def test_prompt_before_the_cache(program, q_t, cache_t, window):
 @pytest.mark.parametrize("mask", edges.ODD_MASKS, ids=lambda m: "-".join(m) or "causal")
 def test_prompt_odd_values(program, q_t, cache_t, dim, mask):
     edges.prompt_odd_values(program, q_t, cache_t, dim, mask)
+
+
+@combos
+@pytest.mark.parametrize("dim", [40, 64, 128, 256])
+@pytest.mark.parametrize("mask", edges.KEY_MASKS, ids=lambda m: "-".join(m) or "causal")
+def test_prompt_odd_keys(program, q_t, cache_t, dim, mask):
+    edges.prompt_odd_keys(program, q_t, cache_t, dim, mask)
+
+
+@combos
+@pytest.mark.parametrize("dim", [40, 64])
+def test_prompt_odd_q(program, q_t, cache_t, dim):
+    edges.prompt_odd_q(program, q_t, cache_t, dim)

@@ -25,7 +25,7 @@
 // reads of one piece of 16 rows (keys) nor those of 64 bytes of four rows (values) meet in a
 // bank.
 // Precision: sums, maxima and the scores are fp32.  f32 queries go in as terms of the
-// cache's type (two of f16, scaled by a power of two, three of bf16), and so do the
+// cache's type (two of f16, scaled by a power of two, three of bf16; see to_query_terms), and so do the
 // weights where the output is f32; where it has 16 bits the weights are rounded to them
 // once, which adds to an output about what its own rounding does (2^-8 of bf16, 2^-11 of f16,
 // at most).
@@ -89,6 +89,36 @@ __device__ __forceinline__ int anew(int v) {
 __device__ __forceinline__ float max_of_halves(float v) {
     const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+}
+
+// f32 elements of q (f16: below 2^15) in N terms of type CT.  All but the last are cut off strictly
+// below what is left, so each term of an element that is not 0 has its sign and is not 0 itself:
+// an infinite key is infinite with all of them alike, where a later term of 0 or of the other sign
+// would make a NaN of the sum.  The terms are off by 2^-22 of the element and 2^-22 (two of f16), or by
+// 2^-100 (three of bf16: 8 bits, the next 8, and 1 to 256 units of the last place).
+template <int CT, int N>
+__device__ __forceinline__ void to_query_terms(const float (&v)[8], srv_u32x4 (&t)[N]) {
+    constexpr bool kF16 = CT == TML_TYPE_F16;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float terms[2][N];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float x = v[e + i];
+            const bool itself = __builtin_isfpclass(x, 0x267);  // zeros, infinities, NaNs
+            float left = __builtin_copysignf(fmaxf(fabsf(x), kF16 ? 0x1p-23f : 0x1p-100f), x);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                float term = left;
+                if (n + 1 < N) term = __uint_as_float((__float_as_uint(left) - 1) & (kF16 ? 0xFFFFE000u : 0xFFFF0000u));
+                else if (kF16) term = __builtin_copysignf(fmaxf(fabsf(left), 0x1p-24f), x);
+                terms[i][n] = itself ? x : term;
+                left -= term;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) t[n][e / 2] = kF16 ? srv_pack_f16(terms[0][n], terms[1][n]) : srv_pack_bf16(terms[0][n], terms[1][n]);
+    }
 }
 
 // New tokens of request r: their first row of q, and how many (not past q's end).
@@ -262,7 +292,7 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= up;
                 srv_u32x4 t[NQ];
-                to_terms<CT, NQ>(v, t);
+                to_query_terms<CT, NQ>(v, t);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) q[n][c] = t[n];
             }
