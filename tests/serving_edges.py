@@ -130,8 +130,10 @@ def decode(program, q_t, cache_t, lens, heads, kv, dim, block, cap=0.0, slopes=F
     for r, length in enumerate(lens):
         pos = np.array([length - 1])
         t, k, v, km, vm = cache.of(r, length)
-        want, tol = expected(values(q[r], q_t).reshape(1, heads, dim), k, v, pos, cap, weight, scale=scale, slopes=sl, seen=ref.sees(pos, t, 0, window),
-                             positions=t, key_mag=km, val_mag=vm)
+        its_q = values(q[r], q_t).reshape(1, heads, dim)
+        if cache_t is None:
+            its_q = np.where(np.isinf(its_q), np.nan, its_q)  # (an infinite element makes its head NaN)
+        want, tol = expected(its_q, k, v, pos, cap, weight, scale=scale, slopes=sl, seen=ref.sees(pos, t, 0, window), positions=t, key_mag=km, val_mag=vm)
         close(values(got[bo][r], q_t).reshape(want[0].shape), want[0], tol[0] + HALF_ULP[q_t] * (np.abs(want[0]) + tol[0]) + TINY[q_t], f"request {r}")
 
 
@@ -215,3 +217,49 @@ def prompt_odd_q(program, q_t, cache_t, dim):
     for cap in (0.0, 20.0):
         prompt(program, q_t, cache_t, [(60, 90), (0, 70)], 4, 2, dim, 16, odd_q=odd_q, cap=cap, seed=42)
         prompt(program, q_t, cache_t, [(60, 90), (0, 70)], 4, 2, dim, 16, odd_q=odd_q, odd=[(0, 30, 0, 0, 3, np.inf)], cap=cap, slopes=True, seed=43)
+
+
+def decode_odd_q_and_keys(program, q_t, cache_t, cap):
+    """Infinite and NaN elements of q, infinite keys (float caches), NaN groups (4-bit caches)."""
+    inf, nan = np.inf, np.nan
+    odd_q = [(0, 5, nan), (0, 64 + 9, inf), (2, 128, -inf), (2, 3 * 64 + 1, nan)]
+    if cache_t is None:
+        decode(program, q_t, None, [70, 3, 40], 4, 2, 64, 16, cap=cap, odd_q=odd_q, seed=51)
+        # a key's group: the heads that look at it; a value's: its 32 elements
+        decode(program, q_t, None, [70, 3, 40], 4, 2, 64, 16, cap=cap, spoil=[(0, 33, 0, 0, 1), (1, 2, 1, 1, 0), (2, 39, 1, 0, 1)], seed=52)
+    else:
+        decode(program, q_t, cache_t, [70, 3, 40], 4, 2, 64, 16, cap=cap, odd_q=odd_q, seed=53)
+        odd = [(0, 30, 0, 0, 3, inf), (0, 69, 0, 1, 3, -inf), (1, 1, 0, 0, 7, -inf), (2, 0, 0, 1, 7, inf), (2, 20, 0, 1, 9, inf)]
+        decode(program, q_t, cache_t, [70, 3, 40], 4, 2, 64, 16, cap=cap, slopes=cap > 0, odd=odd, seed=54)
+
+
+# ---------------------------------------------------------------- other scales
+SCALES = [-0.3, 0.0, -1e-4, 2.0]
+
+
+def other_scales(program, q_t, cache_t, scale):
+    """Negative scales, one of 0 (every token alike), one that leaves few tokens with a weight."""
+    decode(program, q_t, cache_t, [70, 3, 0], 4, 2, 64, 16, scale=scale, seed=61)
+    decode(program, q_t, cache_t, [70, 3, 0], 4, 2, 64, 16, scale=scale, cap=4.0, slopes=True, seed=62)
+    if cache_t is not None:
+        prompt(program, q_t, cache_t, [(60, 90), (0, 20)], 4, 2, 64, 16, scale=scale, seed=63)
+        prompt(program, q_t, cache_t, [(60, 90), (0, 20)], 4, 2, 40, 16, scale=scale, cap=4.0, slopes=True, window=50, seed=64)
+
+
+# ------------------------------------------------------ more workgroups than CUs
+MANY_MASKS = [dict(), dict(window=77), dict(some_prefix=True), dict(lost=[(0, 2, -1), (1, 5, 1 << 30), (2, 0, 99999)], layout="htd"), dict(odd=True)]
+
+
+def prompt_many(program, q_t, cache_t, dim, mask, cus, requests):
+    """More workgroups than CUs: prompts in 16 bits then go by one team of waves each."""
+    rng = np.random.default_rng(dim)
+    both = [(0, 150), (300, 40), (64, 64), (0, 0), (200, 130)] + [(int(rng.integers(40)), int(rng.integers(1, 6))) for _ in range(requests)]
+    tokens, kv = sum(n for _, n in both) + 2, 4
+    assert (tokens // 128 + len(both)) * kv > cus
+    more = {k: v for k, v in mask.items() if k not in ("some_prefix", "odd")}
+    if "some_prefix" in mask:
+        more["prefix"] = [int(rng.integers(c + n + 1)) for c, n in both]
+    if "odd" in mask:
+        more["odd"] = sprinkled(rng, [c + n for c, n in both[:3]], kv, dim, 1, 0.05, [np.inf, -np.inf, np.nan])
+    prompt(program, q_t, cache_t, both, kv, kv, dim, 16, seed=71, cus=cus, **more)
+

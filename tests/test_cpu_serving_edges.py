@@ -69,3 +69,22 @@ def test_prompt_odd_keys(program, q_t, cache_t, dim, mask):
 @pytest.mark.parametrize("dim", [40, 64])
 def test_prompt_odd_q(program, q_t, cache_t, dim):
     edges.prompt_odd_q(program, q_t, cache_t, dim)
+
+
+@decodes
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_decode_odd_q_and_keys(program, q_t, cache_t, cap):
+    edges.decode_odd_q_and_keys(program, q_t, cache_t, cap)
+
+
+@decodes
+@pytest.mark.parametrize("scale", edges.SCALES)
+def test_other_scales(program, q_t, cache_t, scale):
+    edges.other_scales(program, q_t, cache_t, scale)
+
+
+@pytest.mark.parametrize("q_t,cache_t", [(F16, F16), (BF16, BF16)], ids=tname)
+@pytest.mark.parametrize("dim", [64])
+@pytest.mark.parametrize("mask", edges.MANY_MASKS, ids=lambda m: "-".join(m) or "causal")
+def test_prompt_many(program, q_t, cache_t, dim, mask):
+    edges.prompt_many(program, q_t, cache_t, dim, mask, 1, 3)
