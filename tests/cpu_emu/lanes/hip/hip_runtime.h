@@ -40,7 +40,6 @@
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 tml_emu_plain_mfma_bf16_32
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16 tml_emu_plain_mfma_f16_32
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16 tml_emu_plain_read_tr
-#define __builtin_amdgcn_s_barrier tml_emu_plain_s_barrier
 #define __builtin_amdgcn_permlane32_swap tml_emu_plain_permlane32_swap
 #define __builtin_amdgcn_permlane16_swap tml_emu_plain_permlane16_swap
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8 tml_emu_plain_mfma_i8
@@ -65,7 +64,6 @@
 #undef __builtin_amdgcn_mfma_f32_32x32x16_bf16
 #undef __builtin_amdgcn_mfma_f32_32x32x16_f16
 #undef __builtin_amdgcn_ds_read_tr16_b64_v4i16
-#undef __builtin_amdgcn_s_barrier
 #undef __builtin_amdgcn_permlane32_swap
 #undef __builtin_amdgcn_permlane16_swap
 #undef __builtin_amdgcn_mfma_i32_16x16x64_i8
@@ -117,7 +115,6 @@ tml_lane_launcher<P...> tml_emu_launch(void (*k)(P...), dim3 g, dim3 b, size_t s
 #define TML_LANE_OP __attribute__((noinline, noduplicate))
 
 inline void __syncthreads() { tml_lane_block_barrier(); }
-inline void __builtin_amdgcn_s_barrier() { tml_lane_block_barrier(); }
 
 template <typename T>
 inline T tml_lane_from(const tml_lane_meeting &m, unsigned lane) {

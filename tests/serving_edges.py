@@ -179,17 +179,19 @@ def sprinkled(rng, lens, kv, dim, what, share, kinds):
 ODD_MASKS = [dict(), dict(window=30), dict(prefix=[110, 0, 64]), dict(window=45, prefix=[130, 70, 0], cap=20.0), dict(slopes=True, lost=[(0, 2, -1), (0, 6, 1 << 30)])]
 
 
-def prompt_odd_values(program, q_t, cache_t, dim, mask, cus=256):
+def prompt_odd_values(program, q_t, cache_t, dim, mask, cus=256, shares=(0.02, 0.5)):
     """Infinite and NaN values reach those who see them and no one else, few and many of them, at the tiles' ends too."""
     both, inf, nan = [(60, 90), (0, 70), (130, 3)], np.inf, np.nan
     lens = [c + n for c, n in both]
     rng = np.random.default_rng(dim)
-    for share in (0.02, 0.5):
+    for share in shares:
         odd = sprinkled(rng, lens, 2, dim, 1, share, [inf, -inf, nan])
         odd += [(0, p, 1, 0, dim - 1, inf) for p in (63, 64, 127, 128, 149)] + [(1, 69, 1, 1, 0, nan)]
         # (a page that is no block of the cache holds no values)
         odd = [o for o in odd if (o[0], o[1] // 16) not in [(r, i) for r, i, _ in mask.get("lost", ())]]
         prompt(program, q_t, cache_t, both, 4, 2, dim, 16, odd=odd, seed=31, cus=cus, **mask)
+    if len(shares) < 2 and mask:
+        return
     # (one head's rows: a workgroup of 128 tokens, whose first and last see tiles far apart)
     prompt(program, q_t, cache_t, [(300, 140)], 1, 1, dim, 32, odd=sprinkled(rng, [440], 1, dim, 1, 0.05, [inf, -inf, nan]), window=mask.get("window", 0), seed=32, cus=cus)
 
@@ -197,7 +199,7 @@ def prompt_odd_values(program, q_t, cache_t, dim, mask, cus=256):
 KEY_MASKS = [dict(), dict(cap=20.0), dict(cap=1e4, slopes=True), dict(window=40), dict(prefix=[100, 0, 133], cap=5.0), dict(scale=-0.2), dict(scale=-0.3, cap=3.0)]
 
 
-def prompt_odd_keys(program, q_t, cache_t, dim, mask, cus=256):
+def prompt_odd_keys(program, q_t, cache_t, dim, mask, cus=256, which=slice(None)):
     """A score of -inf weighs nothing, one of +inf makes its row NaN, a capped one is the cap: whatever the terms of q are."""
     both, inf, nan = [(60, 90), (0, 70), (130, 3)], np.inf, np.nan
     lens = [c + n for c, n in both]
@@ -205,9 +207,10 @@ def prompt_odd_keys(program, q_t, cache_t, dim, mask, cus=256):
     rng = np.random.default_rng(dim)
     tiny = 1e-6 if q_t == F16 else 1e-20 if q_t == F32 and cache_t != BF16 else 1e-35
     odd_q = [(int(rng.integers(160)), int(rng.integers(4)) * dim + 3, x) for x in (0.0, -0.0, tiny, -tiny, 1.0, -2.0, 0.3) * 6]
-    for odd in ([(0, 30, 0, 0, 3, inf)], [(0, 5, 0, 0, 3, -inf), (0, 100, 0, 1, 3, -inf), (1, 3, 0, 1, 3, inf), (2, 131, 0, 0, 3, inf)],
-                [(0, 64, 0, 0, 3, inf), (0, 64, 0, 0, 4, inf), (0, 70, 0, 0, 3, -inf)], [(0, 20, 0, 0, 3, inf), (0, 120, 0, 0, 5, nan), (1, 0, 0, 0, 3, inf)],
-                [(0, 20, 0, 0, 3, inf), (0, 130, 1, 0, 7, -inf)]):
+    sets = ([(0, 30, 0, 0, 3, inf)], [(0, 5, 0, 0, 3, -inf), (0, 100, 0, 1, 3, -inf), (1, 3, 0, 1, 3, inf), (2, 131, 0, 0, 3, inf)],
+            [(0, 64, 0, 0, 3, inf), (0, 64, 0, 0, 4, inf), (0, 70, 0, 0, 3, -inf)], [(0, 20, 0, 0, 3, inf), (0, 120, 0, 0, 5, nan), (1, 0, 0, 0, 3, inf)],
+            [(0, 20, 0, 0, 3, inf), (0, 130, 1, 0, 7, -inf)])
+    for odd in sets[which]:
         prompt(program, q_t, cache_t, both, 4, 2, dim, 16, odd=odd, odd_q=odd_q, seed=41, cus=cus, **mask)
 
 

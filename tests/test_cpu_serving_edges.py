@@ -25,11 +25,12 @@ def program():
 
 
 combos = pytest.mark.parametrize("q_t,cache_t", edges.COMBOS, ids=tname)
+some = pytest.mark.parametrize("q_t,cache_t", [(F32, F32), (F32, F16), (BF16, BF16), (F32, BF16)], ids=tname)  # (the GPU's tests have all)
 decodes = pytest.mark.parametrize("q_t,cache_t", [*edges.COMBOS, (F32, None), (F16, None), (BF16, None)], ids=tname)
 
 
 @combos
-@pytest.mark.parametrize("cap", edges.CAPS)
+@pytest.mark.parametrize("cap", edges.CAPS[::2] + edges.CAPS[-1:])
 def test_prompt_caps(program, q_t, cache_t, cap):
     edges.prompt_caps(program, q_t, cache_t, cap)
 
@@ -40,29 +41,29 @@ def test_prompt_cap_of_large_scale(program, q_t, cache_t):
 
 
 @decodes
-@pytest.mark.parametrize("cap", edges.CAPS)
+@pytest.mark.parametrize("cap", edges.CAPS[::3])
 def test_decode_caps(program, q_t, cache_t, cap):
     edges.decode_caps(program, q_t, cache_t, cap)
 
 
 @combos
-@pytest.mark.parametrize("window", edges.WINDOWS)
+@pytest.mark.parametrize("window", edges.WINDOWS[::3])
 def test_prompt_before_the_cache(program, q_t, cache_t, window):
     edges.prompt_before_the_cache(program, q_t, cache_t, window)
 
 
-@combos
+@some
 @pytest.mark.parametrize("dim", [40])
 @pytest.mark.parametrize("mask", edges.ODD_MASKS, ids=lambda m: "-".join(m) or "causal")
 def test_prompt_odd_values(program, q_t, cache_t, dim, mask):
-    edges.prompt_odd_values(program, q_t, cache_t, dim, mask, cus=1 if "window" in mask else 256)
+    edges.prompt_odd_values(program, q_t, cache_t, dim, mask, cus=1 if "window" in mask else 256, shares=(0.02,))
 
 
-@combos
+@some
 @pytest.mark.parametrize("dim", [40])
-@pytest.mark.parametrize("mask", edges.KEY_MASKS[::2], ids=lambda m: "-".join(m) or "causal")
+@pytest.mark.parametrize("mask", edges.KEY_MASKS[::3], ids=lambda m: "-".join(m) or "causal")
 def test_prompt_odd_keys(program, q_t, cache_t, dim, mask):
-    edges.prompt_odd_keys(program, q_t, cache_t, dim, mask)
+    edges.prompt_odd_keys(program, q_t, cache_t, dim, mask, which=slice(1, None, 2))
 
 
 @combos
@@ -78,12 +79,12 @@ def test_decode_odd_q_and_keys(program, q_t, cache_t, cap):
 
 
 @decodes
-@pytest.mark.parametrize("scale", edges.SCALES)
+@pytest.mark.parametrize("scale", edges.SCALES[:2])
 def test_other_scales(program, q_t, cache_t, scale):
     edges.other_scales(program, q_t, cache_t, scale)
 
 
-@pytest.mark.parametrize("q_t,cache_t", [(F16, F16), (BF16, BF16)], ids=tname)
+@pytest.mark.parametrize("q_t,cache_t", [(BF16, BF16)], ids=tname)
 @pytest.mark.parametrize("dim", [64])
 @pytest.mark.parametrize("mask", edges.MANY_MASKS, ids=lambda m: "-".join(m) or "causal")
 def test_prompt_many(program, q_t, cache_t, dim, mask):

@@ -6,7 +6,7 @@
 //
 // A workgroup takes a row.  One pass keeps m, S and T in every lane (a lane's own
 // maximum: it rises a few times a row) and joins them at the end.  2048 rows of 51866 bf16
-// logits take 47 us, 4.5 TB/s: bound by memory.  Four f32 rows with the five best take 12 us,
+// logits take 42 us, 5.1 TB/s: bound by memory.  Four f32 rows with the five best take 12 us,
 // most of it the instructions of one CU a row (some nine an element); a row on more CUs would
 // take a second launch and a workspace to save about a third of that.
 //
@@ -195,7 +195,9 @@ void launch_rows(const LogprobsArgs &a, hipStream_t s) {
 //   2048 columns  7.5 /  5.4 / 27      12 / 15 / 288
 //   8192          14  /  7.3 /  7.6    28 / 26 /  66
 //   32768         34  / 13   / 10      84 / 81 / 105
-// and for 512 rows of 32768 38 / 18.1 / 17.2.
+// and for 512 rows of 32768 38 / 18.1 / 17.2.  f32 is within a tenth of that where memory does not bound it
+// (2048 rows of 32768, top 20, 89 / 85 / 82).  Without alternatives the same rule is right by smaller
+// steps: 4 rows 3.7 / 4.1, 6.1 / 5.0 / 4.3 and 16.2 / 6.3 / 5.9; 2048 rows 4.9 / 6.2, 10.2 / 10.7 / 17.9 and 27.7 / 26.3 / 29.7.
 template <int T>
 void launch_waves(const LogprobsArgs &a, hipStream_t s) {
     if (a.cols <= 2048) launch_rows<T, 1>(a, s);

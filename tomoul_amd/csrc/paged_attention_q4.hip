@@ -34,10 +34,14 @@
 //
 // Measured on MI355X (launches in a graph): bf16, 64 requests of up to 4096 tokens, 32 heads on 8
 // of 128 65 us (2.3 TB/s of the cache's 5 bits; in 16 bits 112 us), two of 40k to 65k tokens,
-// f16, 41 us (3.2 TB/s); one of 448 tokens, f32, 20 heads of 64, 9.5 us.  Memory does not bound it:
-// a tile of 4 KB is some 300 vector instructions of a wave, of which the nibbles of values are
-// 100 and the weights 60, and they take 0.5 us of a SIMD; loads two tiles ahead gained nothing
-// (41.3 for 39 us).  Short lists are bound by the chain of dependent loads and by the joining.
+// f16, 40 us (3.3 TB/s); one of 448 tokens, f32, 20 heads of 64, 9.3 us.  Memory does not bound it:
+// a tile of 4 KB is some 360 vector instructions of a wave, of which the nibbles of values are
+// 100 and the weights 60.  By the counters (64 requests, two long ones): vector instructions issue
+// for 70 % of the time in which a CU has waves, but a CU has waves for 47 and 65 % of the kernel alone.  The
+// rest is uneven shares: with requests of 2048 tokens each a tile takes 1.63 ns of the GPU, with lengths from
+// 512 on 1.67, with the ragged ones 2.23, of which the short ones put many lists, each with its
+// prologue and its joining, into one workgroup's share.  Loads two tiles ahead gained nothing (41.3 for 39
+// us).  Short lists are bound by the chain of dependent loads and by the joining.
 #include "paged_split.hpp"
 #include "terms.hpp"
 

@@ -32,10 +32,10 @@
 // An f32 cache runs on the fp32 matrix cores.
 //
 // Measured on MI355X (launches in a graph): bf16, two causal prompts of 6000 to 8192 tokens, 32
-// heads on 8 of 128, 0.98 ms, 830 TFLOP/s of the pairs seen (a library product reaches 1130);
-// 1500 frames, 20 heads of 64, f16, 32 us; sixteen chunks of 1 to 256 tokens over contexts to 4096,
-// capped, 170 us.  The first is bound by issue: without the exponentials it took 918, without the
-// second product 722, without the copies 713 of 970 us, so a SIMD's two waves hardly overlap
+// heads on 8 of 128, 0.95 ms, 856 TFLOP/s of the pairs seen (a library product reaches 1130);
+// 1500 frames, 20 heads of 64, f16, 28 to 32 us; sixteen chunks of 1 to 256 tokens over contexts to 4096,
+// capped, 171 us.  The first is bound by issue: without the exponentials it took 918, without the
+// second product 722, without the copies 713 of then 970 us, so a SIMD's two waves hardly overlap
 // their products with each other's exponentials.  The others are bound by their longest workgroups (66 tiles of
 // 2.5 us): a request's tokens are not split.
 #include "terms.hpp"
@@ -733,8 +733,10 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
 // Two teams halve a workgroup's way through its tiles and fill the SIMDs where there are few
 // workgroups, for the joining of their parts; where two workgroups of one team share a CU they go their ways
 // apart, which eight waves behind one barrier do not.  Measured, one / two teams: 1500 frames, 20 heads
-// of 64 (240 workgroups) 37.8 / 32.7 us; sixteen chunks over contexts to 4096 (512) 171 / 205; two
-// prompts of 6000 to 8192 tokens (3500) 978 / 1129.
+// of 64 (240 workgroups) 37.8 / 32.7 us; two prompts of 6000 to 8192 tokens (3500) 978 / 1129; 16 heads on
+// 8 of 128, f16, 448 new tokens 23.1 / 21.9, 128 over 966 39.3 / 36.1, 64 13.4 / 16.9 (a tile a team, and the
+// joining).  Capped or biased scores and f32 q have one team whatever the grid: the same three 28.0 / 25.3,
+// 50.5 / 44.8 and 14.8 / 18.7 capped, 33.6 / 36.1, 55.9 / 57.5 and 20.2 / 27.8 with f32 q on f16.
 template <int CT, int QT, int DP, bool FORM>
 void launch_teams(const PromptAttentionArgs &a, const PromptShape &sh, hipStream_t s) {
     const dim3 grid(sh.tiles * (unsigned)a.kv_heads);
