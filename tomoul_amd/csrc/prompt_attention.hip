@@ -32,9 +32,9 @@
 // An f32 cache runs on the fp32 matrix cores.
 //
 // Measured on MI355X (launches in a graph): bf16, two causal prompts of 6000 to 8192 tokens, 32
-// heads on 8 of 128, 0.95 ms, 856 TFLOP/s of the pairs seen (a library product reaches 1130);
+// heads on 8 of 128, 0.94 ms, 867 TFLOP/s of the pairs seen (a library product reaches 1130);
 // 1500 frames, 20 heads of 64, f16, 28 to 32 us; sixteen chunks of 1 to 256 tokens over contexts to 4096,
-// capped, 171 us.  The first is bound by issue: without the exponentials it took 918, without the
+// capped, 160 to 165 us.  The first is bound by issue: without the exponentials it took 918, without the
 // second product 722, without the copies 713 of then 970 us, so a SIMD's two waves hardly overlap
 // their products with each other's exponentials.  The others are bound by their longest workgroups (66 tiles of
 // 2.5 us): a request's tokens are not split.
@@ -527,21 +527,25 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
 
     // What some rows of the workgroup do not see of a tile weighs nothing for them, but zero times
     // an infinity or a NaN is a NaN.  Such a tile's infinities and NaNs are cleared before anyone
-    // multiplies it, by the wave that copied them, and go to those who see them in the end.  One of
-    // them near the ends of two bf16 prompts of 4096 tokens, 32 heads on 8 of 128: 380 -> 423 us (taking
-    // the workgroup's rows again one by one: 101 ms).
+    // multiplies it, by the wave that copied them, and go to those who see them in the end.  With one
+    // of them near the ends of two bf16 prompts of 4096 tokens, 32 heads on 8 of 128, 381 to 423 us, without
+    // 359 to 394 (taking the workgroup's rows again one by one: 101 ms).
     constexpr uint32_t kExponent = kF32 ? 0x7F800000u : CT == TML_TYPE_F16 ? 0x7C00u : 0x7F80u;
     // (bits of a word that hold its infinities and NaNs)
     auto odd_bits = [](uint32_t w) __attribute__((always_inline)) {
         if constexpr (kF32) return (w & kExponent) == kExponent ? ~0u : 0u;
         return ((w & kExponent) == kExponent ? 0xFFFFu : 0u) | ((w >> 16 & kExponent) == kExponent ? 0xFFFF0000u : 0u);
     };
-    auto seen_by_all = [&](int64_t k0) { return min(k0 + BN, end) <= high_of(block_first) && k0 >= low_of(block_last); };
+    const int64_t all_from = low_of(block_last), all_to = high_of(block_first);
+    auto seen_by_all = [&](int64_t k0) { return min(k0 + BN, end) <= all_to && k0 >= all_from; };
+    // (the tiles from .. to .. are seen by all; where all see the end, the last may be too)
+    const int whole_from = uniform((int)((max(all_from - begin, (int64_t)0) + BN - 1) / BN)), whole_to = uniform((int)(max(all_to - begin, (int64_t)0) / BN));
     auto clear_odd = [&](srv_u32x4 *tile_v, int it) __attribute__((always_inline)) {
-        const int64_t k0 = tile_at(it);
-        if (__builtin_expect(k0 < begin || seen_by_all(k0), 1)) return;  // (before the first tile: zeros that other waves write)
+        const int tile = TEAMS * it + team;
+        if (__builtin_expect(tile < 0 || (tile >= whole_from && tile < whole_to), 1)) return;  // (before the first tile: zeros that other waves write)
+        if (seen_by_all(tile_at(it))) return;
         srv_u32x4 *const mine = tile_v + any_wave * kOwn * KP + lane;
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < C::kCopies; ++i) {
             srv_u32x4 v = mine[64 * i];
             uint32_t odd = 0;
@@ -695,11 +699,10 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
     if (__builtin_expect(steps > 0 && lds_odd != 0, 0)) {  // (set before the last barrier)
         // A lane a token finds the ones that were cleared; their rows' lanes then take them one by one.
         // The tiles that all see, in the middle, are left out.
-        const int64_t all_see = high_of(block_first);
         for (int64_t k0 = begin; k0 < end; k0 += BN) {
             if (seen_by_all(k0)) {
-                if (end <= all_see) break;
-                k0 = begin + ((all_see - begin) / BN - 1) * BN;
+                if (end <= all_to) break;
+                k0 = begin + (whole_to - 1) * (int64_t)BN;
                 continue;
             }
             const int64_t tok = k0 + lane % BN;
