@@ -444,7 +444,7 @@ int tml_hip_kv_store_dev(int type, int cache_type, int64_t tokens, int64_t kv_he
  * a negative one counts as 0, and one past table_width * block_size as that.
  * A score of -inf, of an infinite key say, weighs nothing, and where there are no
  * others the output is zeros too; a score that is NaN or +inf makes its head NaN.
- * An infinite value makes its element infinite or NaN.
+ * An infinite value makes its element infinite or NaN otherwise.
  *   q, out   [batch, q_heads, head_dim], rows q_stride / out_stride apart, of
  *            q_type: F32 or the cache's type
  *   caches   as in tml_hip_kv_store_dev; rows start on 16-byte boundaries
@@ -489,9 +489,10 @@ int tml_hip_paged_attention_ex_dev(int q_type, int cache_type, int64_t batch, in
  * prefix_len NULL: causal.  A prefix of the whole length: every token sees every other, as
  * in an encoder.  The scores are
  *   s_t = cap * tanh(scale * q . k_t / cap) - slopes[h] * |pos - t|
- * with cap and slopes as in tml_hip_paged_attention_ex_dev; a token that sees nothing gets
- * zeros, and what lies in other positions, NaN among it, is not looked at.  An infinite
- * value makes its element infinite or NaN in the outputs of those who see it.
+ * with cap and slopes as in tml_hip_paged_attention_ex_dev; a token that sees nothing, or
+ * scores of -inf alone, gets zeros, and what lies in other positions, NaN among it, is not
+ * looked at.  An infinite value makes its element infinite or NaN in the other outputs of
+ * those who see it.
  *   tokens       rows of q and out; those at query_start[requests] and after are left as they
  *                were.  Starts and lengths that do not fit (negative, past tokens, past the
  *                table) count as the nearest that do

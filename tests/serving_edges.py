@@ -266,3 +266,15 @@ def prompt_many(program, q_t, cache_t, dim, mask, cus, requests):
         more["odd"] = sprinkled(rng, [c + n for c, n in both[:3]], kv, dim, 1, 0.05, [np.inf, -np.inf, np.nan])
     prompt(program, q_t, cache_t, both, kv, kv, dim, 16, seed=71, cus=cus, **more)
 
+
+# ------------------------------------------------------------- nothing weighs
+def nothing_weighs(program, q_t, cache_t):
+    """Scores of -inf alone: zeros, whatever the values are."""
+    inf, nan = np.inf, np.nan
+    lens, kv, heads, dim = [1, 2, 70, 33], 2, 4, 64
+    odd = [(r, p, 0, h, 3, inf) for r, n in enumerate(lens) for p in range(n) for h in range(kv)]
+    odd += [(0, 0, 1, 0, 5, inf), (1, 1, 1, 1, 6, nan), (2, 3, 1, 0, 7, -inf), (2, 69, 1, 1, 8, nan), (3, 20, 1, 0, 9, inf)]
+    decode(program, q_t, cache_t, lens, heads, kv, dim, 16, odd=odd, odd_q=[(r, h * dim + 3, -1.0) for r in range(4) for h in range(heads)], seed=91)
+    both = [(0, 1), (1, 1), (60, 10), (0, 33)]
+    prompt(program, q_t, cache_t, both, heads, kv, dim, 16, odd=odd, odd_q=[(r, h * dim + 3, -1.0) for r in range(45) for h in range(heads)], seed=92)
+

@@ -89,3 +89,8 @@ def test_other_scales(program, q_t, cache_t, scale):
 @pytest.mark.parametrize("mask", edges.MANY_MASKS, ids=lambda m: "-".join(m) or "causal")
 def test_prompt_many(program, q_t, cache_t, dim, mask):
     edges.prompt_many(program, q_t, cache_t, dim, mask, 1, 3)
+
+
+@combos
+def test_nothing_weighs(program, q_t, cache_t):
+    edges.nothing_weighs(program, q_t, cache_t)

@@ -83,3 +83,8 @@ def test_other_scales(program, q_t, cache_t, scale):
 def test_prompt_many(program, q_t, cache_t, dim, mask):
     import torch
     edges.prompt_many(program, q_t, cache_t, dim, mask, torch.cuda.get_device_properties(0).multi_processor_count, 70)
+
+
+@combos
+def test_nothing_weighs(program, q_t, cache_t):
+    edges.nothing_weighs(program, q_t, cache_t)

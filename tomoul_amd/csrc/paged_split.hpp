@@ -78,10 +78,12 @@ __device__ __forceinline__ float rescale(float m, float top) { return m == -INFI
 
 // Elements d and d + 1 of a head's output.
 __device__ __forceinline__ void store_result(int qt, const PagedAttentionArgs &a, int64_t b, int64_t head, int d, srv_f32x2 sum, float sum_l) {
-    const float r = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
+    // (nothing weighs: zeros, also where a value is infinite or NaN and so its sum is a NaN)
+    const bool none = sum_l == 0.0f;
+    const float r = 1.0f / sum_l;
     const int64_t to = b * a.out_stride + head * a.head_dim + d;
-    srv_store1(qt, a.out, to, sum[0] * r);
-    srv_store1(qt, a.out, to + 1, sum[1] * r);
+    srv_store1(qt, a.out, to, none ? 0.0f : sum[0] * r);
+    srv_store1(qt, a.out, to + 1, none ? 0.0f : sum[1] * r);
 }
 
 // A workgroup's way through its share.

@@ -680,7 +680,13 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
         }
     }
     const bool mine = row0 + 32 * wave + l32 < rows;
-    const float r = l == 0.0f ? 0.0f : 1.0f / l;
+    const bool none = l == 0.0f;  // nothing weighs: zeros, also where a value is infinite or NaN
+    const float r = none ? 0.0f : 1.0f / l;
+    if (__builtin_amdgcn_ballot_w64(none) != 0)
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = none ? 0.0f : o[t][i];
     const int64_t to = (first + token) * a.out_stride + head * D;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -722,7 +728,7 @@ __global__ __launch_bounds__(64 * kWaves * TEAMS, (Prompt<CT, QT, DP, FORM>::kTw
                 const int from = __builtin_ctzll(todo);
                 todo &= todo - 1;
                 const int64_t at = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(off >> 32), from) << 32) | (uint32_t)__shfl((int)(uint32_t)off, from));
-                const bool sees = mine && k0 + from >= low && k0 + from < high && l != 0.0f;
+                const bool sees = mine && k0 + from >= low && k0 + from < high && !none;
                 for (int i = 0; i < D / 2; ++i) {
                     const int d = 8 * (i / 4) + 4 * half + i % 4;
                     const float x = srv_load1(CT, (const char *)a.v_cache + at, d);
